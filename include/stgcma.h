@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define STG_VERSION 220
+#define STG_VERSION 221
 
 enum stg_act { STG_ACT_NONE_ = 0, STG_ACT_GELU_ = 1, STG_ACT_QUICKGELU_ = 2 };
 enum stg_dtype { STG_F32 = 0, STG_BF16 = 1, STG_FP8_MX = 2, STG_U8_LIN = 3 };
@@ -636,6 +636,91 @@ int stg_bn_colsum(const void* a, const void* b, const float* mean, const float* 
 int stg_bn_apply(const void* x, const float* mean, const float* rstd, const float* gamma, const float* beta, void* y, int64_t R, int C, void* stream);
 int stg_bn_bwd(const void* x, const void* dy, const float* mean, const float* rstd, const float* gamma, const float* sums, void* dx,
                int64_t R, int C, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Sequence operators (ABI 221; no counterpart in the reference): attention over ragged token sequences with a learned relative position
+ * bias by buckets, its single-token form over a key / value cache (csrc/relattn.hip), and the norm - gate - residual - norm join
+ * (csrc/normjoin.hip).
+ *
+ * x_ij = scale q_i.k_j + table[bucket(j - p_i)][h], p_i = i + (n_k - n_q) (the last query stands at the last key), P = softmax over the visible
+ * keys, O = P V.  A key is hidden by key_mask (byte 0) and, with `causal`, when j > p_i; a query that sees no key yields a zero row and lse -inf.
+ *   Q [Tq, H D], K / V [Tk, Hkv D] bf16 rows with leading dimensions in elements (multiples of 8; 16-byte aligned bases), head h at column h D,
+ *   query head h reads key / value head h / (H / Hkv).  D in {32, 64, 96, 128}.
+ *   cu_q / cu_k int32 [S + 1] on the device: sequence s owns rows cu[s] .. cu[s + 1] - 1 (cu[0] is taken as 0; offsets outside the tensors are
+ *   clamped, so no content of theirs makes a kernel leave its operands).  max_q / max_k: the longest sequences, on the host; they size the grid
+ *   only -- every row of a longer sequence is still computed.
+ *   table fp32 [num_buckets, H]; an entry at or below -1e30 (the type's lowest value too) hides its bucket's keys as -inf does.  plan int32 [2 far + 1 + half] on the device: the bucket of every distance -far .. far (distances beyond share
+ *   the ends), then the first distance of each of the `half` buckets of a side (half = num_buckets with `causal`, else num_buckets / 2, positive
+ *   distances then using the second half); every bucket is one run of distances and far = first distance of the last one, <= 2048.
+ *   lse fp32 [H, Tq] (natural logarithm; may be NULL in a forward without backward).  Olo bf16 [Tq, H D] or NULL: O's rounding error, which a
+ *   backward that wants the table's gradient reads (without it the gradient carries bf16's rounding of O).
+ *   Rows behind the last sequence are left as they were, or zeroed when zero_tail != 0 (by the backward too, in dQ, dK and dV).
+ */
+typedef struct {
+    const void* Q; int64_t ldq;
+    const void* K; int64_t ldk;
+    const void* V; int64_t ldv;
+    void* O; int64_t ldo;
+    void* Olo;
+    float* lse;
+    const int32_t* cu_q; const int32_t* cu_k;
+    const void* key_mask;             /* uint8 [Tk] or NULL */
+    int64_t Tq, Tk;                   /* rows of the tensors */
+    int S; int max_q; int max_k;
+    int H; int Hkv; int D;
+    float scale; int causal;
+    const float* table; const int32_t* plan;
+    int num_buckets; int far;
+    int zero_tail;
+} stg_relattn_args;
+int stg_relattn_fwd(const stg_relattn_args* a, void* stream);
+/* dQ / dK / dV written (not accumulated; shared heads summed over their group), dtable fp32 [num_buckets, H] written, or NULL.  `a` describes the
+ * forward (O, Olo and lse as it left them).  ws: fp32 scratch of stg_relattn_bwd_ws_floats(a, dtable != NULL) floats.  No atomics on memory: the
+ * same call gives the same bits. */
+int64_t stg_relattn_bwd_ws_floats(const stg_relattn_args* a, int want_table);
+int stg_relattn_bwd(const stg_relattn_args* a, const void* dO, int64_t lddo, void* dQ, int64_t lddq, void* dK, int64_t lddk, void* dV,
+                    int64_t lddv, float* dtable, float* ws, int64_t ws_floats, void* stream);
+/* One query per sequence over a cache: Q / O [S, H D]; K / V row t of sequence s at base + s * bs + t * ld; lens int32 [S] on the device (clamped
+ * to 0 .. cap): the query stands at position lens[s] - 1 and sees keys 0 .. lens[s] - 1; a sequence of length 0 yields a zero row. */
+typedef struct {
+    const void* Q; int64_t ldq;
+    const void* K; int64_t ldk; int64_t bsk;
+    const void* V; int64_t ldv; int64_t bsv;
+    void* O; int64_t ldo;
+    const int32_t* lens;
+    int S; int cap;
+    int H; int Hkv; int D;
+    float scale; int causal;
+    const float* table; const int32_t* plan;
+    int num_buckets; int far;
+} stg_relattn_decode_args;
+int64_t stg_relattn_decode_ws_floats(int S, int cap, int H, int Hkv, int D);
+int stg_relattn_decode(const stg_relattn_decode_args* a, float* ws, int64_t ws_floats, void* stream);
+
+/* n = Norm(h) w1 (+ b1); xo = alpha x + gate o n; y = Norm(xo) w2 (+ b2): the norm after a block, its gate, the scaled residual sum and the norm
+ * before the next block in one pass.  rms = 0: LayerNorm, 1: RMS norm (no mean), eps inside the square root.  x / xo in x_dtype (STG_F32 or
+ * STG_BF16; xo is rounded before the second norm reads it), h / y bf16, weights and gate fp32.  gate_kind 0: none (gate == NULL), 1: one value, 2:
+ * [C], 3: [ceil(rows / rows_per_group), C].  stats fp32 [rows, 4] (mean1, rstd1, mean2, rstd2) for the backward, or NULL.  C % 8 == 0, C <= 8192. */
+typedef struct {
+    const void* x; int64_t ldx; int x_dtype;
+    const void* h; int64_t ldh;
+    const float* gate; int gate_kind; int64_t rows_per_group;
+    const float* w1; const float* b1; const float* w2; const float* b2;
+    float alpha; float eps; int rms;
+    void* xo; int64_t ldxo;
+    void* y; int64_t ldy;
+    float* stats;
+    int64_t rows; int C;
+} stg_norm_join_args;
+int stg_norm_join_fwd(const stg_norm_join_args* a, void* stream);
+/* dy bf16 (gradient of y), dxo (gradient of xo from its other readers, x_dtype, or NULL = 0) -> dx (x_dtype), dh (bf16), and, unless NULL,
+ * dparams: fp32, dw1 [C], db1 [C] (if b1), dw2 [C], db2 [C] (if b2), dgate [C] (gate_kind 2) or one value (gate_kind 1), one after the other and
+ * padded to a multiple of 4; dgate_groups: fp32, the gate's gradient of gate_kind 3.  `a`: the forward's arguments (x and y are not read).  ws: fp32
+ * scratch of stg_norm_join_bwd_ws_floats(a) floats.  stg_norm_join_param_floats(a): floats of dparams before the padding. */
+int64_t stg_norm_join_param_floats(const stg_norm_join_args* a);
+int64_t stg_norm_join_bwd_ws_floats(const stg_norm_join_args* a);
+int stg_norm_join_bwd(const stg_norm_join_args* a, const void* dy, int64_t lddy, const void* dxo, int64_t lddxo, void* dx, int64_t lddx,
+                      void* dh, int64_t lddh, float* dparams, float* dgate_groups, float* ws, int64_t ws_floats, void* stream);
 
 #ifdef __cplusplus
 }

@@ -118,6 +118,25 @@ class AdamDesc(C.Structure):
     _fields_ = [("p", c_vp), ("g", c_vp), ("m", c_vp), ("v", c_vp), ("st", c_vp), ("n", c_i64), ("group", C.c_int), ("pad_", C.c_int)]
 
 
+class RelAttnArgs(C.Structure):
+    _fields_ = [("Q", c_vp), ("ldq", c_i64), ("K", c_vp), ("ldk", c_i64), ("V", c_vp), ("ldv", c_i64), ("O", c_vp), ("ldo", c_i64), ("Olo", c_vp),
+                ("lse", c_vp), ("cu_q", c_vp), ("cu_k", c_vp), ("key_mask", c_vp), ("Tq", c_i64), ("Tk", c_i64), ("S", C.c_int), ("max_q", C.c_int),
+                ("max_k", C.c_int), ("H", C.c_int), ("Hkv", C.c_int), ("D", C.c_int), ("scale", C.c_float), ("causal", C.c_int), ("table", c_vp),
+                ("plan", c_vp), ("num_buckets", C.c_int), ("far", C.c_int), ("zero_tail", C.c_int)]
+
+
+class RelAttnDecodeArgs(C.Structure):
+    _fields_ = [("Q", c_vp), ("ldq", c_i64), ("K", c_vp), ("ldk", c_i64), ("bsk", c_i64), ("V", c_vp), ("ldv", c_i64), ("bsv", c_i64), ("O", c_vp),
+                ("ldo", c_i64), ("lens", c_vp), ("S", C.c_int), ("cap", C.c_int), ("H", C.c_int), ("Hkv", C.c_int), ("D", C.c_int),
+                ("scale", C.c_float), ("causal", C.c_int), ("table", c_vp), ("plan", c_vp), ("num_buckets", C.c_int), ("far", C.c_int)]
+
+
+class NormJoinArgs(C.Structure):
+    _fields_ = [("x", c_vp), ("ldx", c_i64), ("x_dtype", C.c_int), ("h", c_vp), ("ldh", c_i64), ("gate", c_vp), ("gate_kind", C.c_int),
+                ("rows_per_group", c_i64), ("w1", c_vp), ("b1", c_vp), ("w2", c_vp), ("b2", c_vp), ("alpha", C.c_float), ("eps", C.c_float),
+                ("rms", C.c_int), ("xo", c_vp), ("ldxo", c_i64), ("y", c_vp), ("ldy", c_i64), ("stats", c_vp), ("rows", c_i64), ("C", C.c_int)]
+
+
 class TAttnArgs(C.Structure):
     _fields_ = [
         ("Q", c_vp), ("K", c_vp), ("V", c_vp), ("ld", c_i64),
@@ -240,10 +259,19 @@ SIGNATURES = {
     "stg_bn_colsum": (C.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, C.c_int, C.c_int, c_vp]),
     "stg_bn_apply": (C.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, C.c_int, c_vp]),
     "stg_bn_bwd": (C.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, C.c_int, c_vp]),
+    "stg_relattn_fwd": (C.c_int, [C.POINTER(RelAttnArgs), c_vp]),
+    "stg_relattn_bwd_ws_floats": (c_i64, [C.POINTER(RelAttnArgs), C.c_int]),
+    "stg_relattn_bwd": (C.c_int, [C.POINTER(RelAttnArgs), c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp]),
+    "stg_relattn_decode_ws_floats": (c_i64, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "stg_relattn_decode": (C.c_int, [C.POINTER(RelAttnDecodeArgs), c_vp, c_i64, c_vp]),
+    "stg_norm_join_fwd": (C.c_int, [C.POINTER(NormJoinArgs), c_vp]),
+    "stg_norm_join_param_floats": (c_i64, [C.POINTER(NormJoinArgs)]),
+    "stg_norm_join_bwd_ws_floats": (c_i64, [C.POINTER(NormJoinArgs)]),
+    "stg_norm_join_bwd": (C.c_int, [C.POINTER(NormJoinArgs), c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp]),
     "stg_vit_embed": (C.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, C.c_int, C.c_int, C.c_int, c_vp]),
 }
 
-ABI_VERSION = 220
+ABI_VERSION = 221
 _lib = None
 
 

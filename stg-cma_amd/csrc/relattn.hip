@@ -1,0 +1,1110 @@
+// Attention over ragged token sequences with a learned relative position bias by buckets: forward, backward (dQ, dK, dV and the
+// bias table's gradient) and the single-token form over a key / value cache.  The additive term depends on the signed distance
+// between key and query position alone, through a table of a few buckets per head (single distances near zero, then buckets evenly
+// spaced in the logarithm up to a border behind which every distance shares the last one), so it is never formed as [n, n]:
+//     x_ij = scale q_i . k_j + table[bucket(j - p_i)][h],  p_i = i + (n_k - n_q),   P = softmax(x),   O = P V.
+//
+// Sequence s owns query rows cu_q[s] .. cu_q[s+1] - 1 and key rows cu_k[s] .. cu_k[s+1] - 1 of packed row tensors; heads share
+// key / value heads (H % Hkv == 0); key_mask and the causal rule hide keys; a query that sees no key gives a zero row, lse = -inf
+// and no gradient.  Rows of masked keys and rows past a sequence's end enter LDS as zeros, so whatever they hold stays out.
+//
+// How the bias costs (almost) nothing: a block spreads its head's row of the table into LDS once, indexed by distance, divided by
+// the scale; a tile whose distances all lie behind the last border starts the score MFMA's accumulator at ONE constant, a nearer tile
+// starts it at 16 LDS words per lane (consecutive lanes read consecutive words).  Neither adds an instruction to the softmax.
+//
+// MFMA v_mfma_f32_32x32x16_bf16; lane l = (r = l & 31, hh = l >> 5); accumulator row (reg, hh) = (reg & 3) + 8 (reg >> 2) + 4 hh.
+#include <math.h>
+#include <float.h>
+#include "common.h"
+#include "../../include/stgcma.h"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int PAD = 96;               // a 64 x 32 tile that touches distance +-(far - 1) reaches at most 94 beyond it
+
+struct RP {
+    const bf16_t* Q; int64_t ldq;
+    const bf16_t* K; int64_t ldk;
+    const bf16_t* V; int64_t ldv;
+    bf16_t* O; int64_t ldo;
+    bf16_t* Olo;                      // [Tq, H D]: O - bf16(O), or NULL
+    float* lse;                       // [H, Tq], natural logarithm
+    const int32_t* cu_q; const int32_t* cu_k;
+    const uint8_t* kmask;
+    int64_t Tq, Tk;
+    int S, H, Hkv, causal, zero_tail;
+    const float* table; const int32_t* plan;
+    int NB, far;
+    float scale, scale2, inv_scale;
+    const bf16_t* dO; int64_t lddo;
+    bf16_t* dQ; int64_t lddq;
+    bf16_t* dK; int64_t lddk;
+    bf16_t* dV; int64_t lddv;
+    float* delta;                     // [H, Tq]
+    float* part;                      // [S * gridDim.x, H, NB] partial table gradients, or NULL
+};
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+#define MFMA32(a, b, c) __builtin_amdgcn_mfma_f32_32x32x16_bf16((a), (b), (c), 0, 0, 0)
+#define ACC_ROW(reg, hh) (((reg) & 3) + 8 * ((reg) >> 2) + 4 * (hh))
+
+__device__ __forceinline__ bf16x8_t ld_frag(const bf16_t* p) { return *reinterpret_cast<const bf16x8_t*>(p); }
+__device__ __forceinline__ f32x16_t splat16(float v) {
+    f32x16_t z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = v;
+    return z;
+}
+__device__ __forceinline__ bf16x8_t zero_frag() { const u32x4_t z = {0u, 0u, 0u, 0u}; return __builtin_bit_cast(bf16x8_t, z); }
+__device__ __forceinline__ bf16x8_t pack8(const float* x) {
+    const u32x4_t w = {pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7])};
+    return __builtin_bit_cast(bf16x8_t, w);
+}
+// bf16(x) and bf16(x - bf16(x)): the two together carry 16 bits of x
+__device__ __forceinline__ void pack8_split(const float* x, bf16x8_t& hi, bf16x8_t& lo) {
+    hi = pack8(x);
+    float d[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[i] = x[i] - bf2f((bf16_t)hi[i]);
+    lo = pack8(d);
+}
+// transposed fragment of a [rows][DP] tile: A[i = d][k slot j] = tile[16 s2 + 4 hh + (j & 3) + 8 (j >> 2)][32 dt + d]
+template <int DP>
+__device__ __forceinline__ bf16x8_t tr_frag(const bf16_t* s, int dt, int s2, int hh, int d) {
+    const int gi = d & 15, c = d >> 4;
+    const bf16_t* p = s + (16 * s2 + 4 * hh + (gi >> 2)) * DP + 32 * dt + 16 * c + 4 * (gi & 3);
+    const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)p);
+    const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)(p + 8 * DP));
+    bf16x8_t f;
+    f[0] = lo[0]; f[1] = lo[1]; f[2] = lo[2]; f[3] = lo[3];
+    f[4] = hi[0]; f[5] = hi[1]; f[6] = hi[2]; f[7] = hi[3];
+    return f;
+}
+template <int DP>
+__device__ __forceinline__ bf16x8_t nat_frag(const bf16_t* s, int r, int hh, int ks) {
+    return *reinterpret_cast<const bf16x8_t*>(s + r * DP + 16 * ks + 8 * hh);
+}
+
+struct Seq { int q0, nq, k0, nk; };
+// The offsets come from device memory: whatever they hold, the rows stay inside the tensors (sequence 0 starts at row 0).
+__device__ __forceinline__ Seq seq_of(const RP& a, int s) {
+    const int tq = (int)a.Tq, tk = (int)a.Tk;
+    auto clampi = [](int v, int hi) { return v < 0 ? 0 : (v > hi ? hi : v); };
+    Seq z;
+    z.q0 = s == 0 ? 0 : clampi(a.cu_q[s], tq);
+    z.nq = clampi(a.cu_q[s + 1], tq) - z.q0;
+    z.k0 = s == 0 ? 0 : clampi(a.cu_k[s], tk);
+    z.nk = clampi(a.cu_k[s + 1], tk) - z.k0;
+    z.nq = z.nq < 0 ? 0 : z.nq;
+    z.nk = z.nk < 0 ? 0 : z.nk;
+    return z;
+}
+
+// A table entry in units of the raw score.  Entries at or below -1e30 (the type's lowest value, a common mask) hide their bucket like -inf: as
+// scores they would swallow q.k in fp32 and leave rows that the log-sum-exp cannot describe.  Other finite entries are held within +-1e8,
+// where the row maximum's own rounding (2^-24 of it, common to the row) still cancels in the normalisation.
+__device__ __forceinline__ float raw_bias(float t, float inv_scale) {
+    if (t <= -1e30f) return -INFINITY;
+    if (t < -1e8f) t = -1e8f;
+    if (t > 1e8f && t < INFINITY) t = 1e8f;
+    return t * inv_scale;
+}
+// bv[i] = bias of distance i - (far + PAD); distances past the border hold its value
+__device__ __forceinline__ void fill_bias(const RP& a, int h, float* bv, int tid, int nthr) {
+    const int len = 2 * (a.far + PAD) + 1;
+    for (int i = tid; i < len; i += nthr) {
+        int d = i - (a.far + PAD);
+        d = d < -a.far ? -a.far : (d > a.far ? a.far : d);
+        int b = a.plan[d + a.far];
+        b = b < 0 ? 0 : (b < a.NB ? b : a.NB - 1);
+        bv[i] = raw_bias(a.table[(int64_t)b * a.H + h], a.inv_scale);
+    }
+}
+
+// Staging of two [64][D] tiles (K and V, or Q and dO) by NTHR threads in 16-byte pieces through registers.
+template <int N> using U4Arr = u32x4_t[N];
+template <int D, int NTHR> struct StageC {
+    static constexpr int ROWP = D / 8;                       // pieces per row
+    static constexpr int TOTAL = 2 * 64 * ROWP;
+    static constexpr int PER = (TOTAL + NTHR - 1) / NTHR;
+    static constexpr int DP = D + 8;                         // padded pitch: conflict-free for row-wise and transposed reads
+    static constexpr int TILE = 64 * DP;
+    static_assert(TOTAL % NTHR == 0, "every thread moves the same number of pieces");
+};
+template <int D, int NTHR>
+__device__ __forceinline__ void stage_fetch(U4Arr<StageC<D, NTHR>::PER>& v, int tid, const bf16_t* t0, int64_t ld0, const bf16_t* t1, int64_t ld1,
+                                            int row0, int n) {
+    using C = StageC<D, NTHR>;
+#pragma unroll
+    for (int i = 0; i < C::PER; ++i) {
+        const int id = tid + NTHR * i;
+        const int which = id / (64 * C::ROWP), rem = id - which * 64 * C::ROWP;
+        const int r = rem / C::ROWP, c = rem - r * C::ROWP;
+        int row = row0 + r;
+        row = row < n ? row : n - 1;
+        v[i] = *reinterpret_cast<const u32x4_t*>((which ? t1 + (int64_t)row * ld1 : t0 + (int64_t)row * ld0) + 8 * c);
+    }
+}
+// `valid`: bit r set = row r of the tile takes part; other rows are written as zeros
+template <int D, int NTHR>
+__device__ __forceinline__ void stage_commit(bf16_t* s, const U4Arr<StageC<D, NTHR>::PER>& v, int tid, uint64_t valid) {
+    using C = StageC<D, NTHR>;
+#pragma unroll
+    for (int i = 0; i < C::PER; ++i) {
+        const int id = tid + NTHR * i;
+        const int which = id / (64 * C::ROWP), rem = id - which * 64 * C::ROWP;
+        const int r = rem / C::ROWP, c = rem - r * C::ROWP;
+        u32x4_t w = v[i];
+        if (valid != ~0ull && !((valid >> r) & 1)) w = (u32x4_t){0u, 0u, 0u, 0u};
+        *reinterpret_cast<u32x4_t*>(s + which * C::TILE + r * C::DP + 8 * c) = w;
+    }
+}
+// bits of the 64 keys kb .. kb + 63 of a sequence that exist and are not masked (wave-uniform)
+__device__ __forceinline__ uint64_t key_bits(const RP& a, const Seq& z, int kb, int lane) {
+    bool ok = kb + lane < z.nk;
+    if (a.kmask != nullptr && ok) ok = a.kmask[(int64_t)z.k0 + kb + lane] != 0;
+    return __builtin_amdgcn_ballot_w64(ok);
+}
+// start of a score accumulator: bias of rows kb + ACC_ROW(., hh) against the lane's query position (idx = bv index of row 0, hh included)
+__device__ __forceinline__ f32x16_t bias16(const float* bv, int idx) {
+    f32x16_t c;
+#pragma unroll
+    for (int reg = 0; reg < 16; ++reg) c[reg] = bv[idx + (reg & 3) + 8 * (reg >> 2)];
+    return c;
+}
+
+// rows behind the last sequence: zeros (and lse = -inf), when the caller owns no content there
+__device__ __forceinline__ void zero_rows(bf16_t* t, int64_t ld, int64_t from, int64_t to, int col0, int D, int step, int off) {
+    const int per = D / 8;
+    for (int64_t i = off; i < (to - from) * per; i += step) {
+        const int64_t row = from + i / per;
+        *reinterpret_cast<u32x4_t*>(t + row * ld + col0 + 8 * (int)(i % per)) = (u32x4_t){0u, 0u, 0u, 0u};
+    }
+}
+__device__ __forceinline__ int64_t tail_start(const int32_t* cu, int S, int64_t T) {
+    const int64_t e = S > 0 ? cu[S] : 0;
+    return e < 0 ? 0 : (e > T ? T : e);
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+// A block = one (sequence, head) and 32 NW queries, 32 per wave; K / V in 64-key tiles, double-buffered in LDS, one barrier per tile.
+// Scores are computed transposed (rows = keys, lane = query): the softmax statistics are lane-local and P feeds the second MFMA from
+// registers.  LO: the product with V also takes bf16(P - bf16(P)), and O's rounding error is stored beside O: the backward's
+// delta = rowsum(dO O) is then good to 2^-16, which the table's gradient needs (its terms cancel row by row).
+template <int D, int NW, bool LO>
+__global__ void __launch_bounds__(NW * 64, 2) relattn_fwd_kernel(RP a) {
+    constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
+    using SC = StageC<D, NTHR>;
+    extern __shared__ __attribute__((aligned(16))) bf16_t smem[];       // two buffers x {K, V} x [64][DP], then the bias by distance
+    float* bv = reinterpret_cast<float*>(smem + 4 * SC::TILE);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = lane & 31, hh = lane >> 5;
+    const int h = blockIdx.y, hk = h / (a.H / a.Hkv);
+    if ((int)blockIdx.z == a.S) {                                       // the slice that clears the rows behind the last sequence
+        const int64_t from = tail_start(a.cu_q, a.S, a.Tq);
+        const int step = gridDim.x * NTHR, off = blockIdx.x * NTHR + tid;
+        zero_rows(a.O, a.ldo, from, a.Tq, h * D, D, step, off);
+        if (LO) zero_rows(a.Olo, (int64_t)a.H * D, from, a.Tq, h * D, D, step, off);
+        if (a.lse) for (int64_t i = from + off; i < a.Tq; i += step) a.lse[(int64_t)h * a.Tq + i] = -INFINITY;
+        return;
+    }
+    const Seq z = seq_of(a, blockIdx.z);
+    const int shift = z.nk - z.nq;
+    bool filled = false;
+    for (int64_t tile = blockIdx.x; tile * 32 * NW < z.nq; tile += gridDim.x) {
+        // heavy tiles first under the causal rule
+        const int nt = (z.nq + 32 * NW - 1) / (32 * NW);
+        const int qt = a.causal ? nt - 1 - (int)tile : (int)tile;
+        const int qw = 32 * (qt * NW + wave);                           // first query of the wave
+        const bool live = qw < z.nq;
+        const int q = qw + r;
+        const int64_t qrow = (int64_t)z.q0 + (q < z.nq ? q : z.nq - 1);
+        const int plo = qw + shift, phi = plo + 31, pos = plo + r;      // positions of the wave's queries
+        bf16x8_t qf[KS];
+        {
+            const bf16_t* qp = a.Q + qrow * a.ldq + h * D + 8 * hh;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) qf[s] = ld_frag(qp + 16 * s);
+        }
+        f32x16_t o[DT];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = splat16(0.f);
+        float m = -INFINITY, l = 0.f;
+
+        int kend = z.nk;                                                // keys any query of the block may see
+        if (a.causal) {
+            const int last = qt * 32 * NW + 32 * NW - 1 + shift + 1;
+            kend = kend < last ? kend : (last < 0 ? 0 : last);
+        }
+        const int np = (kend + 63) >> 6;
+        const bf16_t* Kb = a.K + (int64_t)z.k0 * a.ldk + hk * D;
+        const bf16_t* Vb = a.V + (int64_t)z.k0 * a.ldv + hk * D;
+        u32x4_t sv[SC::PER];
+        uint64_t bits = 0, nbits = 0;
+        if (np > 0) {
+            stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, 0, z.nk);
+            bits = key_bits(a, z, 0, lane);
+        }
+        if (!filled) { fill_bias(a, h, bv, tid, NTHR); filled = true; }
+        if (np > 0) stage_commit<D, NTHR>(smem, sv, tid, bits);
+        __syncthreads();
+        const float cleft = bv[0], cright = bv[2 * (a.far + PAD)];
+        for (int kp = 0; kp < np; ++kp) {
+            const bf16_t* sK = smem + (kp & 1) * 2 * SC::TILE;
+            const bf16_t* sV = sK + SC::TILE;
+            const int kb = 64 * kp;
+            if (kp + 1 < np) {
+                stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, kb + 64, z.nk);
+                nbits = key_bits(a, z, kb + 64, lane);
+            }
+            if (live && bits != 0 && !(a.causal && kb > phi)) {
+                f32x16_t sA, sB;                                        // St[key][q] of keys kb .. + 31 / + 32 .. + 63
+                if (kb + 63 - plo <= -a.far) { sA = splat16(cleft); sB = sA; }
+                else if (kb - phi >= a.far) { sA = splat16(cright); sB = sA; }
+                else {
+                    const int idx = kb + 4 * hh - pos + a.far + PAD;
+                    sA = bias16(bv, idx);
+                    sB = bias16(bv, idx + 32);
+                }
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    sA = MFMA32(nat_frag<DP>(sK, r, hh, s), qf[s], sA);
+                    sB = MFMA32(nat_frag<DP>(sK + 32 * DP, r, hh, s), qf[s], sB);
+                }
+                float xA[16], xB[16];
+                const bool edge = bits != ~0ull || (a.causal && kb + 63 > plo);
+                if (edge) {
+                    uint64_t vis = bits;                                // keys this lane's query may see
+                    if (a.causal) {
+                        const int c = pos - kb;                         // last visible key of the tile
+                        vis = c < 0 ? 0 : (c >= 63 ? vis : vis & ((2ull << c) - 1));
+                    }
+                    vis >>= 4 * hh;
+#pragma unroll
+                    for (int reg = 0; reg < 16; ++reg) {
+                        xA[reg] = (vis >> ACC_ROW(reg, 0)) & 1 ? sA[reg] : -INFINITY;
+                        xB[reg] = (vis >> (32 + ACC_ROW(reg, 0))) & 1 ? sB[reg] : -INFINITY;
+                    }
+                } else {
+#pragma unroll
+                    for (int reg = 0; reg < 16; ++reg) { xA[reg] = sA[reg]; xB[reg] = sB[reg]; }
+                }
+                float mr = -INFINITY;                                   // the maximum on the raw scores (scale > 0)
+#pragma unroll
+                for (int reg = 0; reg < 16; ++reg) mr = fmaxf(mr, fmaxf(xA[reg], xB[reg]));
+                mr = fmaxf(mr, __shfl_xor(mr, 32, 64));
+                const float mx = fmaxf(m, mr * a.scale2);
+                const float nm = mx == -INFINITY ? 0.f : -mx;           // nothing seen so far: every exponent is -inf
+                const float alpha = __builtin_amdgcn_exp2f(m + nm);
+                m = mx;
+                float ls = 0.f;
+#pragma unroll
+                for (int reg = 0; reg < 16; ++reg) {
+                    xA[reg] = __builtin_amdgcn_exp2f(fmaf(xA[reg], a.scale2, nm));
+                    xB[reg] = __builtin_amdgcn_exp2f(fmaf(xB[reg], a.scale2, nm));
+                    ls += xA[reg] + xB[reg];
+                }
+                ls += __shfl_xor(ls, 32, 64);
+                l = l * alpha + ls;
+                if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {  // rescale only when some query's maximum moved
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int reg = 0; reg < 16; ++reg) o[dt][reg] *= alpha;
+                }
+                bf16x8_t pf[4], pl[4];
+                if (LO) {
+                    pack8_split(xA, pf[0], pl[0]); pack8_split(xA + 8, pf[1], pl[1]);
+                    pack8_split(xB, pf[2], pl[2]); pack8_split(xB + 8, pf[3], pl[3]);
+                } else {
+                    pf[0] = pack8(xA); pf[1] = pack8(xA + 8); pf[2] = pack8(xB); pf[3] = pack8(xB + 8);
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bf16x8_t vf = tr_frag<DP>(sV, dt, i, hh, r);
+                        o[dt] = MFMA32(vf, pf[i], o[dt]);
+                        if (LO) o[dt] = MFMA32(vf, pl[i], o[dt]);
+                    }
+            }
+            if (kp + 1 < np) stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, nbits);
+            bits = nbits;
+            __syncthreads();
+        }
+        {
+            const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+            const bool ok = q < z.nq;
+            const int64_t row = (int64_t)z.q0 + q;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                if (l == 0.f) o[dt] = splat16(0.f);
+                store_tile32(a.O + row * a.ldo + h * D + 32 * dt, o[dt], inv, hh, ok);
+                if (LO) {
+                    f32x16_t e;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) { const float f = o[dt][i] * inv; e[i] = f - bf2f(f2bf(f)); }
+                    store_tile32(a.Olo + row * ((int64_t)a.H * D) + h * D + 32 * dt, e, 1.0f, hh, ok);
+                }
+            }
+            if (ok && a.lse && hh == 0) a.lse[(int64_t)h * a.Tq + row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
+        }
+        __syncthreads();                                                // the next tile of this block refills the first buffer
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dQ, delta, table gradient
+// The forward's tiling with P recomputed from lse: dS = P (dO V^T - delta), dQ = scale dS K.  TAB: dS is also summed along the diagonals
+// of the score matrix (one distance each) with LDS additions into an array that belongs to the wave alone -- instructions of one wave
+// stay in order, so the sums do not depend on timing -- and behind the last border in two registers; each block leaves its sums by
+// bucket in its own row of `part`, which relattn_dtable_kernel adds up in a fixed order.
+template <int D, int NW, bool TAB>
+__global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
+    constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
+    using SC = StageC<D, NTHR>;
+    extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
+    const int blen = 2 * (a.far + PAD) + 1;
+    float* bv = reinterpret_cast<float*>(smem + 4 * SC::TILE);
+    float* diag = bv + blen;                                            // [NW][blen]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = lane & 31, hh = lane >> 5;
+    const int h = blockIdx.y, hk = h / (a.H / a.Hkv);
+    if ((int)blockIdx.z == a.S) {
+        const int64_t from = tail_start(a.cu_q, a.S, a.Tq);
+        zero_rows(a.dQ, a.lddq, from, a.Tq, h * D, D, gridDim.x * NTHR, blockIdx.x * NTHR + tid);
+        return;
+    }
+    const Seq z = seq_of(a, blockIdx.z);
+    const int shift = z.nk - z.nq;
+    fill_bias(a, h, bv, tid, NTHR);
+    float* mine = diag + wave * blen;
+    if (TAB)
+        for (int i = tid; i < NW * blen; i += NTHR) diag[i] = 0.f;
+    float far_l = 0.f, far_r = 0.f;
+    __syncthreads();
+    const float cleft = bv[0], cright = bv[blen - 1];
+    for (int64_t tile = blockIdx.x; tile * 32 * NW < z.nq; tile += gridDim.x) {
+        const int nt = (z.nq + 32 * NW - 1) / (32 * NW);
+        const int qt = a.causal ? nt - 1 - (int)tile : (int)tile;
+        const int qw = 32 * (qt * NW + wave);
+        const bool live = qw < z.nq;
+        const int q = qw + r;
+        const bool qok = q < z.nq;
+        const int64_t qrow = (int64_t)z.q0 + (qok ? q : z.nq - 1);
+        const int plo = qw + shift, phi = plo + 31, pos = plo + r;
+        bf16x8_t qf[KS], df[KS];
+        float delta = 0.f;
+        {
+            const bf16_t* qp = a.Q + qrow * a.ldq + h * D + 8 * hh;
+            const bf16_t* dp = a.dO + qrow * a.lddo + h * D + 8 * hh;
+            const bf16_t* op = a.O + qrow * a.ldo + h * D + 8 * hh;
+            const bf16_t* lp = a.Olo + qrow * ((int64_t)a.H * D) + h * D + 8 * hh;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                qf[s] = ld_frag(qp + 16 * s);
+                df[s] = ld_frag(dp + 16 * s);
+                const bf16x8_t of = ld_frag(op + 16 * s);
+                const bf16x8_t lf = a.Olo ? ld_frag(lp + 16 * s) : zero_frag();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) delta += bf2f((bf16_t)df[s][j]) * (bf2f((bf16_t)of[j]) + bf2f((bf16_t)lf[j]));
+            }
+        }
+        delta += __shfl_xor(delta, 32, 64);
+        const float lse = a.lse[(int64_t)h * a.Tq + qrow];
+        const bool seen = qok && lse != -INFINITY;                      // a row that saw no key has no gradient
+        const float nl = seen ? -lse * LOG2E : -INFINITY;
+        if (!seen) delta = 0.f;
+        if (qok && hh == 0) a.delta[(int64_t)h * a.Tq + qrow] = delta;
+        f32x16_t dq[DT];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) dq[dt] = splat16(0.f);
+        int kend = z.nk;
+        if (a.causal) {
+            const int last = qt * 32 * NW + 32 * NW - 1 + shift + 1;
+            kend = kend < last ? kend : (last < 0 ? 0 : last);
+        }
+        const int np = (kend + 63) >> 6;
+        const bf16_t* Kb = a.K + (int64_t)z.k0 * a.ldk + hk * D;
+        const bf16_t* Vb = a.V + (int64_t)z.k0 * a.ldv + hk * D;
+        u32x4_t sv[SC::PER];
+        uint64_t bits = 0, nbits = 0;
+        if (np > 0) {
+            stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, 0, z.nk);
+            bits = key_bits(a, z, 0, lane);
+            stage_commit<D, NTHR>(smem, sv, tid, bits);
+        }
+        __syncthreads();
+        for (int kp = 0; kp < np; ++kp) {
+            const bf16_t* sK = smem + (kp & 1) * 2 * SC::TILE;
+            const bf16_t* sV = sK + SC::TILE;
+            const int kb = 64 * kp;
+            if (kp + 1 < np) {
+                stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, kb + 64, z.nk);
+                nbits = key_bits(a, z, kb + 64, lane);
+            }
+            if (live && bits != 0 && !(a.causal && kb > phi)) {
+                const bool left = kb + 63 - plo <= -a.far, right = kb - phi >= a.far;
+                const int idx0 = kb + 4 * hh - pos + a.far + PAD;
+                uint64_t vis = bits;
+                if (a.causal) {
+                    const int c = pos - kb;
+                    vis = c < 0 ? 0 : (c >= 63 ? vis : vis & ((2ull << c) - 1));
+                }
+                vis >>= 4 * hh;
+                const bool edge = bits != ~0ull || (a.causal && kb + 63 > plo);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {                  // the two 32-key tiles, one after the other (register budget)
+                    const bf16_t* tK = sK + half * 32 * DP;
+                    const bf16_t* tV = sV + half * 32 * DP;
+                    const int idx = idx0 + 32 * half;
+                    f32x16_t sc = left ? splat16(cleft) : (right ? splat16(cright) : bias16(bv, idx));
+                    f32x16_t dp = splat16(-delta);                      // dP - delta: the MFMA's accumulator starts there
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        sc = MFMA32(nat_frag<DP>(tK, r, hh, s), qf[s], sc);
+                        dp = MFMA32(nat_frag<DP>(tV, r, hh, s), df[s], dp);
+                    }
+                    float ds[16];
+#pragma unroll
+                    for (int reg = 0; reg < 16; ++reg) {
+                        ds[reg] = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nl)) * dp[reg];
+                        if (edge) ds[reg] = (vis >> (32 * half + ACC_ROW(reg, 0))) & 1 ? ds[reg] : 0.f;
+                    }
+                    if (TAB) {
+                        if (left || right) {
+                            float t = 0.f;
+#pragma unroll
+                            for (int reg = 0; reg < 16; ++reg) t += ds[reg];
+                            if (left) far_l += t; else far_r += t;
+                        } else {
+#pragma unroll
+                            for (int reg = 0; reg < 16; ++reg)
+                                __hip_atomic_fetch_add(mine + idx + ACC_ROW(reg, 0), ds[reg], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                        }
+                    }
+                    const bf16x8_t d0 = pack8(ds), d1 = pack8(ds + 8);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 0, hh, r), d0, dq[dt]);
+                        dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 1, hh, r), d1, dq[dt]);
+                    }
+                }
+            }
+            if (kp + 1 < np) stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, nbits);
+            bits = nbits;
+            __syncthreads();
+        }
+        bf16_t* dqp = a.dQ + ((int64_t)z.q0 + q) * a.lddq + h * D;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) store_tile32(dqp + 32 * dt, dq[dt], a.scale, hh, qok);
+        __syncthreads();
+    }
+    if (TAB) {
+        far_l = wave_sum<64>(far_l);
+        far_r = wave_sum<64>(far_r);
+        if (lane == 0) { mine[0] += far_l; mine[blen - 1] += far_r; }   // ends of the array: distances behind the border
+        __syncthreads();
+        for (int i = tid; i < blen; i += NTHR) {
+            float t = 0.f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) t += diag[w * blen + i];
+            diag[i] = t;
+        }
+        __syncthreads();
+        // a bucket is one run of distances (the last of a side runs to the array's end): first distances in plan[2 far + 1 ..]
+        const int32_t* border = a.plan + 2 * a.far + 1;
+        const int half = a.causal ? a.NB : a.NB / 2;
+        float* out = a.part + (((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * a.H + h) * a.NB;
+        for (int b = wave; b < a.NB; b += NW) {
+            const int side = b >= half, i = side ? b - half : b;
+            int lo = border[i], hi = i + 1 < half ? border[i + 1] : a.far + PAD + 1;
+            if (side && lo == 0) lo = 1;                                // distance 0 belongs to the first side
+            lo = lo < 0 ? 0 : lo;
+            hi = hi < a.far + PAD + 1 ? hi : a.far + PAD + 1;
+            float t = 0.f;
+            for (int d = lo + lane; d < hi; d += 64) t += diag[a.far + PAD + (side ? d : -d)];
+            t = wave_sum<64>(t);
+            if (lane == 0) out[b] = t;
+        }
+    }
+}
+
+// dtable[b][h] = sum over the blocks' rows, in order
+__global__ void __launch_bounds__(256) relattn_dtable_kernel(const float* part, float* dtable, int rows, int H, int NB) {
+    __shared__ float s[256];
+    const int h = blockIdx.x, b = blockIdx.y;
+    float t = 0.f;
+    for (int i = threadIdx.x; i < rows; i += 256) t += part[((int64_t)i * H + h) * NB + b];
+    s[threadIdx.x] = t;
+    __syncthreads();
+    for (int w = 128; w > 0; w >>= 1) {
+        if ((int)threadIdx.x < w) s[threadIdx.x] += s[threadIdx.x + w];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) dtable[(int64_t)b * H + h] = s[0];
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dK, dV
+// A block = one (sequence, key / value head) and 32 NW keys, 32 per wave; it walks the queries of every head of the group in 64-row tiles
+// of Q and dO, so the gradients of a shared head are summed in registers, in one order.  S[q][key]: rows = queries, lane = key.
+template <int D, int NW>
+__global__ void __launch_bounds__(NW * 64, 1) relattn_dkv_kernel(RP a) {
+    constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
+    using SC = StageC<D, NTHR>;
+    constexpr int BUF = 2 * SC::TILE + 256;                             // Q and dO tiles + 128 floats of statistics
+    extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
+    float* bv = reinterpret_cast<float*>(smem + 2 * BUF);
+    const int blen = 2 * (a.far + PAD) + 1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = lane & 31, hh = lane >> 5;
+    const int hk = blockIdx.y, rep = a.H / a.Hkv;
+    if ((int)blockIdx.z == a.S) {
+        const int64_t from = tail_start(a.cu_k, a.S, a.Tk);
+        const int step = gridDim.x * NTHR, off = blockIdx.x * NTHR + tid;
+        zero_rows(a.dK, a.lddk, from, a.Tk, hk * D, D, step, off);
+        zero_rows(a.dV, a.lddv, from, a.Tk, hk * D, D, step, off);
+        return;
+    }
+    const Seq z = seq_of(a, blockIdx.z);
+    const int shift = z.nk - z.nq;
+    for (int64_t tile = blockIdx.x; tile * 32 * NW < z.nk; tile += gridDim.x) {
+        const int kw = 32 * ((int)tile * NW + wave);
+        const int key = kw + r;
+        bool kok = key < z.nk;
+        const int64_t krow = (int64_t)z.k0 + (kok ? key : z.nk - 1);
+        const bool stored = kok;
+        if (a.kmask != nullptr && kok) kok = a.kmask[krow] != 0;
+        const bool live = __builtin_amdgcn_ballot_w64(kok) != 0;
+        bf16x8_t kf[KS], vf[KS];
+        {
+            const bf16_t* kp = a.K + krow * a.ldk + hk * D + 8 * hh;
+            const bf16_t* vp = a.V + krow * a.ldv + hk * D + 8 * hh;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                kf[s] = ld_frag(kp + 16 * s);
+                vf[s] = ld_frag(vp + 16 * s);
+                if (!kok) { kf[s] = zero_frag(); vf[s] = zero_frag(); }
+            }
+        }
+        f32x16_t dk[DT], dv[DT];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) { dk[dt] = splat16(0.f); dv[dt] = splat16(0.f); }
+        // first query that may see the block's first key
+        int qfirst = a.causal ? (int)tile * 32 * NW - shift : 0;
+        qfirst = qfirst < 0 ? 0 : qfirst;
+        const int p0 = qfirst >> 6, np = (z.nq + 63) >> 6;
+        for (int g = 0; g < rep && p0 < np; ++g) {
+            const int h = hk * rep + g;
+            const bf16_t* Qb = a.Q + (int64_t)z.q0 * a.ldq + h * D;
+            const bf16_t* Db = a.dO + (int64_t)z.q0 * a.lddo + h * D;
+            const float* lseb = a.lse + (int64_t)h * a.Tq + z.q0;
+            const float* delb = a.delta + (int64_t)h * a.Tq + z.q0;
+            u32x4_t sv[SC::PER];
+            float nl = 0.f, nd = 0.f;
+            auto fetch_all = [&](int q0) {
+                stage_fetch<D, NTHR>(sv, tid, Qb, a.ldq, Db, a.lddo, q0, z.nq);
+                if (tid < 64) {
+                    const int qi = q0 + tid;
+                    nl = qi < z.nq ? lseb[qi] : -INFINITY;
+                    nd = qi < z.nq ? -delb[qi] : 0.f;
+                    nl = nl == -INFINITY ? -INFINITY : -nl * LOG2E;     // a row that saw nothing, or none at all: P = 0
+                }
+            };
+            auto commit_all = [&](bf16_t* buf, int q0) {
+                const int left = z.nq - q0;
+                stage_commit<D, NTHR>(buf, sv, tid, left >= 64 ? ~0ull : (1ull << left) - 1);
+                float* st = reinterpret_cast<float*>(buf + 2 * SC::TILE);
+                if (tid < 64) { st[tid] = nl; st[64 + tid] = nd; }
+            };
+            fetch_all(64 * p0);
+            fill_bias(a, h, bv, tid, NTHR);
+            commit_all(smem + (p0 & 1) * BUF, 64 * p0);
+            __syncthreads();
+            const float cleft = bv[0], cright = bv[blen - 1];
+            for (int qp = p0; qp < np; ++qp) {
+                const bf16_t* sQ = smem + (qp & 1) * BUF;
+                const bf16_t* sD = sQ + SC::TILE;
+                const float* sL = reinterpret_cast<const float*>(sQ + 2 * SC::TILE);
+                if (qp + 1 < np) fetch_all(64 * (qp + 1));
+                const int pb = 64 * qp + shift;                         // position of the tile's first query
+                if (live && !(a.causal && pb + 63 < kw)) {
+                    const bool left = kw + 31 - pb <= -a.far, right = kw - (pb + 63) >= a.far;
+                    const bool edge = a.causal && kw + 31 > pb;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const bf16_t* tQ = sQ + half * 32 * DP;
+                        const bf16_t* tD = sD + half * 32 * DP;
+                        const int rel = key - (pb + 32 * half) - 4 * hh;    // distance of accumulator row 0
+                        f32x16_t sc, dp;
+                        if (left) sc = splat16(cleft);
+                        else if (right) sc = splat16(cright);
+                        else {
+                            const float* bp = bv + rel + a.far + PAD;
+#pragma unroll
+                            for (int reg = 0; reg < 16; ++reg) sc[reg] = bp[-ACC_ROW(reg, 0)];
+                        }
+                        float lv[16];
+#pragma unroll
+                        for (int g4 = 0; g4 < 4; ++g4) {
+                            const float4 ls = *reinterpret_cast<const float4*>(sL + 32 * half + 8 * g4 + 4 * hh);
+                            const float4 de = *reinterpret_cast<const float4*>(sL + 64 + 32 * half + 8 * g4 + 4 * hh);
+                            lv[4 * g4] = ls.x; lv[4 * g4 + 1] = ls.y; lv[4 * g4 + 2] = ls.z; lv[4 * g4 + 3] = ls.w;
+                            dp[4 * g4] = de.x; dp[4 * g4 + 1] = de.y; dp[4 * g4 + 2] = de.z; dp[4 * g4 + 3] = de.w;
+                        }
+#pragma unroll
+                        for (int s = 0; s < KS; ++s) {
+                            sc = MFMA32(nat_frag<DP>(tQ, r, hh, s), kf[s], sc);
+                            dp = MFMA32(nat_frag<DP>(tD, r, hh, s), vf[s], dp);
+                        }
+                        float pr[16], ds[16];
+#pragma unroll
+                        for (int reg = 0; reg < 16; ++reg) {
+                            float p = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, lv[reg]));
+                            if (edge) p = rel <= ACC_ROW(reg, 0) ? p : 0.f;     // hidden by the causal rule (and so is dS, whatever dP holds)
+                            pr[reg] = p;
+                            ds[reg] = edge && rel > ACC_ROW(reg, 0) ? 0.f : p * dp[reg];
+                        }
+                        const bf16x8_t a0 = pack8(pr), a1 = pack8(pr + 8), d0 = pack8(ds), d1 = pack8(ds + 8);
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) {
+                            dv[dt] = MFMA32(tr_frag<DP>(tD, dt, 0, hh, r), a0, dv[dt]);
+                            dv[dt] = MFMA32(tr_frag<DP>(tD, dt, 1, hh, r), a1, dv[dt]);
+                            dk[dt] = MFMA32(tr_frag<DP>(tQ, dt, 0, hh, r), d0, dk[dt]);
+                            dk[dt] = MFMA32(tr_frag<DP>(tQ, dt, 1, hh, r), d1, dk[dt]);
+                        }
+                    }
+                }
+                if (qp + 1 < np) commit_all(smem + ((qp + 1) & 1) * BUF, 64 * (qp + 1));
+                __syncthreads();
+            }
+        }
+        bf16_t* kp = a.dK + ((int64_t)z.k0 + key) * a.lddk + hk * D;
+        bf16_t* vp = a.dV + ((int64_t)z.k0 + key) * a.lddv + hk * D;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            if (!kok) { dk[dt] = splat16(0.f); dv[dt] = splat16(0.f); }     // a masked key has no gradient
+            store_tile32(kp + 32 * dt, dk[dt], a.scale, hh, stored);
+            store_tile32(vp + 32 * dt, dv[dt], 1.0f, hh, stored);
+        }
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ one new token per sequence
+struct DP_ {
+    const bf16_t* Q; int64_t ldq;
+    const bf16_t* K; int64_t ldk, bsk;
+    const bf16_t* V; int64_t ldv, bsv;
+    bf16_t* O; int64_t ldo;
+    const int32_t* lens;
+    int S, cap, H, Hkv;
+    const float* table; const int32_t* plan;
+    int NB, far, causal;
+    float scale2, inv_scale;
+    int chunk, nsplit;
+    float* po;                        // [S, nsplit, H, D] partial outputs (normalised by their own sum)
+    float* pl;                        // [S, nsplit, H] log2-domain lse of the part, -inf when empty
+};
+
+// A block = `chunk` keys of one (sequence, key / value head) against all query heads of the group: the heads are the 32 columns of the
+// MFMA (unused columns are zero), so a key or value row is read once whatever the group's size.  Each of the four waves walks its own
+// 32-key tiles with its own LDS tile (no barrier in the loop), the next tile's 16-byte pieces in flight meanwhile; the waves' statistics
+// meet in LDS at the end.  Bound by the bytes of K and V.
+template <int D>
+__global__ void __launch_bounds__(256, 2) relattn_decode_kernel(DP_ a) {
+    constexpr int KS = D / 16, DT = D / 32, DP = D + 8, ROWP = D / 8, PER = 2 * 32 * ROWP / 64, TILE = 32 * DP;
+    extern __shared__ __attribute__((aligned(16))) bf16_t smem[];       // per wave {K, V} x [32][DP]; then bias [far + 1][32]: see host
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = lane & 31, hh = lane >> 5;
+    const int rep = a.H / a.Hkv, ncg = (rep + 31) / 32;
+    const int hk = blockIdx.y / ncg, cg = blockIdx.y - hk * ncg;
+    const int ncol = rep - 32 * cg < 32 ? rep - 32 * cg : 32;
+    const int h0 = hk * rep + 32 * cg;                                  // head of column 0
+    const int s = blockIdx.z, sp = blockIdx.x;
+    int len = a.lens[s];
+    len = len < 0 ? 0 : (len > a.cap ? a.cap : len);
+    const int k0 = sp * a.chunk, k1 = k0 + a.chunk < len ? k0 + a.chunk : len;
+    if (k0 >= len && sp > 0) return;                                    // the combining pass knows which parts exist
+    const int pos = len - 1;
+    const bf16_t* Kb = a.K + (int64_t)s * a.bsk + hk * D;
+    const bf16_t* Vb = a.V + (int64_t)s * a.bsv + hk * D;
+    bf16_t* sK = smem + wave * 2 * TILE;
+    bf16_t* sV = sK + TILE;
+    float* sb = reinterpret_cast<float*>(smem + 8 * TILE);              // [NB][32] table columns in raw score units
+    const bool col = r < ncol;
+    u32x4_t sv[PER];
+    auto fetch = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int id = lane + 64 * i;
+            const int which = id / (32 * ROWP), rem = id - which * 32 * ROWP;
+            const int rr = rem / ROWP, c = rem - rr * ROWP;
+            int row = kb + rr;
+            row = row < k1 ? row : k1 - 1;
+            sv[i] = *reinterpret_cast<const u32x4_t*>((which ? Vb + (int64_t)row * a.ldv : Kb + (int64_t)row * a.ldk) + 8 * c);
+        }
+    };
+    int kb = k0 + 32 * wave;
+    if (kb < k1) fetch(kb);
+    for (int i = tid; i < a.NB * 32; i += 256) {
+        const int b = i >> 5, c = i & 31;
+        float v = 0.f;
+        if (c < ncol) v = raw_bias(a.table[(int64_t)b * a.H + h0 + c], a.inv_scale);
+        sb[i] = v;
+    }
+    bf16x8_t qf[KS];
+    {
+        const bf16_t* qp = a.Q + (int64_t)s * a.ldq + (int64_t)(h0 + (col ? r : 0)) * D + 8 * hh;
+#pragma unroll
+        for (int t = 0; t < KS; ++t) { qf[t] = ld_frag(qp + 16 * t); if (!col) qf[t] = zero_frag(); }
+    }
+    const int32_t* map = a.plan + a.far;                                // map[d], d = key - pos in [-far, 0]
+    auto row_of = [&](int d) { const int b = map[d]; return b < 0 ? 0 : (b < a.NB ? b : a.NB - 1); };
+    f32x16_t o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = splat16(0.f);
+    float m = -INFINITY, l = 0.f;
+    __syncthreads();
+    const float cleft = sb[row_of(-a.far) * 32 + r];
+    for (; kb < k1; kb += 128) {
+        const bool tail = kb + 32 > k1;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int id = lane + 64 * i;
+            const int which = id / (32 * ROWP), rem = id - which * 32 * ROWP;
+            const int rr = rem / ROWP, c = rem - rr * ROWP;
+            u32x4_t w = sv[i];
+            if (tail && kb + rr >= k1) w = (u32x4_t){0u, 0u, 0u, 0u};
+            *reinterpret_cast<u32x4_t*>(sK + which * TILE + rr * DP + 8 * c) = w;
+        }
+        const bool near = kb + 31 - pos > -a.far;
+        f32x16_t sc = splat16(cleft);
+        if (near) {
+#pragma unroll
+            for (int reg = 0; reg < 16; ++reg) {
+                int d = kb + ACC_ROW(reg, hh) - pos;
+                d = d > 0 ? 0 : (d < -a.far ? -a.far : d);
+                sc[reg] = sb[row_of(d) * 32 + r];
+            }
+        }
+        if (kb + 128 < k1) fetch(kb + 128);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");          // the wave's own LDS tile: its instructions stay in order
+#pragma unroll
+        for (int t = 0; t < KS; ++t) sc = MFMA32(nat_frag<DP>(sK, r, hh, t), qf[t], sc);
+        float x[16];
+        float mr = -INFINITY;
+#pragma unroll
+        for (int reg = 0; reg < 16; ++reg) {
+            x[reg] = tail && kb + ACC_ROW(reg, hh) >= k1 ? -INFINITY : sc[reg];
+            mr = fmaxf(mr, x[reg]);
+        }
+        mr = fmaxf(mr, __shfl_xor(mr, 32, 64));
+        const float mx = fmaxf(m, mr * a.scale2);
+        const float nm = mx == -INFINITY ? 0.f : -mx;
+        const float alpha = __builtin_amdgcn_exp2f(m + nm);
+        m = mx;
+        float ls = 0.f;
+#pragma unroll
+        for (int reg = 0; reg < 16; ++reg) {
+            x[reg] = __builtin_amdgcn_exp2f(fmaf(x[reg], a.scale2, nm));
+            ls += x[reg];
+        }
+        ls += __shfl_xor(ls, 32, 64);
+        l = l * alpha + ls;
+        if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int reg = 0; reg < 16; ++reg) o[dt][reg] *= alpha;
+        }
+        const bf16x8_t p0 = pack8(x), p1 = pack8(x + 8);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            o[dt] = MFMA32(tr_frag<DP>(sV, dt, 0, hh, r), p0, o[dt]);
+            o[dt] = MFMA32(tr_frag<DP>(sV, dt, 1, hh, r), p1, o[dt]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    // ---- the four waves meet: statistics, then the scaled outputs, one wave's after the other's so that the sum has one order
+    __syncthreads();
+    float* st = reinterpret_cast<float*>(smem);                         // [4][32] maxima, [4][32] sums, then [D][32] outputs
+    float* so = st + 256;
+    if (hh == 0) { st[32 * wave + r] = m; st[128 + 32 * wave + r] = l; }
+    __syncthreads();
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, st[32 * w + r]);
+    const float nM = M == -INFINITY ? 0.f : -M;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) L += st[128 + 32 * w + r] * __builtin_amdgcn_exp2f(st[32 * w + r] + nM);
+    const float f = __builtin_amdgcn_exp2f(m + nM);
+    for (int w = 0; w < 4; ++w) {
+        if (wave == w) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int reg = 0; reg < 16; ++reg) {
+                    const int d = 32 * dt + ACC_ROW(reg, hh);
+                    const float v = f == 0.f ? 0.f : o[dt][reg] * f;
+                    so[d * 33 + r] = w == 0 ? v : so[d * 33 + r] + v;
+                }
+        }
+        __syncthreads();
+    }
+    if (wave == 0 && hh == 0) st[r] = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
+    if (wave == 1 && hh == 0 && col && a.nsplit > 1)
+        a.pl[((int64_t)s * a.nsplit + sp) * a.H + h0 + r] = L == 0.f ? -INFINITY : M + __log2f(L);
+    __syncthreads();
+    for (int i = tid; i < ncol * D; i += 256) {
+        const int c = i / D, d = i - c * D;
+        const float v = so[d * 33 + c] * st[c];
+        if (a.nsplit == 1) a.O[(int64_t)s * a.ldo + (int64_t)(h0 + c) * D + d] = f2bf(v);
+        else a.po[(((int64_t)s * a.nsplit + sp) * a.H + h0 + c) * D + d] = v;
+    }
+}
+
+// joins the parts of a sequence: O = sum_p 2^(lse_p - M) O_p / sum_p 2^(lse_p - M); one wave per (sequence, head), parts in order
+template <int D>
+__global__ void __launch_bounds__(256) relattn_parts_kernel(DP_ a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= (int64_t)a.S * a.H) return;
+    const int s = (int)(item / a.H), h = (int)(item - (int64_t)s * a.H);
+    int len = a.lens[s];
+    len = len < 0 ? 0 : (len > a.cap ? a.cap : len);
+    const int np = len == 0 ? 1 : (len + a.chunk - 1) / a.chunk;
+    const float* pl = a.pl + ((int64_t)s * a.nsplit) * a.H + h;
+    float M = -INFINITY;
+    for (int p = lane; p < np; p += 64) M = fmaxf(M, pl[(int64_t)p * a.H]);
+    M = wave_max<64>(M);
+    const float nM = M == -INFINITY ? 0.f : -M;
+    float w = 0.f, acc[(D + 63) / 64] = {};
+    for (int p = 0; p < np; ++p) {
+        const float e = __builtin_amdgcn_exp2f(pl[(int64_t)p * a.H] + nM);
+        w += e;
+        if (e == 0.f) continue;
+        const float* po = a.po + (((int64_t)s * a.nsplit + p) * a.H + h) * D;
+#pragma unroll
+        for (int i = 0; i < (D + 63) / 64; ++i)
+            if (lane + 64 * i < D) acc[i] = fmaf(e, po[lane + 64 * i], acc[i]);
+    }
+    const float inv = w == 0.f ? 0.f : 1.0f / w;
+#pragma unroll
+    for (int i = 0; i < (D + 63) / 64; ++i)
+        if (lane + 64 * i < D) a.O[(int64_t)s * a.ldo + (int64_t)h * D + lane + 64 * i] = f2bf(acc[i] * inv);
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+constexpr int MAX_FAR = 2048, MAX_NB = 256;      // the widest bias arrays (155 KB with the tiles at head dim 128) fit the 160 KB of LDS
+
+bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
+
+int check_bias(const char* who, const float* table, const int32_t* plan, int NB, int far, int causal, float scale) {
+    STG_CHECK(table && plan, -1, "%s: null table / plan", who);
+    STG_CHECK(NB >= (causal ? 2 : 4) && NB <= MAX_NB && (causal || NB % 2 == 0), -2, "%s: %d buckets (2..%d, even and >= 4 without the causal rule)", who, NB, MAX_NB);
+    STG_CHECK(far >= 1 && far <= MAX_FAR, -2, "%s: the last bucket starts at distance %d (1..%d)", who, far, MAX_FAR);
+    STG_CHECK(scale > 0.f && scale < 1e10f && scale > 1e-10f, -2, "%s: scale %g (1e-10 .. 1e10)", who, scale);
+    return 0;
+}
+
+int check_args(const char* who, const stg_relattn_args* a) {
+    STG_CHECK(a != nullptr, -1, "%s: null arguments", who);
+    STG_CHECK(a->S >= 0 && a->S < 65535 && a->Tq >= 0 && a->Tk >= 0 && a->Tq <= INT32_MAX - 1024 && a->Tk <= INT32_MAX - 1024, -2,
+              "%s: S=%d (< 65535), Tq=%lld, Tk=%lld (< 2^31 - 1024)", who, a->S, (long long)a->Tq, (long long)a->Tk);
+    STG_CHECK((a->Tq == 0 || (a->Q && a->O)) && (a->Tk == 0 || (a->K && a->V)) && a->cu_q && a->cu_k, -1, "%s: null tensor", who);
+    STG_CHECK(a->D == 32 || a->D == 64 || a->D == 96 || a->D == 128, -2, "%s: head dim %d (32, 64, 96 or 128)", who, a->D);
+    STG_CHECK(a->H > 0 && a->H <= 65535 && a->Hkv > 0 && a->H % a->Hkv == 0, -2, "%s: %d heads over %d key / value heads", who, a->H, a->Hkv);
+    STG_CHECK(a->max_q >= 0 && a->max_k >= 0, -2, "%s: max_q=%d, max_k=%d", who, a->max_q, a->max_k);
+    const int64_t hd = (int64_t)a->H * a->D, kd = (int64_t)a->Hkv * a->D;
+    STG_CHECK(a->ldq >= hd && a->ldo >= hd && a->ldk >= kd && a->ldv >= kd && a->ldq % 8 == 0 && a->ldk % 8 == 0 && a->ldv % 8 == 0 && a->ldo % 8 == 0, -3,
+              "%s: leading dimensions must be multiples of 8 and hold every head", who);
+    STG_CHECK(!misaligned(a->Q) && !misaligned(a->K) && !misaligned(a->V) && !misaligned(a->O) && !misaligned(a->Olo), -3, "%s: tensors must be 16-byte aligned", who);
+    return check_bias(who, a->table, a->plan, a->num_buckets, a->far, a->causal, a->scale);
+}
+
+RP make_rp(const stg_relattn_args* a) {
+    RP p{};
+    p.Q = (const bf16_t*)a->Q; p.ldq = a->ldq;
+    p.K = (const bf16_t*)a->K; p.ldk = a->ldk;
+    p.V = (const bf16_t*)a->V; p.ldv = a->ldv;
+    p.O = (bf16_t*)a->O; p.ldo = a->ldo;
+    p.Olo = (bf16_t*)a->Olo;
+    p.lse = a->lse;
+    p.cu_q = a->cu_q; p.cu_k = a->cu_k; p.kmask = (const uint8_t*)a->key_mask;
+    p.Tq = a->Tq; p.Tk = a->Tk; p.S = a->S; p.H = a->H; p.Hkv = a->Hkv; p.causal = a->causal != 0; p.zero_tail = a->zero_tail != 0;
+    p.table = a->table; p.plan = a->plan; p.NB = a->num_buckets; p.far = a->far;
+    p.scale = a->scale; p.scale2 = a->scale * LOG2E; p.inv_scale = 1.0f / a->scale;
+    return p;
+}
+
+int64_t lds_fwd(int D, int far) { return (int64_t)4 * 64 * (D + 8) * 2 + (2 * (far + PAD) + 1) * 4; }
+int64_t lds_dq(int D, int far, bool tab) { return (int64_t)4 * 64 * (D + 8) * 2 + (2 * (far + PAD) + 1) * 4 * (tab ? 5 : 1); }
+int64_t lds_dkv(int D, int far) { return (int64_t)2 * (2 * 64 * (D + 8) + 256) * 2 + (2 * (far + PAD) + 1) * 4; }
+int64_t lds_dec(int D, int NB) { return (int64_t)8 * 32 * (D + 8) * 2 + (int64_t)NB * 32 * 4; }
+
+int grid_tiles(int max_n, int64_t T, int rows) {
+    int64_t n = max_n > 0 ? max_n : 1;
+    n = n < T ? n : (T > 0 ? T : 1);
+    const int64_t t = (n + rows - 1) / rows;
+    return (int)(t < 1 ? 1 : t);
+}
+
+template <int D, bool LO>
+int launch_fwd(const RP& p, int max_q, hipStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    auto k = relattn_fwd_kernel<D, 4, LO>;
+    STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_fwd: cannot reserve LDS");
+    const dim3 grid(grid_tiles(max_q, p.Tq, 128), p.H, p.S + (p.zero_tail ? 1 : 0));
+    if (grid.z == 0) return 0;
+    k<<<grid, 256, lds_fwd(D, p.far), st>>>(p);
+    STG_LAUNCH_CHECK();
+    return 0;
+}
+template <int D, bool TAB>
+int launch_dq(const RP& p, int max_q, hipStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    auto k = relattn_dq_kernel<D, 4, TAB>;
+    STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_bwd: cannot reserve LDS");
+    const dim3 grid(grid_tiles(max_q, p.Tq, 128), p.H, p.S + (p.zero_tail ? 1 : 0));
+    if (grid.z == 0) return 0;
+    k<<<grid, 256, lds_dq(D, p.far, TAB), st>>>(p);
+    STG_LAUNCH_CHECK();
+    return 0;
+}
+template <int D>
+int launch_dkv(const RP& p, int max_k, hipStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    auto k = relattn_dkv_kernel<D, 4>;
+    STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_bwd: cannot reserve LDS");
+    const dim3 grid(grid_tiles(max_k, p.Tk, 128), p.Hkv, p.S + (p.zero_tail ? 1 : 0));
+    if (grid.z == 0) return 0;
+    k<<<grid, 256, lds_dkv(D, p.far), st>>>(p);
+    STG_LAUNCH_CHECK();
+    return 0;
+}
+template <int D>
+int launch_decode(const DP_& p, hipStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    auto k = relattn_decode_kernel<D>;
+    STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_decode: cannot reserve LDS");
+    const int ncg = (p.H / p.Hkv + 31) / 32;
+    k<<<dim3(p.nsplit, p.Hkv * ncg, p.S), 256, lds_dec(D, p.NB), st>>>(p);
+    STG_LAUNCH_CHECK();
+    if (p.nsplit > 1) {
+        relattn_parts_kernel<D><<<dim3((unsigned)(((int64_t)p.S * p.H + 3) / 4)), 256, 0, st>>>(p);
+        STG_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+#define BY_DIM(D_, CALL)                                             \
+    switch (D_) {                                                    \
+        case 32: { constexpr int DIM = 32; return CALL; }            \
+        case 64: { constexpr int DIM = 64; return CALL; }            \
+        case 96: { constexpr int DIM = 96; return CALL; }            \
+        default: { constexpr int DIM = 128; return CALL; }           \
+    }
+
+int run_fwd(const RP& p, int D, int max_q, hipStream_t st) {
+    if (p.Olo) BY_DIM(D, (launch_fwd<DIM, true>(p, max_q, st)));
+    BY_DIM(D, (launch_fwd<DIM, false>(p, max_q, st)));
+}
+int run_dq(const RP& p, int D, int max_q, hipStream_t st) {
+    if (p.part) BY_DIM(D, (launch_dq<DIM, true>(p, max_q, st)));
+    BY_DIM(D, (launch_dq<DIM, false>(p, max_q, st)));
+}
+int run_dkv(const RP& p, int D, int max_k, hipStream_t st) { BY_DIM(D, (launch_dkv<DIM>(p, max_k, st))); }
+int run_decode(const DP_& p, int D, hipStream_t st) { BY_DIM(D, (launch_decode<DIM>(p, st))); }
+
+// keys per block of the single-token form: enough blocks for the chip, at least 128 keys (one 32-key tile for each of the four waves)
+int decode_chunk(int S, int Hkv, int rep, int cap) {
+    const int64_t groups = (int64_t)S * Hkv * ((rep + 31) / 32);
+    const int64_t total = groups * cap;
+    int64_t c = (total / 1024 + 127) / 128 * 128;
+    c = c < 128 ? 128 : (c > 1024 ? 1024 : c);
+    while ((cap + c - 1) / c > 4096) c *= 2;
+    return (int)c;
+}
+
+}  // namespace
+
+extern "C" int stg_relattn_fwd(const stg_relattn_args* a, void* stream) {
+    const int rc = check_args("stg_relattn_fwd", a);
+    if (rc) return rc;
+    if (a->Tq == 0) return 0;
+    return run_fwd(make_rp(a), a->D, a->max_q, (hipStream_t)stream);
+}
+
+extern "C" int64_t stg_relattn_bwd_ws_floats(const stg_relattn_args* a, int want_table) {
+    if (a == nullptr || a->S < 0 || a->H <= 0 || a->Tq < 0 || a->num_buckets <= 0) return -1;
+    int64_t n = (int64_t)a->H * a->Tq;
+    if (want_table) n += (int64_t)grid_tiles(a->max_q, a->Tq, 128) * a->S * a->H * a->num_buckets;
+    return n > 0 ? n : 1;
+}
+
+extern "C" int stg_relattn_bwd(const stg_relattn_args* a, const void* dO, int64_t lddo, void* dQ, int64_t lddq, void* dK, int64_t lddk, void* dV,
+                               int64_t lddv, float* dtable, float* ws, int64_t ws_floats, void* stream) {
+    const int rc = check_args("stg_relattn_bwd", a);
+    if (rc) return rc;
+    const int64_t hd = (int64_t)a->H * a->D, kd = (int64_t)a->Hkv * a->D;
+    STG_CHECK((a->Tq == 0 || (dO && dQ && a->lse)) && (a->Tk == 0 || (dK && dV)) && ws, -1, "stg_relattn_bwd: null tensor");
+    STG_CHECK(lddo >= hd && lddq >= hd && lddk >= kd && lddv >= kd && lddo % 8 == 0 && lddq % 8 == 0 && lddk % 8 == 0 && lddv % 8 == 0, -3,
+              "stg_relattn_bwd: leading dimensions must be multiples of 8 and hold every head");
+    STG_CHECK(!misaligned(dO) && !misaligned(dQ) && !misaligned(dK) && !misaligned(dV), -3, "stg_relattn_bwd: tensors must be 16-byte aligned");
+    STG_CHECK(ws_floats >= stg_relattn_bwd_ws_floats(a, dtable != nullptr), -4, "stg_relattn_bwd: workspace of %lld floats is too small", (long long)ws_floats);
+    hipStream_t st = (hipStream_t)stream;
+    RP p = make_rp(a);
+    p.dO = (const bf16_t*)dO; p.lddo = lddo; p.dQ = (bf16_t*)dQ; p.lddq = lddq;
+    p.dK = (bf16_t*)dK; p.lddk = lddk; p.dV = (bf16_t*)dV; p.lddv = lddv;
+    p.delta = ws;
+    p.part = dtable ? ws + (int64_t)a->H * a->Tq : nullptr;
+    if (a->Tq > 0) { const int e = run_dq(p, a->D, a->max_q, st); if (e) return e; }
+    if (a->Tk > 0) { const int e = run_dkv(p, a->D, a->max_k, st); if (e) return e; }
+    if (dtable) {
+        const int rows = a->Tq > 0 ? grid_tiles(a->max_q, a->Tq, 128) * a->S : 0;
+        relattn_dtable_kernel<<<dim3(a->H, a->num_buckets), 256, 0, st>>>(p.part, dtable, rows, a->H, a->num_buckets);
+        STG_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+extern "C" int64_t stg_relattn_decode_ws_floats(int S, int cap, int H, int Hkv, int D) {
+    if (S <= 0 || cap <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || D <= 0) return 0;
+    const int c = decode_chunk(S, Hkv, H / Hkv, cap);
+    const int64_t ns = (cap + c - 1) / c;
+    return ns > 1 ? (int64_t)S * ns * H * (D + 1) : 0;
+}
+
+extern "C" int stg_relattn_decode(const stg_relattn_decode_args* a, float* ws, int64_t ws_floats, void* stream) {
+    STG_CHECK(a != nullptr, -1, "stg_relattn_decode: null arguments");
+    STG_CHECK(a->S >= 0 && a->S <= 65535 && a->cap >= 0 && a->cap <= INT32_MAX - 1024, -2, "stg_relattn_decode: S=%d (<= 65535), cap=%d", a->S, a->cap);
+    STG_CHECK(a->D == 32 || a->D == 64 || a->D == 96 || a->D == 128, -2, "stg_relattn_decode: head dim %d (32, 64, 96 or 128)", a->D);
+    STG_CHECK(a->H > 0 && a->H <= 32768 && a->Hkv > 0 && a->H % a->Hkv == 0, -2, "stg_relattn_decode: %d heads over %d key / value heads", a->H, a->Hkv);
+    STG_CHECK(a->Q && a->O && a->lens && (a->cap == 0 || (a->K && a->V)), -1, "stg_relattn_decode: null tensor");
+    const int64_t hd = (int64_t)a->H * a->D, kd = (int64_t)a->Hkv * a->D;
+    STG_CHECK(a->ldq >= hd && a->ldo >= hd && a->ldk >= kd && a->ldv >= kd && a->ldq % 8 == 0 && a->ldk % 8 == 0 && a->ldv % 8 == 0 && a->bsk % 8 == 0 &&
+              a->bsv % 8 == 0 && a->bsk >= 0 && a->bsv >= 0, -3, "stg_relattn_decode: strides must be multiples of 8 and hold every head");
+    STG_CHECK(!misaligned(a->Q) && !misaligned(a->K) && !misaligned(a->V), -3, "stg_relattn_decode: tensors must be 16-byte aligned");
+    const int rc = check_bias("stg_relattn_decode", a->table, a->plan, a->num_buckets, a->far, a->causal, a->scale);
+    if (rc) return rc;
+    if (a->S == 0) return 0;
+    DP_ p{};
+    p.Q = (const bf16_t*)a->Q; p.ldq = a->ldq;
+    p.K = (const bf16_t*)a->K; p.ldk = a->ldk; p.bsk = a->bsk;
+    p.V = (const bf16_t*)a->V; p.ldv = a->ldv; p.bsv = a->bsv;
+    p.O = (bf16_t*)a->O; p.ldo = a->ldo;
+    p.lens = a->lens; p.S = a->S; p.cap = a->cap; p.H = a->H; p.Hkv = a->Hkv;
+    p.table = a->table; p.plan = a->plan; p.NB = a->num_buckets; p.far = a->far; p.causal = a->causal != 0;
+    p.scale2 = a->scale * LOG2E; p.inv_scale = 1.0f / a->scale;
+    const int cap1 = a->cap > 0 ? a->cap : 1;
+    p.chunk = decode_chunk(a->S, a->Hkv, a->H / a->Hkv, cap1);
+    p.nsplit = (cap1 + p.chunk - 1) / p.chunk;
+    const int64_t need = stg_relattn_decode_ws_floats(a->S, a->cap, a->H, a->Hkv, a->D);
+    STG_CHECK(need == 0 || (ws != nullptr && ws_floats >= need), -4, "stg_relattn_decode: workspace of %lld floats is too small", (long long)ws_floats);
+    p.po = ws;
+    p.pl = ws ? ws + (int64_t)a->S * p.nsplit * a->H * a->D : nullptr;
+    return run_decode(p, a->D, (hipStream_t)stream);
+}

@@ -3,6 +3,7 @@
 Every wrapper validates shapes/dtypes/devices on the host before the launch -- a kernel must never see an operand whose
 extent differs from what its grid assumes.  PyTorch supplies device memory and the stream only.
 """
+import bisect
 import ctypes as C
 
 import torch
@@ -2118,3 +2119,295 @@ def ln_param_grad(dy, x, mean, rstd, dgamma, dbeta):
     R, Cc = x.shape
     _chk1d(mean, "mean", F32, R); _chk1d(rstd, "rstd", F32, R); _chk1d(dgamma, "dgamma", F32, Cc); _chk1d(dbeta, "dbeta", F32, Cc)
     _lib.check(_lib.lib().stg_ln_param_grad(_p(dy), _p(x), _p(mean), _p(rstd), _p(dgamma), _p(dbeta), R, Cc, _stream()), "stg_ln_param_grad")
+
+
+# ------------------------------------------------------------------------------------------------ sequence operators (relattn.hip, normjoin.hip)
+
+def rel_bucket_borders(num_buckets, max_distance, causal):
+    """First distance of each bucket of one side: single distances up to half of the side's buckets, then borders evenly spaced in the
+    logarithm up to max_distance -- bucket t of n holds the distances d with (d / first)^n >= (max_distance / first)^t, decided with whole
+    numbers, so a distance on a border never depends on a rounding.  Borders that fall together leave buckets without any distance."""
+    half = int(num_buckets) if causal else int(num_buckets) // 2
+    first = half // 2
+    if num_buckets != int(num_buckets) or first < 1 or (not causal and num_buckets % 2) or num_buckets > 256:
+        raise ValueError(f"rel_bucket_borders: {num_buckets} buckets (causal: 2..256, else 4..256 and even)")
+    n = half - first
+    if max_distance != int(max_distance) or max_distance <= first:
+        raise ValueError(f"rel_bucket_borders: max_distance={max_distance} must be a whole number above {first}")
+    far = int(max_distance)
+    out = list(range(first))
+    for t in range(n):
+        lo, hi = first, far                                   # smallest d with d^n first^t >= far^t first^n
+        want = far ** t * first ** n
+        while lo < hi:
+            mid = (lo + hi) // 2
+            if mid ** n * first ** t >= want:
+                hi = mid
+            else:
+                lo = mid + 1
+        out.append(lo)
+    return out
+
+
+class RelGeom:
+    """Geometry of relattn_fwd / relattn_bwd / relattn_decode: H query heads over kv_heads key / value heads of width D, and the learned
+    relative position bias (table [num_buckets, H]).  Without `causal` half of the buckets serve keys before the query (and at it), half keys
+    behind it.  scale defaults to D ** -0.5.  The bucket of every distance is kept on each device that uses it (built here for `device`, the
+    current one by default, or at the first call from another)."""
+
+    def __init__(self, H, D, *, kv_heads=None, num_buckets=32, max_distance=128, causal=False, scale=None, device=None):
+        self.H, self.D, self.Hkv = int(H), int(D), int(H if kv_heads is None else kv_heads)
+        if self.D not in (32, 64, 96, 128):
+            raise RuntimeError(f"RelGeom: head dim {D} (32, 64, 96 or 128)")
+        if self.H < 1 or self.Hkv < 1 or self.H % self.Hkv:
+            raise RuntimeError(f"RelGeom: {H} query heads over {kv_heads} key / value heads")
+        self.causal, self.num_buckets = bool(causal), int(num_buckets)
+        self.scale = float(self.D ** -0.5 if scale is None else scale)
+        if not 1e-10 < self.scale < 1e10:
+            raise RuntimeError(f"RelGeom: scale {scale} must be positive")
+        self.borders = rel_bucket_borders(num_buckets, max_distance, causal)
+        self.far = max(1, self.borders[-1])                   # every distance from here on shares the last bucket
+        if self.far > 2048:
+            raise RuntimeError(f"RelGeom: the last bucket starts at distance {self.far} (at most 2048)")
+        self._plans = {}
+        if device is not None or torch.cuda.is_available():
+            self.plan(torch.device("cuda" if device is None else device))
+
+    def bucket(self, distance):
+        """Bucket of a signed distance (key position - query position)."""
+        b = bisect.bisect_right(self.borders, abs(distance)) - 1
+        return b + (self.num_buckets // 2 if distance > 0 and not self.causal else 0)
+
+    def plan(self, device):
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        p = self._plans.get(device)
+        if p is None:
+            ids = [self.bucket(d if not self.causal else min(d, 0)) for d in range(-self.far, self.far + 1)]
+            p = self._plans[device] = torch.tensor(ids + self.borders, dtype=torch.int32, device=device)
+        return p
+
+
+def _rel_chk(t, name, dtype, cols, dev, rows=None):
+    _chk2d(t, name, dtype)
+    if t.device != dev:
+        raise RuntimeError(f"{name}: on {t.device}, expected {dev}")
+    if t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
+        raise RuntimeError(f"{name}: expected {'any number of' if rows is None else rows} rows x {cols} columns, got {tuple(t.shape)}")
+    if _ld(t) % 8 or t.data_ptr() % 16:
+        raise RuntimeError(f"{name}: rows must start 16-byte aligned (leading dimension {_ld(t)}, a multiple of 8)")
+
+
+def _rel_int32(t, name, n, dev):
+    if t.device != dev or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n) or t.shape[0] < 1:
+        raise RuntimeError(f"{name}: expected a contiguous int32 vector{'' if n is None else f' of {n}'} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _rel_table(g, table, dev):
+    if table.device != dev or table.dtype != F32 or tuple(table.shape) != (g.num_buckets, g.H) or not table.is_contiguous():
+        raise RuntimeError(f"table: expected contiguous fp32 [{g.num_buckets}, {g.H}] on {dev}, got {table.dtype} {tuple(table.shape)} on {table.device}")
+
+
+def _rel_fill(g, q, k, v, o, olo, lse, table, cu_q, cu_k, max_q, max_k, key_mask):
+    dev = q.device
+    _rel_chk(q, "q", BF16, g.H * g.D, dev)
+    _rel_chk(k, "k", BF16, g.Hkv * g.D, dev)
+    _rel_chk(v, "v", BF16, g.Hkv * g.D, dev, rows=k.shape[0])
+    _rel_chk(o, "o", BF16, g.H * g.D, dev, rows=q.shape[0])
+    _rel_table(g, table, dev)
+    self_attn = cu_k is None or cu_k is cu_q
+    cu_k = cu_q if cu_k is None else cu_k
+    _rel_int32(cu_q, "cu_q", None, dev)
+    _rel_int32(cu_k, "cu_k", cu_q.shape[0], dev)
+    max_q = q.shape[0] if max_q is None else int(max_q)
+    max_k = (max_q if self_attn else k.shape[0]) if max_k is None else int(max_k)
+    if max_q < 0 or max_k < 0:
+        raise RuntimeError(f"relattn: max_q={max_q}, max_k={max_k}")
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.dim() != 1 or key_mask.shape[0] != k.shape[0] or not key_mask.is_contiguous() or key_mask.device != dev:
+            raise RuntimeError(f"key_mask: expected a contiguous bool / uint8 vector of {k.shape[0]} on {dev}, got {key_mask.dtype} {tuple(key_mask.shape)}")
+    if lse is not None and (lse.dtype != F32 or tuple(lse.shape) != (g.H, q.shape[0]) or not lse.is_contiguous() or lse.device != dev):
+        raise RuntimeError(f"lse: expected contiguous fp32 [{g.H}, {q.shape[0]}]")
+    if olo is not None and (olo.dtype != BF16 or tuple(olo.shape) != (q.shape[0], g.H * g.D) or not olo.is_contiguous() or olo.device != dev):
+        raise RuntimeError(f"olo: expected contiguous bf16 [{q.shape[0]}, {g.H * g.D}]")
+    a = _lib.RelAttnArgs()
+    a.Q, a.ldq, a.K, a.ldk, a.V, a.ldv, a.O, a.ldo = _p(q), _ld(q), _p(k), _ld(k), _p(v), _ld(v), _p(o), _ld(o)
+    a.Olo, a.lse, a.cu_q, a.cu_k, a.key_mask = _p(olo), _p(lse), _p(cu_q), _p(cu_k), _p(key_mask)
+    a.Tq, a.Tk, a.S, a.max_q, a.max_k = q.shape[0], k.shape[0], cu_q.shape[0] - 1, min(max_q, q.shape[0]), min(max_k, k.shape[0])
+    a.H, a.Hkv, a.D, a.scale, a.causal = g.H, g.Hkv, g.D, g.scale, int(g.causal)
+    a.plan, a.num_buckets, a.far = _p(g.plan(dev)), g.num_buckets, g.far
+    a.table = _p(table)
+    return a
+
+
+def relattn_fwd(g, q, k, v, table, cu_q, cu_k=None, *, max_q=None, max_k=None, key_mask=None, out=None, want_lse=True, want_olo=False):
+    """Attention over ragged sequences with a learned relative position bias by buckets (stg_relattn_fwd).
+
+    q bf16 [Tq, H * D], k / v bf16 [Tk, Hkv * D] (column slices of a fused projection are fine); table fp32 [num_buckets, H] (an
+    entry at or below -1e30 hides its bucket like -inf); cu_q / cu_k int32
+    [S + 1] on the device: sequence s owns rows cu[s] .. cu[s + 1] - 1 (cu_k = None: cu_q); max_q / max_k: the longest sequences, known on the host
+    (they size the launch; without them the whole tensor is assumed).  key_mask bool [Tk]: False hides a key.  The last query of a sequence stands
+    at its last key.  Returns (o bf16 [Tq, H * D], lse fp32 [H, Tq] or None), and with want_olo a third: the rounding error of o that relattn_bwd
+    wants for the table's gradient.  Rows behind the last sequence are zero in a fresh output and left alone in `out`."""
+    o = torch.empty((q.shape[0], g.H * g.D), dtype=BF16, device=q.device) if out is None else out
+    lse = torch.empty((g.H, q.shape[0]), dtype=F32, device=q.device) if want_lse else None
+    olo = torch.empty((q.shape[0], g.H * g.D), dtype=BF16, device=q.device) if want_olo else None
+    a = _rel_fill(g, q, k, v, o, olo, lse, table, cu_q, cu_k, max_q, max_k, key_mask)
+    a.zero_tail = int(out is None)
+    _lib.check(_lib.lib().stg_relattn_fwd(C.byref(a), _stream()), "stg_relattn_fwd")
+    return (o, lse, olo) if want_olo else (o, lse)
+
+
+def relattn_bwd(g, q, k, v, table, cu_q, cu_k, o, lse, do, *, olo=None, max_q=None, max_k=None, key_mask=None, want_table=True):
+    """(dq, dk, dv, dtable or None) of relattn_fwd (stg_relattn_bwd): the probabilities are recomputed from lse, shared key / value heads summed
+    over their group, dtable fp32.  Gradient rows behind the last sequence are zero."""
+    if lse is None:
+        raise RuntimeError("relattn_bwd: needs the forward's lse")
+    a = _rel_fill(g, q, k, v, o, olo, lse, table, cu_q, cu_k, max_q, max_k, key_mask)
+    _rel_chk(do, "do", BF16, g.H * g.D, q.device, rows=q.shape[0])
+    dq = torch.empty((q.shape[0], g.H * g.D), dtype=BF16, device=q.device)
+    dk = torch.empty((k.shape[0], g.Hkv * g.D), dtype=BF16, device=q.device)
+    dv = torch.empty_like(dk)
+    dtable = torch.empty_like(table) if want_table else None
+    a.zero_tail = 1
+    n = _lib.lib().stg_relattn_bwd_ws_floats(C.byref(a), int(want_table))
+    ws = torch.empty((max(n, 1),), dtype=F32, device=q.device)
+    _lib.check(_lib.lib().stg_relattn_bwd(C.byref(a), _p(do), _ld(do), _p(dq), _ld(dq), _p(dk), _ld(dk), _p(dv), _ld(dv), _p(dtable), _p(ws), ws.numel(),
+                                          _stream()), "stg_relattn_bwd")
+    return dq, dk, dv, dtable
+
+
+def relattn_decode(g, q, k_cache, v_cache, table, lens, out=None):
+    """One new token per sequence over a key / value cache (stg_relattn_decode): q bf16 [S, H * D]; k_cache / v_cache bf16 [S, cap, Hkv * D] (any
+    row and sequence strides that are multiples of 8, so a larger cache's slice is fine), the new token's own key and value already in
+    place; lens int32 [S] on the device: tokens in the cache, the new one included.  Returns o bf16 [S, H * D] (zero where lens is 0)."""
+    S, dev = q.shape[0], q.device
+    _rel_chk(q, "q", BF16, g.H * g.D, dev)
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if not t.is_cuda or t.dtype != BF16 or t.dim() != 3 or t.shape[0] != S or t.shape[2] != g.Hkv * g.D or t.device != dev or t.shape[1] != k_cache.shape[1]:
+            raise RuntimeError(f"{name}: expected bf16 [{S}, cap, {g.Hkv * g.D}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and (t.stride(1) % 8 or t.stride(1) < t.shape[2])) or (S > 1 and t.stride(0) % 8)
+                          or t.data_ptr() % 16):
+            raise RuntimeError(f"{name}: rows must be contiguous and start 16-byte aligned, strides {t.stride()}")
+    _rel_table(g, table, dev)
+    _rel_int32(lens, "lens", S, dev) if S else None
+    if out is None:
+        out = torch.empty((S, g.H * g.D), dtype=BF16, device=dev)
+    _rel_chk(out, "out", BF16, g.H * g.D, dev, rows=S)
+    if S == 0:
+        return out
+    a = _lib.RelAttnDecodeArgs()
+    cap = k_cache.shape[1]
+    a.Q, a.ldq, a.O, a.ldo = _p(q), _ld(q), _p(out), _ld(out)
+    for t, ptr, ld, bs in ((k_cache, "K", "ldk", "bsk"), (v_cache, "V", "ldv", "bsv")):
+        setattr(a, ptr, _p(t))
+        setattr(a, ld, t.stride(1) if cap > 1 else g.Hkv * g.D)
+        setattr(a, bs, t.stride(0) if S > 1 else 0)
+    a.lens, a.S, a.cap, a.H, a.Hkv, a.D, a.scale, a.causal = _p(lens), S, cap, g.H, g.Hkv, g.D, g.scale, int(g.causal)
+    a.plan, a.num_buckets, a.far = _p(g.plan(dev)), g.num_buckets, g.far
+    a.table = _p(table)
+    n = _lib.lib().stg_relattn_decode_ws_floats(S, cap, g.H, g.Hkv, g.D)
+    ws = torch.empty((n,), dtype=F32, device=dev) if n else None
+    _lib.check(_lib.lib().stg_relattn_decode(C.byref(a), _p(ws), n, _stream()), "stg_relattn_decode")
+    return out
+
+
+_NORM_KINDS = {"layer": 0, "rms": 1}
+
+
+def _norm_join_args(x_new, h, gate, post_w, post_b, pre_w, pre_b, kind, alpha, eps, rows_per_group, stats):
+    dev = x_new.device
+    if x_new.dtype not in (BF16, F32):
+        raise RuntimeError(f"norm_join: the stream is bf16 or fp32, got {x_new.dtype}")
+    if kind not in _NORM_KINDS:
+        raise RuntimeError(f"norm_join: kind {kind!r} (layer or rms)")
+    R, Cw = x_new.shape
+    if Cw % 8 or Cw > 8192 or Cw == 0:
+        raise RuntimeError(f"norm_join: width {Cw} (a multiple of 8 up to 8192)")
+    _rel_chk(h, "h", BF16, Cw, dev, rows=R)
+    for t, name, must in ((post_w, "post_w", True), (post_b, "post_b", False), (pre_w, "pre_w", True), (pre_b, "pre_b", False)):
+        if t is None:
+            if must:
+                raise RuntimeError(f"norm_join: {name} is needed")
+            continue
+        _chk1d(t, name, F32, Cw)
+        if t.device != dev or t.data_ptr() % 16:
+            raise RuntimeError(f"{name}: expected a 16-byte aligned vector on {dev}")
+    a = _lib.NormJoinArgs()
+    a.gate_kind, a.rows_per_group = 0, 0
+    if gate is not None:
+        if gate.device != dev or gate.dtype != F32 or not gate.is_contiguous() or gate.data_ptr() % 16:
+            raise RuntimeError(f"gate: expected a contiguous, 16-byte aligned fp32 tensor on {dev}")
+        if gate.dim() == 2:
+            if not rows_per_group or int(rows_per_group) < 1:
+                raise RuntimeError("norm_join: a gate by row groups needs rows_per_group")
+            a.gate_kind, a.rows_per_group = 3, int(rows_per_group)
+            if tuple(gate.shape) != (-(-R // a.rows_per_group), Cw):
+                raise RuntimeError(f"gate: expected [{-(-R // a.rows_per_group)}, {Cw}], got {tuple(gate.shape)}")
+        elif gate.numel() == 1 and gate.dim() <= 1:
+            a.gate_kind = 1
+        elif gate.dim() == 1 and gate.shape[0] == Cw:
+            a.gate_kind = 2
+        else:
+            raise RuntimeError(f"gate: expected one value, [{Cw}] or [groups, {Cw}], got {tuple(gate.shape)}")
+    if stats is not None and (stats.dtype != F32 or tuple(stats.shape) != (R, 4) or not stats.is_contiguous() or stats.device != dev):
+        raise RuntimeError(f"norm_join: stats must be contiguous fp32 [{R}, 4]")
+    a.x_dtype = _dt(x_new)
+    a.h, a.ldh, a.gate = _p(h), _ld(h), _p(gate)
+    a.w1, a.b1, a.w2, a.b2 = _p(post_w), _p(post_b), _p(pre_w), _p(pre_b)
+    a.alpha, a.eps, a.rms = float(alpha), float(eps), _NORM_KINDS[kind]
+    a.stats, a.rows, a.C = _p(stats), R, Cw
+    a.xo, a.ldxo = _p(x_new), _ld(x_new)
+    return a
+
+
+def norm_join_fwd(x, h, gate, post_w, post_b, pre_w, pre_b, *, kind="layer", alpha=1.0, eps=1e-5, rows_per_group=None, want_stats=True):
+    """x_new = alpha x + gate * (Norm(h) post_w + post_b), y = Norm(x_new) pre_w + pre_b in one pass (stg_norm_join_fwd).
+
+    x fp32 / bf16 [rows, C] (the residual stream), h bf16 [rows, C] (the block's output); gate None, one fp32 value, [C], or [groups, C] with
+    rows_per_group consecutive rows to a group; weights fp32 [C] (biases may be None); kind "layer" or "rms".  Returns (x_new in x's type,
+    y bf16, stats fp32 [rows, 4] for norm_join_bwd or None)."""
+    _chk2d(x, "x", x.dtype)
+    x_new = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty(x.shape, dtype=BF16, device=x.device)
+    stats = torch.empty((x.shape[0], 4), dtype=F32, device=x.device) if want_stats else None
+    a = _norm_join_args(x_new, h, gate, post_w, post_b, pre_w, pre_b, kind, alpha, eps, rows_per_group, stats)
+    _rel_chk(x, "x", x.dtype, x.shape[1], x.device)
+    a.y, a.ldy = _p(y), _ld(y)
+    a.x, a.ldx = _p(x), _ld(x)
+    _lib.check(_lib.lib().stg_norm_join_fwd(C.byref(a), _stream()), "stg_norm_join_fwd")
+    return x_new, y, stats
+
+
+def norm_join_bwd(x_new, h, gate, post_w, post_b, pre_w, pre_b, stats, dy, dx_new=None, *, kind="layer", alpha=1.0, eps=1e-5, rows_per_group=None,
+                  want_params=True, want_gate=True):
+    """Gradients of norm_join_fwd (stg_norm_join_bwd) from dy (bf16) and dx_new (the stream's type, None = 0): a dict with dx, dh and, with
+    want_params, dpost_w, dpost_b, dpre_w, dpre_b, dgate (want_gate; the ones whose tensor is None are None)."""
+    _chk2d(x_new, "x_new", x_new.dtype)
+    R, Cw = x_new.shape
+    if stats is None:
+        raise RuntimeError("norm_join_bwd: needs the forward's stats")
+    a = _norm_join_args(x_new, h, gate, post_w, post_b, pre_w, pre_b, kind, alpha, eps, rows_per_group, stats)
+    _rel_chk(x_new, "x_new", x_new.dtype, Cw, x_new.device)
+    _rel_chk(dy, "dy", BF16, Cw, x_new.device, rows=R)
+    if dx_new is not None:
+        _rel_chk(dx_new, "dx_new", x_new.dtype, Cw, x_new.device, rows=R)
+    dx = torch.empty((R, Cw), dtype=x_new.dtype, device=x_new.device)
+    dh = torch.empty((R, Cw), dtype=BF16, device=x_new.device)
+    lib = _lib.lib()
+    params = want_params or (want_gate and a.gate_kind in (1, 2))
+    n = lib.stg_norm_join_param_floats(C.byref(a))
+    dpar = torch.empty(((n + 3) // 4 * 4,), dtype=F32, device=x_new.device) if params else None
+    dgate = torch.empty_like(gate) if want_gate and a.gate_kind == 3 else None
+    nws = lib.stg_norm_join_bwd_ws_floats(C.byref(a)) if params or dgate is not None else 0
+    ws = torch.empty((nws,), dtype=F32, device=x_new.device) if nws else None
+    _lib.check(lib.stg_norm_join_bwd(C.byref(a), _p(dy), _ld(dy), _p(dx_new), _ld(dx_new) if dx_new is not None else 0, _p(dx), _ld(dx), _p(dh), _ld(dh),
+                                     _p(dpar), _p(dgate), _p(ws), nws, _stream()), "stg_norm_join_bwd")
+    out = {"dx": dx, "dh": dh, "dpost_w": None, "dpost_b": None, "dpre_w": None, "dpre_b": None, "dgate": dgate}
+    if params:
+        at = 0
+        for name, t in (("dpost_w", post_w), ("dpost_b", post_b), ("dpre_w", pre_w), ("dpre_b", pre_b), ("dgate", gate if a.gate_kind in (1, 2) else None)):
+            if t is not None:
+                out[name] = dpar[at:at + t.numel()].view(t.shape)
+                at += t.numel()
+    return out
