@@ -652,8 +652,7 @@ int stg_bn_bwd(const void* x, const void* dy, const float* mean, const float* rs
  *   table fp32 [num_buckets, H]; an entry at or below -1e30 (the type's lowest value too) hides its bucket's keys as -inf does.  plan int32 [2 far + 1 + half] on the device: the bucket of every distance -far .. far (distances beyond share
  *   the ends), then the first distance of each of the `half` buckets of a side (half = num_buckets with `causal`, else num_buckets / 2, positive
  *   distances then using the second half); every bucket is one run of distances and far = first distance of the last one, <= 2048.
- *   lse fp32 [H, Tq] (natural logarithm; may be NULL in a forward without backward).  Olo bf16 [Tq, H D] or NULL: O's rounding error, which a
- *   backward that wants the table's gradient reads (without it the gradient carries bf16's rounding of O).
+ *   lse fp32 [H, Tq] (natural logarithm; may be NULL in a forward without backward).
  *   Rows behind the last sequence are left as they were, or zeroed when zero_tail != 0 (by the backward too, in dQ, dK and dV).
  */
 typedef struct {
@@ -661,7 +660,6 @@ typedef struct {
     const void* K; int64_t ldk;
     const void* V; int64_t ldv;
     void* O; int64_t ldo;
-    void* Olo;
     float* lse;
     const int32_t* cu_q; const int32_t* cu_k;
     const void* key_mask;             /* uint8 [Tk] or NULL */
@@ -675,7 +673,7 @@ typedef struct {
 } stg_relattn_args;
 int stg_relattn_fwd(const stg_relattn_args* a, void* stream);
 /* dQ / dK / dV written (not accumulated; shared heads summed over their group), dtable fp32 [num_buckets, H] written, or NULL.  `a` describes the
- * forward (O, Olo and lse as it left them).  ws: fp32 scratch of stg_relattn_bwd_ws_floats(a, dtable != NULL) floats.  No atomics on memory: the
+ * forward (O and lse as it left them).  ws: fp32 scratch of stg_relattn_bwd_ws_floats(a, dtable != NULL) floats.  No atomics on memory: the
  * same call gives the same bits. */
 int64_t stg_relattn_bwd_ws_floats(const stg_relattn_args* a, int want_table);
 int stg_relattn_bwd(const stg_relattn_args* a, const void* dO, int64_t lddo, void* dQ, int64_t lddq, void* dK, int64_t lddk, void* dV,

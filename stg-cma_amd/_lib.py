@@ -119,7 +119,7 @@ class AdamDesc(C.Structure):
 
 
 class RelAttnArgs(C.Structure):
-    _fields_ = [("Q", c_vp), ("ldq", c_i64), ("K", c_vp), ("ldk", c_i64), ("V", c_vp), ("ldv", c_i64), ("O", c_vp), ("ldo", c_i64), ("Olo", c_vp),
+    _fields_ = [("Q", c_vp), ("ldq", c_i64), ("K", c_vp), ("ldk", c_i64), ("V", c_vp), ("ldv", c_i64), ("O", c_vp), ("ldo", c_i64),
                 ("lse", c_vp), ("cu_q", c_vp), ("cu_k", c_vp), ("key_mask", c_vp), ("Tq", c_i64), ("Tk", c_i64), ("S", C.c_int), ("max_q", C.c_int),
                 ("max_k", C.c_int), ("H", C.c_int), ("Hkv", C.c_int), ("D", C.c_int), ("scale", C.c_float), ("causal", C.c_int), ("table", c_vp),
                 ("plan", c_vp), ("num_buckets", C.c_int), ("far", C.c_int), ("zero_tail", C.c_int)]

@@ -14,7 +14,7 @@
 //
 // MFMA v_mfma_f32_32x32x16_bf16; lane l = (r = l & 31, hh = l >> 5); accumulator row (reg, hh) = (reg & 3) + 8 (reg >> 2) + 4 hh.
 #include <math.h>
-#include <float.h>
+#include <type_traits>
 #include "common.h"
 #include "../../include/stgcma.h"
 
@@ -29,7 +29,6 @@ struct RP {
     const bf16_t* K; int64_t ldk;
     const bf16_t* V; int64_t ldv;
     bf16_t* O; int64_t ldo;
-    bf16_t* Olo;                      // [Tq, H D]: O - bf16(O), or NULL
     float* lse;                       // [H, Tq], natural logarithm
     const int32_t* cu_q; const int32_t* cu_k;
     const uint8_t* kmask;
@@ -62,14 +61,6 @@ __device__ __forceinline__ bf16x8_t zero_frag() { const u32x4_t z = {0u, 0u, 0u,
 __device__ __forceinline__ bf16x8_t pack8(const float* x) {
     const u32x4_t w = {pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7])};
     return __builtin_bit_cast(bf16x8_t, w);
-}
-// bf16(x) and bf16(x - bf16(x)): the two together carry 16 bits of x
-__device__ __forceinline__ void pack8_split(const float* x, bf16x8_t& hi, bf16x8_t& lo) {
-    hi = pack8(x);
-    float d[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) d[i] = x[i] - bf2f((bf16_t)hi[i]);
-    lo = pack8(d);
 }
 // transposed fragment of a [rows][DP] tile: A[i = d][k slot j] = tile[16 s2 + 4 hh + (j & 3) + 8 (j >> 2)][32 dt + d]
 template <int DP>
@@ -192,10 +183,9 @@ __device__ __forceinline__ int64_t tail_start(const int32_t* cu, int S, int64_t 
 // ------------------------------------------------------------------------------------------------ forward
 // A block = one (sequence, head) and 32 NW queries, 32 per wave; K / V in 64-key tiles, double-buffered in LDS, one barrier per tile.
 // Scores are computed transposed (rows = keys, lane = query): the softmax statistics are lane-local and P feeds the second MFMA from
-// registers.  LO: the product with V also takes bf16(P - bf16(P)), and O's rounding error is stored beside O: the backward's
-// delta = rowsum(dO O) is then good to 2^-16, which the table's gradient needs (its terms cancel row by row).
-template <int D, int NW, bool LO>
-__global__ void __launch_bounds__(NW * 64, 2) relattn_fwd_kernel(RP a) {
+// registers.
+template <int D, int NW>
+__global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_fwd_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
     using SC = StageC<D, NTHR>;
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];       // two buffers x {K, V} x [64][DP], then the bias by distance
@@ -207,7 +197,6 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_fwd_kernel(RP a) {
         const int64_t from = tail_start(a.cu_q, a.S, a.Tq);
         const int step = gridDim.x * NTHR, off = blockIdx.x * NTHR + tid;
         zero_rows(a.O, a.ldo, from, a.Tq, h * D, D, step, off);
-        if (LO) zero_rows(a.Olo, (int64_t)a.H * D, from, a.Tq, h * D, D, step, off);
         if (a.lse) for (int64_t i = from + off; i < a.Tq; i += step) a.lse[(int64_t)h * a.Tq + i] = -INFINITY;
         return;
     }
@@ -315,21 +304,11 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_fwd_kernel(RP a) {
 #pragma unroll
                         for (int reg = 0; reg < 16; ++reg) o[dt][reg] *= alpha;
                 }
-                bf16x8_t pf[4], pl[4];
-                if (LO) {
-                    pack8_split(xA, pf[0], pl[0]); pack8_split(xA + 8, pf[1], pl[1]);
-                    pack8_split(xB, pf[2], pl[2]); pack8_split(xB + 8, pf[3], pl[3]);
-                } else {
-                    pf[0] = pack8(xA); pf[1] = pack8(xA + 8); pf[2] = pack8(xB); pf[3] = pack8(xB + 8);
-                }
+                const bf16x8_t pf[4] = {pack8(xA), pack8(xA + 8), pack8(xB), pack8(xB + 8)};
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bf16x8_t vf = tr_frag<DP>(sV, dt, i, hh, r);
-                        o[dt] = MFMA32(vf, pf[i], o[dt]);
-                        if (LO) o[dt] = MFMA32(vf, pl[i], o[dt]);
-                    }
+                    for (int i = 0; i < 4; ++i) o[dt] = MFMA32(tr_frag<DP>(sV, dt, i, hh, r), pf[i], o[dt]);
             }
             if (kp + 1 < np) stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, nbits);
             bits = nbits;
@@ -343,12 +322,6 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_fwd_kernel(RP a) {
             for (int dt = 0; dt < DT; ++dt) {
                 if (l == 0.f) o[dt] = splat16(0.f);
                 store_tile32(a.O + row * a.ldo + h * D + 32 * dt, o[dt], inv, hh, ok);
-                if (LO) {
-                    f32x16_t e;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) { const float f = o[dt][i] * inv; e[i] = f - bf2f(f2bf(f)); }
-                    store_tile32(a.Olo + row * ((int64_t)a.H * D) + h * D + 32 * dt, e, 1.0f, hh, ok);
-                }
             }
             if (ok && a.lse && hh == 0) a.lse[(int64_t)h * a.Tq + row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
         }
@@ -357,12 +330,25 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_fwd_kernel(RP a) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dQ, delta, table gradient
-// The forward's tiling with P recomputed from lse: dS = P (dO V^T - delta), dQ = scale dS K.  TAB: dS is also summed along the diagonals
-// of the score matrix (one distance each) with LDS additions into an array that belongs to the wave alone -- instructions of one wave
-// stay in order, so the sums do not depend on timing -- and behind the last border in two registers; each block leaves its sums by
-// bucket in its own row of `part`, which relattn_dtable_kernel adds up in a fixed order.
+// The forward's tiling with P recomputed from lse: dS = P (dO V^T - delta), dQ = scale dS K.
+//
+// TAB, the table's gradient: dtable[b] = sum of dS over a bucket's distances.  A row of dS sums to zero, so these sums cancel to a small part of
+// their terms, and delta = rowsum(dO O) from the bf16 output would leave 2^-9 of it in them.  The first walk over the keys therefore also
+// sums dS by row: r = rowsum(P dP) - delta, the exact delta's distance from the rounded one (sum P = 1).  Tiles behind the last border are summed
+// in that walk, in compensated fp32, and corrected by r times their probability; the tiles around the diagonal, a band of 2 far + 160
+// distances whatever the length, are walked a second time with the exact delta and summed along the diagonals (one distance each) with LDS
+// additions into an array that belongs to the wave alone -- instructions of one wave stay in order, so the sums do not depend on timing.
+// Each block leaves its sums by bucket in its own row of `part`, which relattn_dtable_kernel adds up in a fixed order.
+struct Comp {                                                           // compensated running sum
+    float s = 0.f, c = 0.f;
+    __device__ __forceinline__ void add(float v) {
+        const float y = v - c, t = s + y;
+        c = (t - s) - y;
+        s = t;
+    }
+};
 template <int D, int NW, bool TAB>
-__global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
+__global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
     using SC = StageC<D, NTHR>;
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
@@ -383,13 +369,13 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
     float* mine = diag + wave * blen;
     if (TAB)
         for (int i = tid; i < NW * blen; i += NTHR) diag[i] = 0.f;
-    float far_l = 0.f, far_r = 0.f;
+    float tab_l = 0.f, tab_r = 0.f;                                     // the lane's sums behind the borders, corrected
     __syncthreads();
     const float cleft = bv[0], cright = bv[blen - 1];
     for (int64_t tile = blockIdx.x; tile * 32 * NW < z.nq; tile += gridDim.x) {
         const int nt = (z.nq + 32 * NW - 1) / (32 * NW);
         const int qt = a.causal ? nt - 1 - (int)tile : (int)tile;
-        const int qw = 32 * (qt * NW + wave);
+        const int qb = qt * 32 * NW, qw = qb + 32 * wave;
         const bool live = qw < z.nq;
         const int q = qw + r;
         const bool qok = q < z.nq;
@@ -401,15 +387,13 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
             const bf16_t* qp = a.Q + qrow * a.ldq + h * D + 8 * hh;
             const bf16_t* dp = a.dO + qrow * a.lddo + h * D + 8 * hh;
             const bf16_t* op = a.O + qrow * a.ldo + h * D + 8 * hh;
-            const bf16_t* lp = a.Olo + qrow * ((int64_t)a.H * D) + h * D + 8 * hh;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 qf[s] = ld_frag(qp + 16 * s);
                 df[s] = ld_frag(dp + 16 * s);
                 const bf16x8_t of = ld_frag(op + 16 * s);
-                const bf16x8_t lf = a.Olo ? ld_frag(lp + 16 * s) : zero_frag();
 #pragma unroll
-                for (int j = 0; j < 8; ++j) delta += bf2f((bf16_t)df[s][j]) * (bf2f((bf16_t)of[j]) + bf2f((bf16_t)lf[j]));
+                for (int j = 0; j < 8; ++j) delta += bf2f((bf16_t)df[s][j]) * bf2f((bf16_t)of[j]);
             }
         }
         delta += __shfl_xor(delta, 32, 64);
@@ -417,95 +401,133 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
         const bool seen = qok && lse != -INFINITY;                      // a row that saw no key has no gradient
         const float nl = seen ? -lse * LOG2E : -INFINITY;
         if (!seen) delta = 0.f;
-        if (qok && hh == 0) a.delta[(int64_t)h * a.Tq + qrow] = delta;
         f32x16_t dq[DT];
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) dq[dt] = splat16(0.f);
         int kend = z.nk;
         if (a.causal) {
-            const int last = qt * 32 * NW + 32 * NW - 1 + shift + 1;
+            const int last = qb + 32 * NW + shift;
             kend = kend < last ? kend : (last < 0 ? 0 : last);
         }
         const int np = (kend + 63) >> 6;
         const bf16_t* Kb = a.K + (int64_t)z.k0 * a.ldk + hk * D;
         const bf16_t* Vb = a.V + (int64_t)z.k0 * a.ldv + hk * D;
-        u32x4_t sv[SC::PER];
-        uint64_t bits = 0, nbits = 0;
-        if (np > 0) {
-            stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, 0, z.nk);
-            bits = key_bits(a, z, 0, lane);
-            stage_commit<D, NTHR>(smem, sv, tid, bits);
-        }
-        __syncthreads();
-        for (int kp = 0; kp < np; ++kp) {
-            const bf16_t* sK = smem + (kp & 1) * 2 * SC::TILE;
-            const bf16_t* sV = sK + SC::TILE;
-            const int kb = 64 * kp;
-            if (kp + 1 < np) {
-                stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, kb + 64, z.nk);
-                nbits = key_bits(a, z, kb + 64, lane);
+        Comp all, sl, sr;                                               // the lane's share of its row: sum dS, behind the left / right border
+        float br = 0.f, bn = 0.f;                                       // probability behind the right border, around the diagonal
+        // one walk over key tiles kp0 .. kp1 - 1; BAND: the second one, tiles around the diagonal only, no dQ
+        auto walk = [&](int kp0, int kp1, auto band) __attribute__((always_inline)) {
+            constexpr bool BAND = decltype(band)::value;
+            u32x4_t sv[SC::PER];
+            uint64_t bits = 0, nbits = 0;
+            if (kp0 < kp1) {
+                stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, 64 * kp0, z.nk);
+                bits = key_bits(a, z, 64 * kp0, lane);
+                stage_commit<D, NTHR>(smem + (kp0 & 1) * 2 * SC::TILE, sv, tid, bits);
             }
-            if (live && bits != 0 && !(a.causal && kb > phi)) {
-                const bool left = kb + 63 - plo <= -a.far, right = kb - phi >= a.far;
-                const int idx0 = kb + 4 * hh - pos + a.far + PAD;
-                uint64_t vis = bits;
-                if (a.causal) {
-                    const int c = pos - kb;
-                    vis = c < 0 ? 0 : (c >= 63 ? vis : vis & ((2ull << c) - 1));
+            __syncthreads();
+            for (int kp = kp0; kp < kp1; ++kp) {
+                const bf16_t* sK = smem + (kp & 1) * 2 * SC::TILE;
+                const bf16_t* sV = sK + SC::TILE;
+                const int kb = 64 * kp;
+                if (kp + 1 < kp1) {
+                    stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, kb + 64, z.nk);
+                    nbits = key_bits(a, z, kb + 64, lane);
                 }
-                vis >>= 4 * hh;
-                const bool edge = bits != ~0ull || (a.causal && kb + 63 > plo);
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {                  // the two 32-key tiles, one after the other (register budget)
-                    const bf16_t* tK = sK + half * 32 * DP;
-                    const bf16_t* tV = sV + half * 32 * DP;
-                    const int idx = idx0 + 32 * half;
-                    f32x16_t sc = left ? splat16(cleft) : (right ? splat16(cright) : bias16(bv, idx));
-                    f32x16_t dp = splat16(-delta);                      // dP - delta: the MFMA's accumulator starts there
-#pragma unroll
-                    for (int s = 0; s < KS; ++s) {
-                        sc = MFMA32(nat_frag<DP>(tK, r, hh, s), qf[s], sc);
-                        dp = MFMA32(nat_frag<DP>(tV, r, hh, s), df[s], dp);
+                const bool left = kb + 63 - plo <= -a.far, right = kb - phi >= a.far;
+                if (live && bits != 0 && !(a.causal && kb > phi) && !(BAND && (left || right))) {
+                    const int idx0 = kb + 4 * hh - pos + a.far + PAD;
+                    uint64_t vis = bits;
+                    if (a.causal) {
+                        const int c = pos - kb;
+                        vis = c < 0 ? 0 : (c >= 63 ? vis : vis & ((2ull << c) - 1));
                     }
-                    float ds[16];
+                    vis >>= 4 * hh;
+                    const bool edge = bits != ~0ull || (a.causal && kb + 63 > plo);
 #pragma unroll
-                    for (int reg = 0; reg < 16; ++reg) {
-                        ds[reg] = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nl)) * dp[reg];
-                        if (edge) ds[reg] = (vis >> (32 * half + ACC_ROW(reg, 0))) & 1 ? ds[reg] : 0.f;
-                    }
-                    if (TAB) {
-                        if (left || right) {
-                            float t = 0.f;
+                    for (int half = 0; half < 2; ++half) {              // the two 32-key tiles, one after the other (register budget)
+                        const bf16_t* tK = sK + half * 32 * DP;
+                        const bf16_t* tV = sV + half * 32 * DP;
+                        const int idx = idx0 + 32 * half;
+                        f32x16_t sc = left ? splat16(cleft) : (right ? splat16(cright) : bias16(bv, idx));
+                        f32x16_t dp = splat16(-delta);                  // dP - delta: the MFMA's accumulator starts there
 #pragma unroll
-                            for (int reg = 0; reg < 16; ++reg) t += ds[reg];
-                            if (left) far_l += t; else far_r += t;
-                        } else {
+                        for (int s = 0; s < KS; ++s) {
+                            sc = MFMA32(nat_frag<DP>(tK, r, hh, s), qf[s], sc);
+                            dp = MFMA32(nat_frag<DP>(tV, r, hh, s), df[s], dp);
+                        }
+                        float p[16], ds[16];
 #pragma unroll
-                            for (int reg = 0; reg < 16; ++reg)
+                        for (int reg = 0; reg < 16; ++reg) {
+                            p[reg] = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nl));
+                            ds[reg] = p[reg] * dp[reg];
+                            if (edge) {
+                                const bool on = (vis >> (32 * half + ACC_ROW(reg, 0))) & 1;
+                                p[reg] = on ? p[reg] : 0.f;
+                                ds[reg] = on ? ds[reg] : 0.f;
+                            }
+                        }
+                        if (BAND) {
+#pragma unroll
+                            for (int reg = 0; reg < 16; ++reg) {
+                                bn += p[reg];
                                 __hip_atomic_fetch_add(mine + idx + ACC_ROW(reg, 0), ds[reg], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                            }
+                        } else {
+                            if (TAB) {
+                                float t = 0.f;
+#pragma unroll
+                                for (int reg = 0; reg < 16; ++reg) t += ds[reg];
+                                all.add(t);
+                                if (left) sl.add(t);
+                                if (right) {
+                                    sr.add(t);
+#pragma unroll
+                                    for (int reg = 0; reg < 16; ++reg) br += p[reg];
+                                }
+                            }
+                            const bf16x8_t d0 = pack8(ds), d1 = pack8(ds + 8);
+#pragma unroll
+                            for (int dt = 0; dt < DT; ++dt) {
+                                dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 0, hh, r), d0, dq[dt]);
+                                dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 1, hh, r), d1, dq[dt]);
+                            }
                         }
                     }
-                    const bf16x8_t d0 = pack8(ds), d1 = pack8(ds + 8);
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 0, hh, r), d0, dq[dt]);
-                        dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 1, hh, r), d1, dq[dt]);
-                    }
                 }
+                if (kp + 1 < kp1) stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, nbits);
+                bits = nbits;
+                __syncthreads();
             }
-            if (kp + 1 < np) stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, nbits);
-            bits = nbits;
-            __syncthreads();
-        }
+        };
+        walk(0, np, std::false_type{});
         bf16_t* dqp = a.dQ + ((int64_t)z.q0 + q) * a.lddq + h * D;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) store_tile32(dqp + 32 * dt, dq[dt], a.scale, hh, qok);
+        if (TAB) {
+            float rs = all.s - all.c;
+            rs += __shfl_xor(rs, 32, 64);
+            delta += rs;                                                // rowsum(P dP) to fp32
+            int lo = qb + shift - a.far - 62, hi = qb + 32 * NW - 1 + shift + a.far;    // keys that can be near a query of the block
+            lo = lo < 0 ? 0 : lo >> 6;
+            hi = hi < 0 ? 0 : (hi >> 6) + 1;
+            walk(lo < np ? lo : np, hi < np ? hi : np, std::true_type{});
+            br += __shfl_xor(br, 32, 64);
+            bn += __shfl_xor(bn, 32, 64);
+            const float bl = fmaxf(1.f - br - bn, 0.f);
+            if (hh == 0) {                                              // once per row: the halves' sums of dS enter below, one per lane
+                tab_l -= rs * bl;
+                tab_r -= rs * br;
+            }
+            tab_l += sl.s - sl.c;
+            tab_r += sr.s - sr.c;
+        }
+        if (qok && hh == 0) a.delta[(int64_t)h * a.Tq + qrow] = delta;
         __syncthreads();
     }
     if (TAB) {
-        far_l = wave_sum<64>(far_l);
-        far_r = wave_sum<64>(far_r);
-        if (lane == 0) { mine[0] += far_l; mine[blen - 1] += far_r; }   // ends of the array: distances behind the border
+        tab_l = wave_sum<64>(tab_l);
+        tab_r = wave_sum<64>(tab_r);
+        if (lane == 0) { mine[0] += tab_l; mine[blen - 1] += tab_r; }   // ends of the array: distances behind the border
         __syncthreads();
         for (int i = tid; i < blen; i += NTHR) {
             float t = 0.f;
@@ -921,7 +943,7 @@ int check_args(const char* who, const stg_relattn_args* a) {
     const int64_t hd = (int64_t)a->H * a->D, kd = (int64_t)a->Hkv * a->D;
     STG_CHECK(a->ldq >= hd && a->ldo >= hd && a->ldk >= kd && a->ldv >= kd && a->ldq % 8 == 0 && a->ldk % 8 == 0 && a->ldv % 8 == 0 && a->ldo % 8 == 0, -3,
               "%s: leading dimensions must be multiples of 8 and hold every head", who);
-    STG_CHECK(!misaligned(a->Q) && !misaligned(a->K) && !misaligned(a->V) && !misaligned(a->O) && !misaligned(a->Olo), -3, "%s: tensors must be 16-byte aligned", who);
+    STG_CHECK(!misaligned(a->Q) && !misaligned(a->K) && !misaligned(a->V) && !misaligned(a->O), -3, "%s: tensors must be 16-byte aligned", who);
     return check_bias(who, a->table, a->plan, a->num_buckets, a->far, a->causal, a->scale);
 }
 
@@ -931,7 +953,6 @@ RP make_rp(const stg_relattn_args* a) {
     p.K = (const bf16_t*)a->K; p.ldk = a->ldk;
     p.V = (const bf16_t*)a->V; p.ldv = a->ldv;
     p.O = (bf16_t*)a->O; p.ldo = a->ldo;
-    p.Olo = (bf16_t*)a->Olo;
     p.lse = a->lse;
     p.cu_q = a->cu_q; p.cu_k = a->cu_k; p.kmask = (const uint8_t*)a->key_mask;
     p.Tq = a->Tq; p.Tk = a->Tk; p.S = a->S; p.H = a->H; p.Hkv = a->Hkv; p.causal = a->causal != 0; p.zero_tail = a->zero_tail != 0;
@@ -952,10 +973,10 @@ int grid_tiles(int max_n, int64_t T, int rows) {
     return (int)(t < 1 ? 1 : t);
 }
 
-template <int D, bool LO>
+template <int D>
 int launch_fwd(const RP& p, int max_q, hipStream_t st) {
     static std::atomic<uint64_t> done{0};
-    auto k = relattn_fwd_kernel<D, 4, LO>;
+    auto k = relattn_fwd_kernel<D, 4>;
     STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_fwd: cannot reserve LDS");
     const dim3 grid(grid_tiles(max_q, p.Tq, 128), p.H, p.S + (p.zero_tail ? 1 : 0));
     if (grid.z == 0) return 0;
@@ -1009,8 +1030,7 @@ int launch_decode(const DP_& p, hipStream_t st) {
     }
 
 int run_fwd(const RP& p, int D, int max_q, hipStream_t st) {
-    if (p.Olo) BY_DIM(D, (launch_fwd<DIM, true>(p, max_q, st)));
-    BY_DIM(D, (launch_fwd<DIM, false>(p, max_q, st)));
+    BY_DIM(D, (launch_fwd<DIM>(p, max_q, st)));
 }
 int run_dq(const RP& p, int D, int max_q, hipStream_t st) {
     if (p.part) BY_DIM(D, (launch_dq<DIM, true>(p, max_q, st)));

@@ -2208,7 +2208,7 @@ def _rel_table(g, table, dev):
         raise RuntimeError(f"table: expected contiguous fp32 [{g.num_buckets}, {g.H}] on {dev}, got {table.dtype} {tuple(table.shape)} on {table.device}")
 
 
-def _rel_fill(g, q, k, v, o, olo, lse, table, cu_q, cu_k, max_q, max_k, key_mask):
+def _rel_fill(g, q, k, v, o, lse, table, cu_q, cu_k, max_q, max_k, key_mask):
     dev = q.device
     _rel_chk(q, "q", BF16, g.H * g.D, dev)
     _rel_chk(k, "k", BF16, g.Hkv * g.D, dev)
@@ -2228,11 +2228,9 @@ def _rel_fill(g, q, k, v, o, olo, lse, table, cu_q, cu_k, max_q, max_k, key_mask
             raise RuntimeError(f"key_mask: expected a contiguous bool / uint8 vector of {k.shape[0]} on {dev}, got {key_mask.dtype} {tuple(key_mask.shape)}")
     if lse is not None and (lse.dtype != F32 or tuple(lse.shape) != (g.H, q.shape[0]) or not lse.is_contiguous() or lse.device != dev):
         raise RuntimeError(f"lse: expected contiguous fp32 [{g.H}, {q.shape[0]}]")
-    if olo is not None and (olo.dtype != BF16 or tuple(olo.shape) != (q.shape[0], g.H * g.D) or not olo.is_contiguous() or olo.device != dev):
-        raise RuntimeError(f"olo: expected contiguous bf16 [{q.shape[0]}, {g.H * g.D}]")
     a = _lib.RelAttnArgs()
     a.Q, a.ldq, a.K, a.ldk, a.V, a.ldv, a.O, a.ldo = _p(q), _ld(q), _p(k), _ld(k), _p(v), _ld(v), _p(o), _ld(o)
-    a.Olo, a.lse, a.cu_q, a.cu_k, a.key_mask = _p(olo), _p(lse), _p(cu_q), _p(cu_k), _p(key_mask)
+    a.lse, a.cu_q, a.cu_k, a.key_mask = _p(lse), _p(cu_q), _p(cu_k), _p(key_mask)
     a.Tq, a.Tk, a.S, a.max_q, a.max_k = q.shape[0], k.shape[0], cu_q.shape[0] - 1, min(max_q, q.shape[0]), min(max_k, k.shape[0])
     a.H, a.Hkv, a.D, a.scale, a.causal = g.H, g.Hkv, g.D, g.scale, int(g.causal)
     a.plan, a.num_buckets, a.far = _p(g.plan(dev)), g.num_buckets, g.far
@@ -2240,30 +2238,28 @@ def _rel_fill(g, q, k, v, o, olo, lse, table, cu_q, cu_k, max_q, max_k, key_mask
     return a
 
 
-def relattn_fwd(g, q, k, v, table, cu_q, cu_k=None, *, max_q=None, max_k=None, key_mask=None, out=None, want_lse=True, want_olo=False):
+def relattn_fwd(g, q, k, v, table, cu_q, cu_k=None, *, max_q=None, max_k=None, key_mask=None, out=None, want_lse=True):
     """Attention over ragged sequences with a learned relative position bias by buckets (stg_relattn_fwd).
 
     q bf16 [Tq, H * D], k / v bf16 [Tk, Hkv * D] (column slices of a fused projection are fine); table fp32 [num_buckets, H] (an
     entry at or below -1e30 hides its bucket like -inf); cu_q / cu_k int32
     [S + 1] on the device: sequence s owns rows cu[s] .. cu[s + 1] - 1 (cu_k = None: cu_q); max_q / max_k: the longest sequences, known on the host
     (they size the launch; without them the whole tensor is assumed).  key_mask bool [Tk]: False hides a key.  The last query of a sequence stands
-    at its last key.  Returns (o bf16 [Tq, H * D], lse fp32 [H, Tq] or None), and with want_olo a third: the rounding error of o that relattn_bwd
-    wants for the table's gradient.  Rows behind the last sequence are zero in a fresh output and left alone in `out`."""
+    at its last key.  Returns (o bf16 [Tq, H * D], lse fp32 [H, Tq] or None).  Rows behind the last sequence are zero in a fresh output and left alone in `out`."""
     o = torch.empty((q.shape[0], g.H * g.D), dtype=BF16, device=q.device) if out is None else out
     lse = torch.empty((g.H, q.shape[0]), dtype=F32, device=q.device) if want_lse else None
-    olo = torch.empty((q.shape[0], g.H * g.D), dtype=BF16, device=q.device) if want_olo else None
-    a = _rel_fill(g, q, k, v, o, olo, lse, table, cu_q, cu_k, max_q, max_k, key_mask)
+    a = _rel_fill(g, q, k, v, o, lse, table, cu_q, cu_k, max_q, max_k, key_mask)
     a.zero_tail = int(out is None)
     _lib.check(_lib.lib().stg_relattn_fwd(C.byref(a), _stream()), "stg_relattn_fwd")
-    return (o, lse, olo) if want_olo else (o, lse)
+    return o, lse
 
 
-def relattn_bwd(g, q, k, v, table, cu_q, cu_k, o, lse, do, *, olo=None, max_q=None, max_k=None, key_mask=None, want_table=True):
+def relattn_bwd(g, q, k, v, table, cu_q, cu_k, o, lse, do, *, max_q=None, max_k=None, key_mask=None, want_table=True):
     """(dq, dk, dv, dtable or None) of relattn_fwd (stg_relattn_bwd): the probabilities are recomputed from lse, shared key / value heads summed
     over their group, dtable fp32.  Gradient rows behind the last sequence are zero."""
     if lse is None:
         raise RuntimeError("relattn_bwd: needs the forward's lse")
-    a = _rel_fill(g, q, k, v, o, olo, lse, table, cu_q, cu_k, max_q, max_k, key_mask)
+    a = _rel_fill(g, q, k, v, o, lse, table, cu_q, cu_k, max_q, max_k, key_mask)
     _rel_chk(do, "do", BF16, g.H * g.D, q.device, rows=q.shape[0])
     dq = torch.empty((q.shape[0], g.H * g.D), dtype=BF16, device=q.device)
     dk = torch.empty((k.shape[0], g.Hkv * g.D), dtype=BF16, device=q.device)

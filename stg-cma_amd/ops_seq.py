@@ -29,26 +29,20 @@ class RelAttentionFn(torch.autograd.Function):
     def forward(ctx, q, k, v, table, geom, cu_q, cu_k, max_q, max_k, key_mask):
         need = ctx.needs_input_grad
         train = any(need[:4])
-        olo = None
-        # the table's gradient sums dS over whole sequences, where it cancels row by row: it takes delta from o and o's rounding error
-        r = K.relattn_fwd(geom, q, k, v, table, cu_q, cu_k, max_q=max_q, max_k=max_k, key_mask=key_mask, want_lse=train, want_olo=need[3])
-        if need[3]:
-            o, lse, olo = r
-        else:
-            o, lse = r
+        o, lse = K.relattn_fwd(geom, q, k, v, table, cu_q, cu_k, max_q=max_q, max_k=max_k, key_mask=key_mask, want_lse=train)
         if train:
-            ctx.save_for_backward(q, k, v, table, cu_q, cu_k, key_mask, o, lse, olo)
+            ctx.save_for_backward(q, k, v, table, cu_q, cu_k, key_mask, o, lse)
             ctx.how = (geom, max_q, max_k)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, table, cu_q, cu_k, key_mask, o, lse, olo = ctx.saved_tensors
+        q, k, v, table, cu_q, cu_k, key_mask, o, lse = ctx.saved_tensors
         geom, max_q, max_k = ctx.how
         need = ctx.needs_input_grad
         with _on(q):
-            grads = K.relattn_bwd(geom, q, k, v, table, cu_q, cu_k, o, lse, _grad(do, BF16), olo=olo, max_q=max_q, max_k=max_k, key_mask=key_mask,
+            grads = K.relattn_bwd(geom, q, k, v, table, cu_q, cu_k, o, lse, _grad(do, BF16), max_q=max_q, max_k=max_k, key_mask=key_mask,
                                   want_table=need[3])
         return tuple(g if n else None for g, n in zip(grads, need)) + (None,) * 6
 

@@ -4,7 +4,8 @@ Attention.  The kernels round P (and in the backward dS) to bf16 before the seco
 With u = 2^-8 (half a bf16 step, relative) and e = the relative error of a probability,
     |o - ref|  <= u |ref| + (u + 2 e) sum_j p |v|
     |dv - ref| <= u |ref| + (u + 2 e) sum_i p |do|
-    |dS - ref| <= 2 e p (|dP| + |delta|) + p E_i =: s_ij     E_i = error of delta_i, from o's error (2^-8 of it without the stored remainder)
+    |dS - ref| <= 2 e p (|dP| + |delta|) + p E_i =: s_ij     E_i = error of delta_i: o's error where delta comes from the stored o (dq, and
+                                                       dk without a table gradient), fp32's where it is summed again (dtable, dk)
     |dq - ref| <= u |ref| + scale sum_j (u |dS| + (1 + u) s_ij) |k|,   dk alike,   dtable <= sum s_ij over the bucket + its own fp32 summation.
 e: the score is a sum of D products in fp32 plus the bias, so its error is at most (D + 8) 2^-24 A with A = scale sum |q||k| + |bias| + |lse|, the
 exponential and the row sum of n terms add (n + 8) 2^-24.
@@ -28,7 +29,7 @@ def bucket(distance, buckets, far, causal):
     return b + (half if distance > 0 and not causal else 0)
 
 
-def attention(q, k, v, table, lens_q, lens_k, H, Hkv, D, buckets, far, causal, scale, mask=None, do=None, remainder=True):
+def attention(q, k, v, table, lens_q, lens_k, H, Hkv, D, buckets, far, causal, scale, mask=None, do=None, table_grad=True):
     """dict of name -> (value, bound), all float64, rows packed; rows behind the last sequence are zero (lse -inf)."""
     dev = q.device
     f = lambda t: t.double()
@@ -82,13 +83,17 @@ def attention(q, k, v, table, lens_q, lens_k, H, Hkv, D, buckets, far, causal, s
             dP = G @ V.t()
             delta = (p * dP).sum(1, keepdim=True)
             dS = p * (dP - delta)
-            oerr = (U * U * O.abs() + (U * U + 2 * e) * pv) if remainder else (U * O.abs() + (U + 2 * e) * pv)
-            E = (G.abs() * oerr).sum(1, keepdim=True) + (D + 8) * E32 * (G.abs() * O.abs()).sum(1, keepdim=True)
             dperr = (D + 8) * E32 * (G.abs() @ V.abs().t())
-            s = 2 * e * p * (dP.abs() + delta.abs()) + p * (E + dperr)
-            w = U * dS.abs() + (1 + U) * s
+
+            def size(oerr):                                       # bounds of |dS - ref| and of that plus dS's own rounding
+                E = (G.abs() * oerr).sum(1, keepdim=True) + (D + 8) * E32 * (G.abs() * O.abs()).sum(1, keepdim=True)
+                s = 2 * e * p * (dP.abs() + delta.abs()) + p * (E + dperr)
+                return s, U * dS.abs() + (1 + U) * s
+            rounded = U * O.abs() + (U + 2 * e) * pv
+            s, w = size(rounded)
             out["dq"][0][rq, cq] = scale * dS @ Kk
             out["dq"][1][rq, cq] = U * (scale * dS @ Kk).abs() + scale * w @ Kk.abs()
+            s, w = size(2 * e * pv if table_grad else rounded)
             out["dk"][0][rk, ck] += scale * dS.t() @ Q
             out["dk"][1][rk, ck] += scale * w.t() @ Q.abs()
             out["dv"][0][rk, ck] += p.t() @ G

@@ -88,10 +88,10 @@ def test_forward_and_gradients(stg, gpu, case):
     R.within(o2, ref["o"], "o (training)")
     for name, g in zip(("dq", "dk", "dv", "dtable"), torch.autograd.grad(o2, leaves, do)):
         R.within(g, ref[name], name, 1e-6)
-    # frozen table: the plain remainder-free delta, same three gradients within that bound
+    # frozen table: delta from the rounded o alone
     o3 = ops_seq.rel_attention(*leaves[:3], table, geom, cu_q, cu_k, key_mask=mask)          # (and no length hint)
     assert torch.equal(o3, o)
-    ref = R.attention(q, k, v, table, lens_q, lens_k, H, Hkv, D, nb, far, causal, D ** -0.5, mask, do, remainder=False)
+    ref = R.attention(q, k, v, table, lens_q, lens_k, H, Hkv, D, nb, far, causal, D ** -0.5, mask, do, table_grad=False)
     for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o3, leaves[:3], do)):
         R.within(g, ref[name], name + " (frozen table)", 1e-6)
 
@@ -192,17 +192,17 @@ def test_same_call_same_bits_and_length_hints(stg, gpu):
         cu = _cu(lens, gpu)
         first = None
         for hint in (333, 333, 333, 64, 1, None, 10 ** 6):        # a hint below the longest still computes every row
-            o, lse, olo = K.relattn_fwd(geom, q, k, v, table, cu, max_q=hint, want_olo=True)
-            dq, dk, dv, dt = K.relattn_bwd(geom, q, k, v, table, cu, None, o, lse, do, olo=olo, max_q=hint)
+            o, lse = K.relattn_fwd(geom, q, k, v, table, cu, max_q=hint)
+            dq, dk, dv, dt = K.relattn_bwd(geom, q, k, v, table, cu, None, o, lse, do, max_q=hint)
             if first is None:
-                first = (o, lse, olo, dq, dk, dv, dt)
+                first = (o, lse, dq, dk, dv, dt)
                 continue
-            for a, b in zip(first[:6], (o, lse, olo, dq, dk, dv)):
+            for a, b in zip(first[:5], (o, lse, dq, dk, dv)):
                 assert torch.equal(a, b)
             if hint == 333:
-                assert torch.equal(first[6], dt)
+                assert torch.equal(first[5], dt)
             else:                                              # other blocks, another order of the fp32 sums
-                assert float((first[6] - dt).abs().max()) <= 1e-4 * float(first[6].abs().max())
+                assert float((first[5] - dt).abs().max()) <= 1e-4 * float(first[5].abs().max())
 
 
 def test_bad_offsets_stay_inside(stg, gpu):
