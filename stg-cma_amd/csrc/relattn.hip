@@ -57,6 +57,17 @@ __device__ __forceinline__ f32x16_t splat16(float v) {
     for (int i = 0; i < 16; ++i) z[i] = v;
     return z;
 }
+// maxima that hand a NaN on (v_maximum3_f32: no canonicalisation of the MFMA results in front of it)
+__device__ __forceinline__ float fmax2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float fmax3(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
+// the other half-wave's value meets the lane's own (lanes r and r + 32 hold the two halves of a query's or key's accumulator rows)
+__device__ __forceinline__ void both_halves(float v, float& lo, float& hi) {
+    const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    lo = __uint_as_float(w[0]);
+    hi = __uint_as_float(w[1]);
+}
+__device__ __forceinline__ float half_sum(float v) { float a, b; both_halves(v, a, b); return a + b; }
+__device__ __forceinline__ float half_max(float v) { float a, b; both_halves(v, a, b); return fmax2(a, b); }
 __device__ __forceinline__ bf16x8_t zero_frag() { const u32x4_t z = {0u, 0u, 0u, 0u}; return __builtin_bit_cast(bf16x8_t, z); }
 __device__ __forceinline__ bf16x8_t pack8(const float* x) {
     const u32x4_t w = {pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7])};
@@ -157,7 +168,8 @@ __device__ __forceinline__ void stage_commit(bf16_t* s, const U4Arr<StageC<D, NT
 __device__ __forceinline__ uint64_t key_bits(const RP& a, const Seq& z, int kb, int lane) {
     bool ok = kb + lane < z.nk;
     if (a.kmask != nullptr && ok) ok = a.kmask[(int64_t)z.k0 + kb + lane] != 0;
-    return __builtin_amdgcn_ballot_w64(ok);
+    const uint64_t b = __builtin_amdgcn_ballot_w64(ok);
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
 }
 // start of a score accumulator: bias of rows kb + ACC_ROW(., hh) against the lane's query position (idx = bv index of row 0, hh included)
 __device__ __forceinline__ f32x16_t bias16(const float* bv, int idx) {
@@ -185,12 +197,12 @@ __device__ __forceinline__ int64_t tail_start(const int32_t* cu, int S, int64_t 
 // Scores are computed transposed (rows = keys, lane = query): the softmax statistics are lane-local and P feeds the second MFMA from
 // registers.
 template <int D, int NW>
-__global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_fwd_kernel(RP a) {
+__global__ void __launch_bounds__(NW * 64, 2) relattn_fwd_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
     using SC = StageC<D, NTHR>;
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];       // two buffers x {K, V} x [64][DP], then the bias by distance
     float* bv = reinterpret_cast<float*>(smem + 4 * SC::TILE);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // (wave-uniform for the compiler too)
     const int r = lane & 31, hh = lane >> 5;
     const int h = blockIdx.y, hk = h / (a.H / a.Hkv);
     if ((int)blockIdx.z == a.S) {                                       // the slice that clears the rows behind the last sequence
@@ -250,22 +262,26 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_fwd_kernel(R
                 nbits = key_bits(a, z, kb + 64, lane);
             }
             if (live && bits != 0 && !(a.causal && kb > phi)) {
-                f32x16_t sA, sB;                                        // St[key][q] of keys kb .. + 31 / + 32 .. + 63
-                if (kb + 63 - plo <= -a.far) { sA = splat16(cleft); sB = sA; }
-                else if (kb - phi >= a.far) { sA = splat16(cright); sB = sA; }
-                else {
+                // St[key][q] of keys kb .. + 31 / + 32 .. + 63.  Behind a border the bias is one number: it joins the exponent's constant and
+                // the MFMA starts at zero; nearer, the accumulator starts at the bias.
+                f32x16_t sA, sB;
+                float far = 0.f;
+                const bool left = kb + 63 - plo <= -a.far;
+                if (left || kb - phi >= a.far) {
+                    far = left ? cleft : cright;
+                    sA = MFMA32(nat_frag<DP>(sK, r, hh, 0), qf[0], splat16(0.f));
+                    sB = MFMA32(nat_frag<DP>(sK + 32 * DP, r, hh, 0), qf[0], splat16(0.f));
+                } else {
                     const int idx = kb + 4 * hh - pos + a.far + PAD;
-                    sA = bias16(bv, idx);
-                    sB = bias16(bv, idx + 32);
+                    sA = MFMA32(nat_frag<DP>(sK, r, hh, 0), qf[0], bias16(bv, idx));
+                    sB = MFMA32(nat_frag<DP>(sK + 32 * DP, r, hh, 0), qf[0], bias16(bv, idx + 32));
                 }
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
+                for (int s = 1; s < KS; ++s) {
                     sA = MFMA32(nat_frag<DP>(sK, r, hh, s), qf[s], sA);
                     sB = MFMA32(nat_frag<DP>(sK + 32 * DP, r, hh, s), qf[s], sB);
                 }
-                float xA[16], xB[16];
-                const bool edge = bits != ~0ull || (a.causal && kb + 63 > plo);
-                if (edge) {
+                if (bits != ~0ull || (a.causal && kb + 63 > plo)) {
                     uint64_t vis = bits;                                // keys this lane's query may see
                     if (a.causal) {
                         const int c = pos - kb;                         // last visible key of the tile
@@ -274,29 +290,30 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_fwd_kernel(R
                     vis >>= 4 * hh;
 #pragma unroll
                     for (int reg = 0; reg < 16; ++reg) {
-                        xA[reg] = (vis >> ACC_ROW(reg, 0)) & 1 ? sA[reg] : -INFINITY;
-                        xB[reg] = (vis >> (32 + ACC_ROW(reg, 0))) & 1 ? sB[reg] : -INFINITY;
+                        sA[reg] = (vis >> ACC_ROW(reg, 0)) & 1 ? sA[reg] : -INFINITY;
+                        sB[reg] = (vis >> (32 + ACC_ROW(reg, 0))) & 1 ? sB[reg] : -INFINITY;
                     }
-                } else {
-#pragma unroll
-                    for (int reg = 0; reg < 16; ++reg) { xA[reg] = sA[reg]; xB[reg] = sB[reg]; }
                 }
-                float mr = -INFINITY;                                   // the maximum on the raw scores (scale > 0)
+                float mr = fmax3(sA[0], sB[0], sA[1]);                  // the maximum on the raw scores (scale > 0)
+                mr = fmax3(mr, sB[1], sB[2]);
 #pragma unroll
-                for (int reg = 0; reg < 16; ++reg) mr = fmaxf(mr, fmaxf(xA[reg], xB[reg]));
-                mr = fmaxf(mr, __shfl_xor(mr, 32, 64));
-                const float mx = fmaxf(m, mr * a.scale2);
+                for (int reg = 2; reg < 15; ++reg) mr = fmax3(mr, sA[reg], sB[reg + 1]);
+                mr = fmax2(mr, sA[15]);
+                mr = half_max(mr) + far;
+                const float mx = fmax2(m, mr * a.scale2);
                 const float nm = mx == -INFINITY ? 0.f : -mx;           // nothing seen so far: every exponent is -inf
                 const float alpha = __builtin_amdgcn_exp2f(m + nm);
+                const float nf = far == 0.f ? nm : fmaf(far, a.scale2, nm);
                 m = mx;
+                float xA[16], xB[16];
                 float ls = 0.f;
 #pragma unroll
                 for (int reg = 0; reg < 16; ++reg) {
-                    xA[reg] = __builtin_amdgcn_exp2f(fmaf(xA[reg], a.scale2, nm));
-                    xB[reg] = __builtin_amdgcn_exp2f(fmaf(xB[reg], a.scale2, nm));
+                    xA[reg] = __builtin_amdgcn_exp2f(fmaf(sA[reg], a.scale2, nf));
+                    xB[reg] = __builtin_amdgcn_exp2f(fmaf(sB[reg], a.scale2, nf));
                     ls += xA[reg] + xB[reg];
                 }
-                ls += __shfl_xor(ls, 32, 64);
+                ls = half_sum(ls);
                 l = l * alpha + ls;
                 if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {  // rescale only when some query's maximum moved
 #pragma unroll
@@ -355,7 +372,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
     const int blen = 2 * (a.far + PAD) + 1;
     float* bv = reinterpret_cast<float*>(smem + 4 * SC::TILE);
     float* diag = bv + blen;                                            // [NW][blen]
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // (wave-uniform for the compiler too)
     const int r = lane & 31, hh = lane >> 5;
     const int h = blockIdx.y, hk = h / (a.H / a.Hkv);
     if ((int)blockIdx.z == a.S) {
@@ -371,7 +388,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
         for (int i = tid; i < NW * blen; i += NTHR) diag[i] = 0.f;
     float tab_l = 0.f, tab_r = 0.f;                                     // the lane's sums behind the borders, corrected
     __syncthreads();
-    const float cleft = bv[0], cright = bv[blen - 1];
+    const float cleft = bv[0] * a.scale2, cright = bv[blen - 1] * a.scale2;
     for (int64_t tile = blockIdx.x; tile * 32 * NW < z.nq; tile += gridDim.x) {
         const int nt = (z.nq + 32 * NW - 1) / (32 * NW);
         const int qt = a.causal ? nt - 1 - (int)tile : (int)tile;
@@ -396,7 +413,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
                 for (int j = 0; j < 8; ++j) delta += bf2f((bf16_t)df[s][j]) * bf2f((bf16_t)of[j]);
             }
         }
-        delta += __shfl_xor(delta, 32, 64);
+        delta = half_sum(delta);
         const float lse = a.lse[(int64_t)h * a.Tq + qrow];
         const bool seen = qok && lse != -INFINITY;                      // a row that saw no key has no gradient
         const float nl = seen ? -lse * LOG2E : -INFINITY;
@@ -417,6 +434,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
         // one walk over key tiles kp0 .. kp1 - 1; BAND: the second one, tiles around the diagonal only, no dQ
         auto walk = [&](int kp0, int kp1, auto band) __attribute__((always_inline)) {
             constexpr bool BAND = decltype(band)::value;
+            const f32x16_t ndel = splat16(-delta);
             u32x4_t sv[SC::PER];
             uint64_t bits = 0, nbits = 0;
             if (kp0 < kp1) {
@@ -443,24 +461,30 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
                     }
                     vis >>= 4 * hh;
                     const bool edge = bits != ~0ull || (a.causal && kb + 63 > plo);
+                    const float nf = left ? nl + cleft : (right ? nl + cright : nl);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {              // the two 32-key tiles, one after the other (register budget)
                         const bf16_t* tK = sK + half * 32 * DP;
                         const bf16_t* tV = sV + half * 32 * DP;
                         const int idx = idx0 + 32 * half;
-                        f32x16_t sc = left ? splat16(cleft) : (right ? splat16(cright) : bias16(bv, idx));
-                        f32x16_t dp = splat16(-delta);                  // dP - delta: the MFMA's accumulator starts there
+                        f32x16_t sc, dp = MFMA32(nat_frag<DP>(tV, r, hh, 0), df[0], ndel);     // dP - delta: the accumulator starts at -delta
+                        if (left || right) sc = MFMA32(nat_frag<DP>(tK, r, hh, 0), qf[0], splat16(0.f));
+                        else sc = MFMA32(nat_frag<DP>(tK, r, hh, 0), qf[0], bias16(bv, idx));
 #pragma unroll
-                        for (int s = 0; s < KS; ++s) {
+                        for (int s = 1; s < KS; ++s) {
                             sc = MFMA32(nat_frag<DP>(tK, r, hh, s), qf[s], sc);
                             dp = MFMA32(nat_frag<DP>(tV, r, hh, s), df[s], dp);
                         }
                         float p[16], ds[16];
 #pragma unroll
                         for (int reg = 0; reg < 16; ++reg) {
-                            p[reg] = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nl));
+                            p[reg] = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nf));
                             ds[reg] = p[reg] * dp[reg];
-                            if (edge) {
+                        }
+                        if (edge) {
+                            asm volatile("");                           // (kept a branch: as selects these run in every tile)
+#pragma unroll
+                            for (int reg = 0; reg < 16; ++reg) {
                                 const bool on = (vis >> (32 * half + ACC_ROW(reg, 0))) & 1;
                                 p[reg] = on ? p[reg] : 0.f;
                                 ds[reg] = on ? ds[reg] : 0.f;
@@ -505,14 +529,14 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
         for (int dt = 0; dt < DT; ++dt) store_tile32(dqp + 32 * dt, dq[dt], a.scale, hh, qok);
         if (TAB) {
             float rs = all.s - all.c;
-            rs += __shfl_xor(rs, 32, 64);
+            rs = half_sum(rs);
             delta += rs;                                                // rowsum(P dP) to fp32
             int lo = qb + shift - a.far - 62, hi = qb + 32 * NW - 1 + shift + a.far;    // keys that can be near a query of the block
             lo = lo < 0 ? 0 : lo >> 6;
             hi = hi < 0 ? 0 : (hi >> 6) + 1;
             walk(lo < np ? lo : np, hi < np ? hi : np, std::true_type{});
-            br += __shfl_xor(br, 32, 64);
-            bn += __shfl_xor(bn, 32, 64);
+            br = half_sum(br);
+            bn = half_sum(bn);
             const float bl = fmaxf(1.f - br - bn, 0.f);
             if (hh == 0) {                                              // once per row: the halves' sums of dS enter below, one per lane
                 tab_l -= rs * bl;
@@ -573,14 +597,14 @@ __global__ void __launch_bounds__(256) relattn_dtable_kernel(const float* part, 
 // A block = one (sequence, key / value head) and 32 NW keys, 32 per wave; it walks the queries of every head of the group in 64-row tiles
 // of Q and dO, so the gradients of a shared head are summed in registers, in one order.  S[q][key]: rows = queries, lane = key.
 template <int D, int NW>
-__global__ void __launch_bounds__(NW * 64, 1) relattn_dkv_kernel(RP a) {
+__global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
     using SC = StageC<D, NTHR>;
     constexpr int BUF = 2 * SC::TILE + 256;                             // Q and dO tiles + 128 floats of statistics
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
     float* bv = reinterpret_cast<float*>(smem + 2 * BUF);
     const int blen = 2 * (a.far + PAD) + 1;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // (wave-uniform for the compiler too)
     const int r = lane & 31, hh = lane >> 5;
     const int hk = blockIdx.y, rep = a.H / a.Hkv;
     if ((int)blockIdx.z == a.S) {
@@ -646,6 +670,8 @@ __global__ void __launch_bounds__(NW * 64, 1) relattn_dkv_kernel(RP a) {
             commit_all(smem + (p0 & 1) * BUF, 64 * p0);
             __syncthreads();
             const float cleft = bv[0], cright = bv[blen - 1];
+            f32x16_t cvec = splat16(cright);
+            int side = 2;
             for (int qp = p0; qp < np; ++qp) {
                 const bf16_t* sQ = smem + (qp & 1) * BUF;
                 const bf16_t* sD = sQ + SC::TILE;
@@ -655,18 +681,24 @@ __global__ void __launch_bounds__(NW * 64, 1) relattn_dkv_kernel(RP a) {
                 if (live && !(a.causal && pb + 63 < kw)) {
                     const bool left = kw + 31 - pb <= -a.far, right = kw - (pb + 63) >= a.far;
                     const bool edge = a.causal && kw + 31 > pb;
+                    // behind a border the accumulator starts at one number: 16 registers that change twice in a walk
+                    if ((left || right) && side != (left ? 1 : 2)) {
+                        side = left ? 1 : 2;
+                        cvec = splat16(left ? cleft : cright);
+                    }
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const bf16_t* tQ = sQ + half * 32 * DP;
                         const bf16_t* tD = sD + half * 32 * DP;
                         const int rel = key - (pb + 32 * half) - 4 * hh;    // distance of accumulator row 0
                         f32x16_t sc, dp;
-                        if (left) sc = splat16(cleft);
-                        else if (right) sc = splat16(cright);
+                        if (left || right) sc = MFMA32(nat_frag<DP>(tQ, r, hh, 0), kf[0], cvec);
                         else {
                             const float* bp = bv + rel + a.far + PAD;
+                            f32x16_t c;
 #pragma unroll
-                            for (int reg = 0; reg < 16; ++reg) sc[reg] = bp[-ACC_ROW(reg, 0)];
+                            for (int reg = 0; reg < 16; ++reg) c[reg] = bp[-ACC_ROW(reg, 0)];
+                            sc = MFMA32(nat_frag<DP>(tQ, r, hh, 0), kf[0], c);
                         }
                         float lv[16];
 #pragma unroll
@@ -678,16 +710,23 @@ __global__ void __launch_bounds__(NW * 64, 1) relattn_dkv_kernel(RP a) {
                         }
 #pragma unroll
                         for (int s = 0; s < KS; ++s) {
-                            sc = MFMA32(nat_frag<DP>(tQ, r, hh, s), kf[s], sc);
+                            if (s > 0) sc = MFMA32(nat_frag<DP>(tQ, r, hh, s), kf[s], sc);
                             dp = MFMA32(nat_frag<DP>(tD, r, hh, s), vf[s], dp);
                         }
                         float pr[16], ds[16];
 #pragma unroll
                         for (int reg = 0; reg < 16; ++reg) {
-                            float p = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, lv[reg]));
-                            if (edge) p = rel <= ACC_ROW(reg, 0) ? p : 0.f;     // hidden by the causal rule (and so is dS, whatever dP holds)
+                            const float p = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, lv[reg]));
                             pr[reg] = p;
-                            ds[reg] = edge && rel > ACC_ROW(reg, 0) ? 0.f : p * dp[reg];
+                            ds[reg] = p * dp[reg];
+                        }
+                        if (edge) {                                     // hidden by the causal rule (dS too, whatever dP holds)
+                            asm volatile("");                           // (kept a branch: as selects these run in every tile)
+#pragma unroll
+                            for (int reg = 0; reg < 16; ++reg) {
+                                pr[reg] = rel <= ACC_ROW(reg, 0) ? pr[reg] : 0.f;
+                                ds[reg] = rel <= ACC_ROW(reg, 0) ? ds[reg] : 0.f;
+                            }
                         }
                         const bf16x8_t a0 = pack8(pr), a1 = pack8(pr + 8), d0 = pack8(ds), d1 = pack8(ds + 8);
 #pragma unroll
@@ -739,7 +778,7 @@ template <int D>
 __global__ void __launch_bounds__(256, 2) relattn_decode_kernel(DP_ a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, ROWP = D / 8, PER = 2 * 32 * ROWP / 64, TILE = 32 * DP;
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];       // per wave {K, V} x [32][DP]; then bias [far + 1][32]: see host
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // (wave-uniform for the compiler too)
     const int r = lane & 31, hh = lane >> 5;
     const int rep = a.H / a.Hkv, ncg = (rep + 31) / 32;
     const int hk = blockIdx.y / ncg, cg = blockIdx.y - hk * ncg;
@@ -823,7 +862,7 @@ __global__ void __launch_bounds__(256, 2) relattn_decode_kernel(DP_ a) {
             x[reg] = tail && kb + ACC_ROW(reg, hh) >= k1 ? -INFINITY : sc[reg];
             mr = fmaxf(mr, x[reg]);
         }
-        mr = fmaxf(mr, __shfl_xor(mr, 32, 64));
+        mr = half_max(mr);
         const float mx = fmaxf(m, mr * a.scale2);
         const float nm = mx == -INFINITY ? 0.f : -mx;
         const float alpha = __builtin_amdgcn_exp2f(m + nm);
@@ -834,7 +873,7 @@ __global__ void __launch_bounds__(256, 2) relattn_decode_kernel(DP_ a) {
             x[reg] = __builtin_amdgcn_exp2f(fmaf(x[reg], a.scale2, nm));
             ls += x[reg];
         }
-        ls += __shfl_xor(ls, 32, 64);
+        ls = half_sum(ls);
         l = l * alpha + ls;
         if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
 #pragma unroll
