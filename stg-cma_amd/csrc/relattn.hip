@@ -350,12 +350,10 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_fwd_kernel(RP a) {
 // The forward's tiling with P recomputed from lse: dS = P (dO V^T - delta), dQ = scale dS K.
 //
 // TAB, the table's gradient: dtable[b] = sum of dS over a bucket's distances.  A row of dS sums to zero, so these sums cancel to a small part of
-// their terms, and delta = rowsum(dO O) from the bf16 output would leave 2^-9 of it in them.  The first walk over the keys therefore also
-// sums dS by row: r = rowsum(P dP) - delta, the exact delta's distance from the rounded one (sum P = 1).  Tiles behind the last border are summed
-// in that walk, in compensated fp32, and corrected by r times their probability; the tiles around the diagonal, a band of 2 far + 160
-// distances whatever the length, are walked a second time with the exact delta and summed along the diagonals (one distance each) with LDS
-// additions into an array that belongs to the wave alone -- instructions of one wave stay in order, so the sums do not depend on timing.
-// Each block leaves its sums by bucket in its own row of `part`, which relattn_dtable_kernel adds up in a fixed order.
+// their terms, and delta = rowsum(dO O) from the bf16 output would leave 2^-9 of it in them.  The walk over the keys therefore also sums dS by
+// row: r = rowsum(P dP) - delta, the exact delta's distance from the rounded one (sum P = 1).  Tiles behind the last border are summed here, in
+// compensated fp32, and corrected by r times their probability; the band of tiles around the diagonal is left to relattn_band_kernel, which has
+// the exact delta.  Each block leaves its sums in its own row of `part`, added up in a fixed order by relattn_dtable_kernel.
 struct Comp {                                                           // compensated running sum
     float s = 0.f, c = 0.f;
     __device__ __forceinline__ void add(float v) {
@@ -371,7 +369,6 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
     const int blen = 2 * (a.far + PAD) + 1;
     float* bv = reinterpret_cast<float*>(smem + 4 * SC::TILE);
-    float* diag = bv + blen;                                            // [NW][blen]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // (wave-uniform for the compiler too)
     const int r = lane & 31, hh = lane >> 5;
     const int h = blockIdx.y, hk = h / (a.H / a.Hkv);
@@ -383,9 +380,6 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
     const Seq z = seq_of(a, blockIdx.z);
     const int shift = z.nk - z.nq;
     fill_bias(a, h, bv, tid, NTHR);
-    float* mine = diag + wave * blen;
-    if (TAB)
-        for (int i = tid; i < NW * blen; i += NTHR) diag[i] = 0.f;
     float tab_l = 0.f, tab_r = 0.f;                                     // the lane's sums behind the borders, corrected
     __syncthreads();
     const float cleft = bv[0] * a.scale2, cright = bv[blen - 1] * a.scale2;
@@ -431,159 +425,303 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
         const bf16_t* Vb = a.V + (int64_t)z.k0 * a.ldv + hk * D;
         Comp all, sl, sr;                                               // the lane's share of its row: sum dS, behind the left / right border
         float br = 0.f, bn = 0.f;                                       // probability behind the right border, around the diagonal
-        // one walk over key tiles kp0 .. kp1 - 1; BAND: the second one, tiles around the diagonal only, no dQ
-        auto walk = [&](int kp0, int kp1, auto band) __attribute__((always_inline)) {
-            constexpr bool BAND = decltype(band)::value;
-            const f32x16_t ndel = splat16(-delta);
-            u32x4_t sv[SC::PER];
-            uint64_t bits = 0, nbits = 0;
-            if (kp0 < kp1) {
-                stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, 64 * kp0, z.nk);
-                bits = key_bits(a, z, 64 * kp0, lane);
-                stage_commit<D, NTHR>(smem + (kp0 & 1) * 2 * SC::TILE, sv, tid, bits);
+        const f32x16_t ndel = splat16(-delta);
+        u32x4_t sv[SC::PER];
+        uint64_t bits = 0, nbits = 0;
+        if (np > 0) {
+            stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, 0, z.nk);
+            bits = key_bits(a, z, 0, lane);
+            stage_commit<D, NTHR>(smem, sv, tid, bits);
+        }
+        __syncthreads();
+        for (int kp = 0; kp < np; ++kp) {
+            const bf16_t* sK = smem + (kp & 1) * 2 * SC::TILE;
+            const bf16_t* sV = sK + SC::TILE;
+            const int kb = 64 * kp;
+            if (kp + 1 < np) {
+                stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, kb + 64, z.nk);
+                nbits = key_bits(a, z, kb + 64, lane);
             }
-            __syncthreads();
-            for (int kp = kp0; kp < kp1; ++kp) {
-                const bf16_t* sK = smem + (kp & 1) * 2 * SC::TILE;
-                const bf16_t* sV = sK + SC::TILE;
-                const int kb = 64 * kp;
-                if (kp + 1 < kp1) {
-                    stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, kb + 64, z.nk);
-                    nbits = key_bits(a, z, kb + 64, lane);
+            const bool left = kb + 63 - plo <= -a.far, right = kb - phi >= a.far;
+            if (live && bits != 0 && !(a.causal && kb > phi)) {
+                const int idx0 = kb + 4 * hh - pos + a.far + PAD;
+                uint64_t vis = bits;
+                if (a.causal) {
+                    const int c = pos - kb;
+                    vis = c < 0 ? 0 : (c >= 63 ? vis : vis & ((2ull << c) - 1));
                 }
-                const bool left = kb + 63 - plo <= -a.far, right = kb - phi >= a.far;
-                if (live && bits != 0 && !(a.causal && kb > phi) && !(BAND && (left || right))) {
-                    const int idx0 = kb + 4 * hh - pos + a.far + PAD;
-                    uint64_t vis = bits;
-                    if (a.causal) {
-                        const int c = pos - kb;
-                        vis = c < 0 ? 0 : (c >= 63 ? vis : vis & ((2ull << c) - 1));
+                vis >>= 4 * hh;
+                const bool edge = bits != ~0ull || (a.causal && kb + 63 > plo);
+                const float nf = left ? nl + cleft : (right ? nl + cright : nl);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {              // the two 32-key tiles, one after the other (register budget)
+                    const bf16_t* tK = sK + half * 32 * DP;
+                    const bf16_t* tV = sV + half * 32 * DP;
+                    const int idx = idx0 + 32 * half;
+                    f32x16_t sc, dp = MFMA32(nat_frag<DP>(tV, r, hh, 0), df[0], ndel);     // dP - delta: the accumulator starts at -delta
+                    if (left || right) sc = MFMA32(nat_frag<DP>(tK, r, hh, 0), qf[0], splat16(0.f));
+                    else sc = MFMA32(nat_frag<DP>(tK, r, hh, 0), qf[0], bias16(bv, idx));
+#pragma unroll
+                    for (int s = 1; s < KS; ++s) {
+                        sc = MFMA32(nat_frag<DP>(tK, r, hh, s), qf[s], sc);
+                        dp = MFMA32(nat_frag<DP>(tV, r, hh, s), df[s], dp);
                     }
-                    vis >>= 4 * hh;
-                    const bool edge = bits != ~0ull || (a.causal && kb + 63 > plo);
-                    const float nf = left ? nl + cleft : (right ? nl + cright : nl);
+                    float p[16], ds[16];
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {              // the two 32-key tiles, one after the other (register budget)
-                        const bf16_t* tK = sK + half * 32 * DP;
-                        const bf16_t* tV = sV + half * 32 * DP;
-                        const int idx = idx0 + 32 * half;
-                        f32x16_t sc, dp = MFMA32(nat_frag<DP>(tV, r, hh, 0), df[0], ndel);     // dP - delta: the accumulator starts at -delta
-                        if (left || right) sc = MFMA32(nat_frag<DP>(tK, r, hh, 0), qf[0], splat16(0.f));
-                        else sc = MFMA32(nat_frag<DP>(tK, r, hh, 0), qf[0], bias16(bv, idx));
-#pragma unroll
-                        for (int s = 1; s < KS; ++s) {
-                            sc = MFMA32(nat_frag<DP>(tK, r, hh, s), qf[s], sc);
-                            dp = MFMA32(nat_frag<DP>(tV, r, hh, s), df[s], dp);
-                        }
-                        float p[16], ds[16];
+                    for (int reg = 0; reg < 16; ++reg) {
+                        p[reg] = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nf));
+                        ds[reg] = p[reg] * dp[reg];
+                    }
+                    if (edge) {
+                        asm volatile("");                           // (kept a branch: as selects these run in every tile)
 #pragma unroll
                         for (int reg = 0; reg < 16; ++reg) {
-                            p[reg] = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nf));
-                            ds[reg] = p[reg] * dp[reg];
-                        }
-                        if (edge) {
-                            asm volatile("");                           // (kept a branch: as selects these run in every tile)
-#pragma unroll
-                            for (int reg = 0; reg < 16; ++reg) {
-                                const bool on = (vis >> (32 * half + ACC_ROW(reg, 0))) & 1;
-                                p[reg] = on ? p[reg] : 0.f;
-                                ds[reg] = on ? ds[reg] : 0.f;
-                            }
-                        }
-                        if (BAND) {
-#pragma unroll
-                            for (int reg = 0; reg < 16; ++reg) {
-                                bn += p[reg];
-                                __hip_atomic_fetch_add(mine + idx + ACC_ROW(reg, 0), ds[reg], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                            }
-                        } else {
-                            if (TAB) {
-                                float t = 0.f;
-#pragma unroll
-                                for (int reg = 0; reg < 16; ++reg) t += ds[reg];
-                                all.add(t);
-                                if (left) sl.add(t);
-                                if (right) {
-                                    sr.add(t);
-#pragma unroll
-                                    for (int reg = 0; reg < 16; ++reg) br += p[reg];
-                                }
-                            }
-                            const bf16x8_t d0 = pack8(ds), d1 = pack8(ds + 8);
-#pragma unroll
-                            for (int dt = 0; dt < DT; ++dt) {
-                                dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 0, hh, r), d0, dq[dt]);
-                                dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 1, hh, r), d1, dq[dt]);
-                            }
+                            const bool on = (vis >> (32 * half + ACC_ROW(reg, 0))) & 1;
+                            p[reg] = on ? p[reg] : 0.f;
+                            ds[reg] = on ? ds[reg] : 0.f;
                         }
                     }
+                    if (TAB) {
+                        float t = 0.f;
+#pragma unroll
+                        for (int reg = 0; reg < 16; ++reg) t += ds[reg];
+                        all.add(t);
+                        if (left) sl.add(t);
+                        if (right) sr.add(t);
+                        if (!left) {                            // the probability behind the left border is what is left of one
+                            float b = 0.f;
+#pragma unroll
+                            for (int reg = 0; reg < 16; ++reg) b += p[reg];
+                            if (right) br += b; else bn += b;
+                        }
+                    }
+                    const bf16x8_t d0 = pack8(ds), d1 = pack8(ds + 8);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 0, hh, r), d0, dq[dt]);
+                        dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 1, hh, r), d1, dq[dt]);
+                    }
                 }
-                if (kp + 1 < kp1) stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, nbits);
-                bits = nbits;
-                __syncthreads();
             }
-        };
-        walk(0, np, std::false_type{});
+            if (kp + 1 < np) stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, nbits);
+            bits = nbits;
+            __syncthreads();
+        }
         bf16_t* dqp = a.dQ + ((int64_t)z.q0 + q) * a.lddq + h * D;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) store_tile32(dqp + 32 * dt, dq[dt], a.scale, hh, qok);
         if (TAB) {
-            float rs = all.s - all.c;
-            rs = half_sum(rs);
-            delta += rs;                                                // rowsum(P dP) to fp32
-            int lo = qb + shift - a.far - 62, hi = qb + 32 * NW - 1 + shift + a.far;    // keys that can be near a query of the block
-            lo = lo < 0 ? 0 : lo >> 6;
-            hi = hi < 0 ? 0 : (hi >> 6) + 1;
-            walk(lo < np ? lo : np, hi < np ? hi : np, std::true_type{});
+            const float rs = half_sum(all.s - all.c);
             br = half_sum(br);
             bn = half_sum(bn);
             const float bl = fmaxf(1.f - br - bn, 0.f);
-            if (hh == 0) {                                              // once per row: the halves' sums of dS enter below, one per lane
+            if (hh == 0 && seen) {                                      // once per row: the halves' sums of dS enter below, one per lane
                 tab_l -= rs * bl;
                 tab_r -= rs * br;
             }
+            delta += rs;                                                // rowsum(P dP) to fp32
             tab_l += sl.s - sl.c;
             tab_r += sr.s - sr.c;
         }
         if (qok && hh == 0) a.delta[(int64_t)h * a.Tq + qrow] = delta;
-        __syncthreads();
     }
     if (TAB) {
         tab_l = wave_sum<64>(tab_l);
         tab_r = wave_sum<64>(tab_r);
-        if (lane == 0) { mine[0] += tab_l; mine[blen - 1] += tab_r; }   // ends of the array: distances behind the border
         __syncthreads();
-        for (int i = tid; i < blen; i += NTHR) {
+        if (lane == 0) { bv[2 * wave] = tab_l; bv[2 * wave + 1] = tab_r; }
+        __syncthreads();
+        if (tid < 2) {
             float t = 0.f;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) t += diag[w * blen + i];
-            diag[i] = t;
-        }
-        __syncthreads();
-        // a bucket is one run of distances (the last of a side runs to the array's end): first distances in plan[2 far + 1 ..]
-        const int32_t* border = a.plan + 2 * a.far + 1;
-        const int half = a.causal ? a.NB : a.NB / 2;
-        float* out = a.part + (((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * a.H + h) * a.NB;
-        for (int b = wave; b < a.NB; b += NW) {
-            const int side = b >= half, i = side ? b - half : b;
-            int lo = border[i], hi = i + 1 < half ? border[i + 1] : a.far + PAD + 1;
-            if (side && lo == 0) lo = 1;                                // distance 0 belongs to the first side
-            lo = lo < 0 ? 0 : lo;
-            hi = hi < a.far + PAD + 1 ? hi : a.far + PAD + 1;
-            float t = 0.f;
-            for (int d = lo + lane; d < hi; d += 64) t += diag[a.far + PAD + (side ? d : -d)];
-            t = wave_sum<64>(t);
-            if (lane == 0) out[b] = t;
+            for (int w = 0; w < NW; ++w) t += bv[2 * w + tid];
+            a.part[(((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * a.H + h) * 2 + tid] = t;
         }
     }
 }
 
-// dtable[b][h] = sum over the blocks' rows, in order
-__global__ void __launch_bounds__(256) relattn_dtable_kernel(const float* part, float* dtable, int rows, int H, int NB) {
+// ------------------------------------------------------------------------------------------------ backward: table gradient, the band
+// The tiles that relattn_dq_kernel does not count as lying behind a border.  A wave walks ALONG a diagonal of 32 x 32 tiles (query tile i, key tile
+// i + t, t fixed): an accumulator register then holds one distance for the whole walk, so summing dS by distance costs one addition per element
+// and the bias is 16 registers loaded once; only at the end do the 16 x 64 sums fold into 63 distances.  A block = four neighbouring diagonals
+// and `chunk` query tiles of one (sequence, head): per step it stages one new query tile (Q, dO) and one new key tile (K, V; a ring of five).
+// Bound by the LDS reads of the four operands (nothing is reused across steps); measured against LDS additions per element in the dQ
+// kernel, which took four times as long.
+template <int D>
+__global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups, int chunk) {
+    constexpr int KS = D / 16, DP = D + 8, ROWP = D / 8, TILE = 32 * DP, PER = 32 * ROWP / 128;     // pieces per thread of one pair of tiles
+    extern __shared__ __attribute__((aligned(16))) bf16_t smem[];       // K / V ring [5][2][32][DP], Q / dO [2][2][32][DP], sums [4][64]
+    bf16_t* sQ = smem + 10 * TILE;
+    float* sums = reinterpret_cast<float*>(sQ + 4 * TILE);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, hh = lane >> 5;
+    const int h = blockIdx.y, hk = h / (a.H / a.Hkv);
+    const int tg = blockIdx.x % tgroups, ch = blockIdx.x / tgroups, nch = gridDim.x / tgroups;
+    const Seq z = seq_of(a, blockIdx.z);
+    const int shift = z.nk - z.nq;
+    const int nqt = (z.nq + 31) >> 5;
+    // diagonals that can hold an element counted here: from t_min on, four to a block
+    const int t0 = ((shift - a.far - 62) >> 5) + 4 * tg, t = t0 + wave;
+    const int tmax = a.causal ? (shift + 31) >> 5 : (shift + a.far + 62) >> 5;
+    f32x16_t acc = splat16(0.f);
+    if (t0 <= tmax && z.nk > 0) {
+        const bool mine = t <= tmax;
+        // bias of the wave's distances: key - query = 32 t - shift + ACC_ROW - r
+        f32x16_t cb;
+#pragma unroll
+        for (int reg = 0; reg < 16; ++reg) {
+            int d = 32 * t - shift + ACC_ROW(reg, hh) - r;
+            d = d < -a.far ? -a.far : (d > a.far ? a.far : d);
+            int b = a.plan[d + a.far];
+            b = b < 0 ? 0 : (b < a.NB ? b : a.NB - 1);
+            cb[reg] = raw_bias(a.table[(int64_t)b * a.H + h], a.inv_scale);
+        }
+        const bf16_t* Kb = a.K + (int64_t)z.k0 * a.ldk + hk * D;
+        const bf16_t* Vb = a.V + (int64_t)z.k0 * a.ldv + hk * D;
+        const bf16_t* Qb = a.Q + (int64_t)z.q0 * a.ldq + h * D;
+        const bf16_t* Db = a.dO + (int64_t)z.q0 * a.lddo + h * D;
+        const float* lseb = a.lse + (int64_t)h * a.Tq + z.q0;
+        const float* delb = a.delta + (int64_t)h * a.Tq + z.q0;
+        const int half = tid >> 7, ti = tid & 127;                      // first or second tensor of a pair
+        auto fetch = [&](u32x4_t (&v)[PER], const bf16_t* t0p, int64_t ld0, const bf16_t* t1p, int64_t ld1, int row0, int n) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int id = ti + 128 * i, rr = id / ROWP, c = id - rr * ROWP;
+                int row = row0 + rr;
+                row = row < 0 ? 0 : (row < n ? row : n - 1);
+                v[i] = *reinterpret_cast<const u32x4_t*>((half ? t1p + (int64_t)row * ld1 : t0p + (int64_t)row * ld0) + 8 * c);
+            }
+        };
+        auto commit = [&](bf16_t* s, const u32x4_t (&v)[PER], uint32_t valid) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int id = ti + 128 * i, rr = id / ROWP, c = id - rr * ROWP;
+                u32x4_t w = v[i];
+                if (valid != ~0u && !((valid >> rr) & 1)) w = (u32x4_t){0u, 0u, 0u, 0u};
+                *reinterpret_cast<u32x4_t*>(s + half * TILE + rr * DP + 8 * c) = w;
+            }
+        };
+        auto kbits = [&](int kt) -> uint32_t {                          // keys of tile kt that exist and are not masked
+            const int key = 32 * kt + (lane & 31);
+            bool ok = key >= 0 && key < z.nk;
+            if (a.kmask != nullptr && ok) ok = a.kmask[(int64_t)z.k0 + key] != 0;
+            return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)__builtin_amdgcn_ballot_w64(ok));
+        };
+        auto qbits = [&](int i) -> uint32_t {
+            const int left = z.nq - 32 * i;
+            return left >= 32 ? ~0u : (1u << left) - 1;
+        };
+        for (int first = ch * chunk; first < nqt; first += nch * chunk) {
+            const int last = first + chunk < nqt ? first + chunk : nqt;
+            u32x4_t kv[PER], qd[PER];
+            __syncthreads();
+            for (int j = 0; j < 4; ++j) {
+                fetch(kv, Kb, a.ldk, Vb, a.ldv, 32 * (first + t0 + j), z.nk);
+                commit(smem + j * 2 * TILE, kv, kbits(first + t0 + j));
+            }
+            fetch(qd, Qb, a.ldq, Db, a.lddo, 32 * first, z.nq);
+            commit(sQ, qd, qbits(first));
+            auto stat = [&](int i, float& nl, float& nd) {
+                const int q = 32 * i + r;
+                const float l = q < z.nq ? lseb[q] : -INFINITY;
+                nl = l == -INFINITY ? -INFINITY : -l * LOG2E;
+                nd = q < z.nq ? -delb[q] : 0.f;
+            };
+            float nl, nd, nl2 = 0.f, nd2 = 0.f;
+            stat(first, nl, nd);
+            uint32_t bits = kbits(first + t), nbits = 0, sbits = 0;
+            int slot = 0;                                               // ring slot of the block's first diagonal
+            __syncthreads();
+            for (int i = first; i < last; ++i) {
+                const bool more = i + 1 < last;
+                if (more) {
+                    fetch(kv, Kb, a.ldk, Vb, a.ldv, 32 * (i + 1 + t0 + 3), z.nk);
+                    fetch(qd, Qb, a.ldq, Db, a.lddo, 32 * (i + 1), z.nq);
+                    stat(i + 1, nl2, nd2);
+                    sbits = kbits(i + 1 + t0 + 3);
+                    nbits = kbits(i + 1 + t);
+                }
+                const int kt = i + t, kb = (32 * kt) & ~63, plo = 32 * i + shift, phi = plo + 31;
+                if (mine && bits != 0 && kb + 63 - plo > -a.far && kb - phi < a.far) {
+                    const int w = slot + wave < 5 ? slot + wave : slot + wave - 5;
+                    const bf16_t* tK = smem + w * 2 * TILE;
+                    const bf16_t* tV = tK + TILE;
+                    const bf16_t* tQ = sQ + ((i - first) & 1) * 2 * TILE;
+                    const bf16_t* tD = tQ + TILE;
+                    f32x16_t sc = cb, dp = splat16(nd);
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        sc = MFMA32(nat_frag<DP>(tK, r, hh, s), nat_frag<DP>(tQ, r, hh, s), sc);
+                        dp = MFMA32(nat_frag<DP>(tV, r, hh, s), nat_frag<DP>(tD, r, hh, s), dp);
+                    }
+                    float ds[16];
+#pragma unroll
+                    for (int reg = 0; reg < 16; ++reg) ds[reg] = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nl)) * dp[reg];
+                    if (bits != ~0u || (a.causal && 32 * kt + 31 > plo)) {
+                        asm volatile("");
+                        uint32_t vis = bits;
+                        if (a.causal) {
+                            const int c = plo + r - 32 * kt;
+                            vis = c < 0 ? 0 : (c >= 31 ? vis : vis & ((2u << c) - 1));
+                        }
+                        vis >>= 4 * hh;
+#pragma unroll
+                        for (int reg = 0; reg < 16; ++reg) ds[reg] = (vis >> ACC_ROW(reg, 0)) & 1 ? ds[reg] : 0.f;
+                    }
+#pragma unroll
+                    for (int reg = 0; reg < 16; ++reg) acc[reg] += ds[reg];
+                }
+                if (more) {
+                    const int w = slot + 4 < 5 ? slot + 4 : slot - 1;
+                    commit(smem + w * 2 * TILE, kv, sbits);
+                    commit(sQ + ((i + 1 - first) & 1) * 2 * TILE, qd, qbits(i + 1));
+                }
+                slot = slot + 1 < 5 ? slot + 1 : 0;
+                nl = nl2; nd = nd2; bits = nbits;
+                __syncthreads();
+            }
+        }
+    }
+    // ---- distances: the wave's instructions stay in order, so each sum has one order
+    if (tid < 256) sums[tid] = 0.f;
+    __syncthreads();
+#pragma unroll
+    for (int reg = 0; reg < 16; ++reg)
+        __hip_atomic_fetch_add(sums + 64 * wave + ACC_ROW(reg, hh) - r + 31, acc[reg], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    __syncthreads();
+    // a bucket is one run of distances (the last of a side has no end): first distances in plan[2 far + 1 ..].  Slot u of the block's 160
+    // holds distance base + u, from two neighbouring diagonals.
+    const int32_t* border = a.plan + 2 * a.far + 1;
+    const int half = a.causal ? a.NB : a.NB / 2, base = 32 * t0 - shift - 31;
+    float* out = a.part + (((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * a.H + h) * a.NB;
+    for (int b = wave; b < a.NB; b += 4) {
+        const int side = b >= half, i = side ? b - half : b;
+        int lo = border[i], hi = i + 1 < half ? border[i + 1] : 1 << 30;    // distances lo .. hi - 1 of the bucket's side
+        if (side && lo == 0) lo = 1;                                    // distance 0 belongs to the first side
+        const int from = side ? lo : (hi == 1 << 30 ? -(1 << 30) : 1 - hi), to = side ? hi : 1 - lo;     // as signed distances, from .. to - 1
+        int u0 = from - base, u1 = to - base;
+        u0 = u0 < 0 ? 0 : u0;
+        u1 = u1 > 160 ? 160 : u1;
+        float v = 0.f;
+        for (int u = u0 + lane; u < u1; u += 64) {
+            const int w = u >> 5, j = u & 31;                           // wave w holds it at 32 w + j - 32 w = j, wave w - 1 at j + 32
+            if (w < 4) v += sums[64 * w + j];
+            if (w > 0) v += sums[64 * (w - 1) + 32 + j];
+        }
+        v = wave_sum<64>(v);
+        if (lane == 0) out[b] = v;
+    }
+}
+
+// dtable[b][h] = sum of the band's rows, and of the rows behind the borders where b is a side's last bucket, in order
+__global__ void __launch_bounds__(256) relattn_dtable_kernel(const float* band, int nband, const float* behind, int nbehind, float* dtable, int H, int NB, int causal) {
     __shared__ float s[256];
     const int h = blockIdx.x, b = blockIdx.y;
     float t = 0.f;
-    for (int i = threadIdx.x; i < rows; i += 256) t += part[((int64_t)i * H + h) * NB + b];
+    for (int i = threadIdx.x; i < nband; i += 256) t += band[((int64_t)i * H + h) * NB + b];
+    const int left = causal ? NB - 1 : NB / 2 - 1;
+    if (b == left || b == NB - 1)
+        for (int i = threadIdx.x; i < nbehind; i += 256) t += behind[((int64_t)i * H + h) * 2 + (b == left ? 0 : 1)];
     s[threadIdx.x] = t;
     __syncthreads();
     for (int w = 128; w > 0; w >>= 1) {
@@ -1001,7 +1139,7 @@ RP make_rp(const stg_relattn_args* a) {
 }
 
 int64_t lds_fwd(int D, int far) { return (int64_t)4 * 64 * (D + 8) * 2 + (2 * (far + PAD) + 1) * 4; }
-int64_t lds_dq(int D, int far, bool tab) { return (int64_t)4 * 64 * (D + 8) * 2 + (2 * (far + PAD) + 1) * 4 * (tab ? 5 : 1); }
+int64_t lds_band(int D) { return (int64_t)14 * 32 * (D + 8) * 2 + 256 * 4; }
 int64_t lds_dkv(int D, int far) { return (int64_t)2 * (2 * 64 * (D + 8) + 256) * 2 + (2 * (far + PAD) + 1) * 4; }
 int64_t lds_dec(int D, int NB) { return (int64_t)8 * 32 * (D + 8) * 2 + (int64_t)NB * 32 * 4; }
 
@@ -1030,7 +1168,17 @@ int launch_dq(const RP& p, int max_q, hipStream_t st) {
     STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_bwd: cannot reserve LDS");
     const dim3 grid(grid_tiles(max_q, p.Tq, 128), p.H, p.S + (p.zero_tail ? 1 : 0));
     if (grid.z == 0) return 0;
-    k<<<grid, 256, lds_dq(D, p.far, TAB), st>>>(p);
+    k<<<grid, 256, lds_fwd(D, p.far), st>>>(p);
+    STG_LAUNCH_CHECK();
+    return 0;
+}
+template <int D>
+int launch_band(const RP& p, int blocks, int tgroups, int chunk, hipStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    auto k = relattn_band_kernel<D>;
+    STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_bwd: cannot reserve LDS");
+    if (p.S == 0) return 0;
+    k<<<dim3(blocks, p.H, p.S), 256, lds_band(D), st>>>(p, tgroups, chunk);
     STG_LAUNCH_CHECK();
     return 0;
 }
@@ -1076,6 +1224,7 @@ int run_dq(const RP& p, int D, int max_q, hipStream_t st) {
     BY_DIM(D, (launch_dq<DIM, false>(p, max_q, st)));
 }
 int run_dkv(const RP& p, int D, int max_k, hipStream_t st) { BY_DIM(D, (launch_dkv<DIM>(p, max_k, st))); }
+int run_band(const RP& p, int D, int blocks, int tgroups, int chunk, hipStream_t st) { BY_DIM(D, (launch_band<DIM>(p, blocks, tgroups, chunk, st))); }
 int run_decode(const DP_& p, int D, hipStream_t st) { BY_DIM(D, (launch_decode<DIM>(p, st))); }
 
 // keys per block of the single-token form: enough blocks for the chip, at least 128 keys (one 32-key tile for each of the four waves)
@@ -1097,10 +1246,26 @@ extern "C" int stg_relattn_fwd(const stg_relattn_args* a, void* stream) {
     return run_fwd(make_rp(a), a->D, a->max_q, (hipStream_t)stream);
 }
 
+// The band's grid: groups of four diagonals, and enough chunks of query tiles that about 2048 blocks exist (a chunk of at least 8 tiles pays
+// for the four key tiles a block stages before its first step).
+static void band_grid(const stg_relattn_args* a, int& tgroups, int& chunk, int& blocks) {
+    const int nt = ((a->causal ? a->far + 62 + 31 : 2 * a->far + 124) >> 5) + 2;
+    tgroups = (nt + 3) / 4;
+    const int64_t tiles = grid_tiles(a->max_q, a->Tq, 32), want = 2048 / ((int64_t)tgroups * a->H * (a->S > 0 ? a->S : 1)) + 1;
+    int64_t c = (tiles + want - 1) / want;
+    c = c < 8 ? 8 : c;
+    chunk = (int)c;
+    blocks = (int)(tgroups * ((tiles + c - 1) / c));
+}
+
 extern "C" int64_t stg_relattn_bwd_ws_floats(const stg_relattn_args* a, int want_table) {
-    if (a == nullptr || a->S < 0 || a->H <= 0 || a->Tq < 0 || a->num_buckets <= 0) return -1;
+    if (a == nullptr || a->S < 0 || a->H <= 0 || a->Tq < 0 || a->num_buckets <= 0 || a->far <= 0) return -1;
     int64_t n = (int64_t)a->H * a->Tq;
-    if (want_table) n += (int64_t)grid_tiles(a->max_q, a->Tq, 128) * a->S * a->H * a->num_buckets;
+    if (want_table) {
+        int tg, chunk, blocks;
+        band_grid(a, tg, chunk, blocks);
+        n += (int64_t)a->S * a->H * ((int64_t)grid_tiles(a->max_q, a->Tq, 128) * 2 + (int64_t)blocks * a->num_buckets);
+    }
     return n > 0 ? n : 1;
 }
 
@@ -1119,12 +1284,20 @@ extern "C" int stg_relattn_bwd(const stg_relattn_args* a, const void* dO, int64_
     p.dO = (const bf16_t*)dO; p.lddo = lddo; p.dQ = (bf16_t*)dQ; p.lddq = lddq;
     p.dK = (bf16_t*)dK; p.lddk = lddk; p.dV = (bf16_t*)dV; p.lddv = lddv;
     p.delta = ws;
-    p.part = dtable ? ws + (int64_t)a->H * a->Tq : nullptr;
+    // table gradient: the dQ kernel's rows (two sums each), then the band's rows
+    const int nbehind = grid_tiles(a->max_q, a->Tq, 128) * a->S;
+    float* behind = ws + (int64_t)a->H * a->Tq;
+    float* band = behind + (int64_t)nbehind * a->H * 2;
+    int tgroups = 0, chunk = 0, blocks = 0;
+    band_grid(a, tgroups, chunk, blocks);
+    p.part = dtable ? behind : nullptr;
     if (a->Tq > 0) { const int e = run_dq(p, a->D, a->max_q, st); if (e) return e; }
     if (a->Tk > 0) { const int e = run_dkv(p, a->D, a->max_k, st); if (e) return e; }
     if (dtable) {
-        const int rows = a->Tq > 0 ? grid_tiles(a->max_q, a->Tq, 128) * a->S : 0;
-        relattn_dtable_kernel<<<dim3(a->H, a->num_buckets), 256, 0, st>>>(p.part, dtable, rows, a->H, a->num_buckets);
+        p.part = band;
+        if (a->Tq > 0) { const int e = run_band(p, a->D, blocks, tgroups, chunk, st); if (e) return e; }
+        relattn_dtable_kernel<<<dim3(a->H, a->num_buckets), 256, 0, st>>>(band, a->Tq > 0 ? blocks * a->S : 0, behind, a->Tq > 0 ? nbehind : 0, dtable, a->H,
+                                                                          a->num_buckets, a->causal != 0);
         STG_LAUNCH_CHECK();
     }
     return 0;
