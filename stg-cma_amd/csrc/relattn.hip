@@ -566,15 +566,17 @@ __global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups,
     f32x16_t acc = splat16(0.f);
     if (t0 <= tmax && z.nk > 0) {
         const bool mine = t <= tmax;
-        // bias of the wave's distances: key - query = 32 t - shift + ACC_ROW - r
+        // bias of the wave's 63 distances, key - query = 32 t - shift + ACC_ROW - r: one lookup per lane, then 16 registers per lane
         f32x16_t cb;
-#pragma unroll
-        for (int reg = 0; reg < 16; ++reg) {
-            int d = 32 * t - shift + ACC_ROW(reg, hh) - r;
+        {
+            int d = 32 * t - shift + lane - 31;
             d = d < -a.far ? -a.far : (d > a.far ? a.far : d);
             int b = a.plan[d + a.far];
             b = b < 0 ? 0 : (b < a.NB ? b : a.NB - 1);
-            cb[reg] = raw_bias(a.table[(int64_t)b * a.H + h], a.inv_scale);
+            sums[64 * wave + lane] = raw_bias(a.table[(int64_t)b * a.H + h], a.inv_scale);
+            __syncthreads();
+#pragma unroll
+            for (int reg = 0; reg < 16; ++reg) cb[reg] = sums[64 * wave + ACC_ROW(reg, hh) - r + 31];
         }
         const bf16_t* Kb = a.K + (int64_t)z.k0 * a.ldk + hk * D;
         const bf16_t* Vb = a.V + (int64_t)z.k0 * a.ldv + hk * D;
@@ -613,34 +615,30 @@ __global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups,
         };
         for (int first = ch * chunk; first < nqt; first += nch * chunk) {
             const int last = first + chunk < nqt ? first + chunk : nqt;
-            u32x4_t kv[PER], qd[PER];
-            __syncthreads();
-            for (int j = 0; j < 4; ++j) {
-                fetch(kv, Kb, a.ldk, Vb, a.ldv, 32 * (first + t0 + j), z.nk);
-                commit(smem + j * 2 * TILE, kv, kbits(first + t0 + j));
-            }
-            fetch(qd, Qb, a.ldq, Db, a.lddo, 32 * first, z.nq);
-            commit(sQ, qd, qbits(first));
-            auto stat = [&](int i, float& nl, float& nd) {
+            // what a step stages is fetched two steps ahead (a step computes for ~600 cycles, an L2 or MALL load takes longer): two register sets
+            struct Next { u32x4_t kv[PER], qd[PER]; float l, d; uint32_t sbits, bits; } n0, n1;
+            auto ahead = [&](int i, Next& n) {                          // query tile i, its new key tile, the wave's key bits
+                fetch(n.kv, Kb, a.ldk, Vb, a.ldv, 32 * (i + t0 + 3), z.nk);
+                fetch(n.qd, Qb, a.ldq, Db, a.lddo, 32 * i, z.nq);
                 const int q = 32 * i + r;
-                const float l = q < z.nq ? lseb[q] : -INFINITY;
-                nl = l == -INFINITY ? -INFINITY : -l * LOG2E;
-                nd = q < z.nq ? -delb[q] : 0.f;
+                n.l = q < z.nq ? lseb[q] : -INFINITY;
+                n.d = q < z.nq ? delb[q] : 0.f;
+                n.sbits = kbits(i + t0 + 3);
+                n.bits = kbits(i + t);
             };
-            float nl, nd, nl2 = 0.f, nd2 = 0.f;
-            stat(first, nl, nd);
-            uint32_t bits = kbits(first + t), nbits = 0, sbits = 0;
             int slot = 0;                                               // ring slot of the block's first diagonal
-            __syncthreads();
-            for (int i = first; i < last; ++i) {
-                const bool more = i + 1 < last;
-                if (more) {
-                    fetch(kv, Kb, a.ldk, Vb, a.ldv, 32 * (i + 1 + t0 + 3), z.nk);
-                    fetch(qd, Qb, a.ldq, Db, a.lddo, 32 * (i + 1), z.nq);
-                    stat(i + 1, nl2, nd2);
-                    sbits = kbits(i + 1 + t0 + 3);
-                    nbits = kbits(i + 1 + t);
-                }
+            float nl, nd;
+            uint32_t bits;
+            auto enter = [&](int i, const Next& n, int kslot) {         // the step's tiles into LDS, its statistics into registers
+                commit(smem + kslot * 2 * TILE, n.kv, n.sbits);
+                commit(sQ + ((i - first) & 1) * 2 * TILE, n.qd, qbits(i));
+            };
+            auto take = [&](const Next& n) {
+                nl = n.l == -INFINITY ? -INFINITY : -n.l * LOG2E;
+                nd = -n.d;
+                bits = n.bits;
+            };
+            auto compute = [&](int i) {
                 const int kt = i + t, kb = (32 * kt) & ~63, plo = 32 * i + shift, phi = plo + 31;
                 if (mine && bits != 0 && kb + 63 - plo > -a.far && kb - phi < a.far) {
                     const int w = slot + wave < 5 ? slot + wave : slot + wave - 5;
@@ -671,45 +669,72 @@ __global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups,
 #pragma unroll
                     for (int reg = 0; reg < 16; ++reg) acc[reg] += ds[reg];
                 }
-                if (more) {
-                    const int w = slot + 4 < 5 ? slot + 4 : slot - 1;
-                    commit(smem + w * 2 * TILE, kv, sbits);
-                    commit(sQ + ((i + 1 - first) & 1) * 2 * TILE, qd, qbits(i + 1));
+            };
+            {
+                u32x4_t w[3][PER];
+                uint32_t ok[3];
+                for (int j = 0; j < 3; ++j) fetch(w[j], Kb, a.ldk, Vb, a.ldv, 32 * (first + t0 + j), z.nk);
+                ahead(first, n0);
+                for (int j = 0; j < 3; ++j) ok[j] = kbits(first + t0 + j);
+                __syncthreads();
+                for (int j = 0; j < 3; ++j) commit(smem + j * 2 * TILE, w[j], ok[j]);
+                enter(first, n0, 3);
+                take(n0);
+            }
+            if (first + 1 < last) ahead(first + 1, n1);
+            __syncthreads();
+            auto step = [&](int i, Next& next, Next& after) {           // next: fetched for step i + 1; after: free
+                if (i + 2 < last) ahead(i + 2, after);
+                compute(i);
+                if (i + 1 < last) {
+                    enter(i + 1, next, slot + 4 < 5 ? slot + 4 : slot - 1);
+                    take(next);
                 }
                 slot = slot + 1 < 5 ? slot + 1 : 0;
-                nl = nl2; nd = nd2; bits = nbits;
                 __syncthreads();
+            };
+            for (int i = first; i < last; i += 2) {
+                step(i, n1, n0);
+                if (i + 1 < last) step(i + 1, n0, n1);
             }
         }
     }
     // ---- distances: the wave's instructions stay in order, so each sum has one order
-    if (tid < 256) sums[tid] = 0.f;
+    __syncthreads();
+    sums[tid] = 0.f;
     __syncthreads();
 #pragma unroll
     for (int reg = 0; reg < 16; ++reg)
         __hip_atomic_fetch_add(sums + 64 * wave + ACC_ROW(reg, hh) - r + 31, acc[reg], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     __syncthreads();
-    // a bucket is one run of distances (the last of a side has no end): first distances in plan[2 far + 1 ..].  Slot u of the block's 160
-    // holds distance base + u, from two neighbouring diagonals.
-    const int32_t* border = a.plan + 2 * a.far + 1;
-    const int half = a.causal ? a.NB : a.NB / 2, base = 32 * t0 - shift - 31;
-    float* out = a.part + (((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * a.H + h) * a.NB;
-    for (int b = wave; b < a.NB; b += 4) {
-        const int side = b >= half, i = side ? b - half : b;
-        int lo = border[i], hi = i + 1 < half ? border[i + 1] : 1 << 30;    // distances lo .. hi - 1 of the bucket's side
-        if (side && lo == 0) lo = 1;                                    // distance 0 belongs to the first side
-        const int from = side ? lo : (hi == 1 << 30 ? -(1 << 30) : 1 - hi), to = side ? hi : 1 - lo;     // as signed distances, from .. to - 1
-        int u0 = from - base, u1 = to - base;
-        u0 = u0 < 0 ? 0 : u0;
-        u1 = u1 > 160 ? 160 : u1;
-        float v = 0.f;
-        for (int u = u0 + lane; u < u1; u += 64) {
-            const int w = u >> 5, j = u & 31;                           // wave w holds it at 32 w + j - 32 w = j, wave w - 1 at j + 32
-            if (w < 4) v += sums[64 * w + j];
-            if (w > 0) v += sums[64 * (w - 1) + 32 + j];
+    // slot u of the block's 160 holds distance 32 t0 - shift - 31 + u, from two neighbouring diagonals; a thread per bucket collects its slots in order
+    float v = 0.f;
+    int id = -1;
+    if (tid < 160) {
+        const int w = tid >> 5, j = tid & 31;                           // wave w holds it at j, wave w - 1 at 32 + j
+        if (w < 4) v += sums[64 * w + j];
+        if (w > 0) v += sums[64 * (w - 1) + 32 + j];
+        int d = 32 * t0 - shift - 31 + tid;
+        d = d < -a.far ? -a.far : (d > a.far ? a.far : d);
+        id = a.plan[d + a.far];
+    }
+    float* val = sums;                                                  // [160] values, then [160] buckets
+    int* ids = reinterpret_cast<int*>(sums + 160);
+    __syncthreads();
+    if (tid < 160) { val[tid] = v; ids[tid] = id; }
+    __syncthreads();
+    if (tid < a.NB) {
+        float t = 0.f;
+#pragma unroll 4
+        for (int u = 0; u < 160; u += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(val + u);
+            const int4 y = *reinterpret_cast<const int4*>(ids + u);
+            t += y.x == tid ? x.x : 0.f;
+            t += y.y == tid ? x.y : 0.f;
+            t += y.z == tid ? x.z : 0.f;
+            t += y.w == tid ? x.w : 0.f;
         }
-        v = wave_sum<64>(v);
-        if (lane == 0) out[b] = v;
+        a.part[(((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * a.H + h) * a.NB + tid] = t;
     }
 }
 
@@ -1139,7 +1164,7 @@ RP make_rp(const stg_relattn_args* a) {
 }
 
 int64_t lds_fwd(int D, int far) { return (int64_t)4 * 64 * (D + 8) * 2 + (2 * (far + PAD) + 1) * 4; }
-int64_t lds_band(int D) { return (int64_t)14 * 32 * (D + 8) * 2 + 256 * 4; }
+int64_t lds_band(int D) { return (int64_t)14 * 32 * (D + 8) * 2 + 320 * 4; }
 int64_t lds_dkv(int D, int far) { return (int64_t)2 * (2 * 64 * (D + 8) + 256) * 2 + (2 * (far + PAD) + 1) * 4; }
 int64_t lds_dec(int D, int NB) { return (int64_t)8 * 32 * (D + 8) * 2 + (int64_t)NB * 32 * 4; }
 
@@ -1246,14 +1271,14 @@ extern "C" int stg_relattn_fwd(const stg_relattn_args* a, void* stream) {
     return run_fwd(make_rp(a), a->D, a->max_q, (hipStream_t)stream);
 }
 
-// The band's grid: groups of four diagonals, and enough chunks of query tiles that about 2048 blocks exist (a chunk of at least 8 tiles pays
+// The band's grid: groups of four diagonals, and enough chunks of query tiles that about 2048 blocks exist (a chunk of at least 16 tiles pays
 // for the four key tiles a block stages before its first step).
 static void band_grid(const stg_relattn_args* a, int& tgroups, int& chunk, int& blocks) {
     const int nt = ((a->causal ? a->far + 62 + 31 : 2 * a->far + 124) >> 5) + 2;
     tgroups = (nt + 3) / 4;
     const int64_t tiles = grid_tiles(a->max_q, a->Tq, 32), want = 2048 / ((int64_t)tgroups * a->H * (a->S > 0 ? a->S : 1)) + 1;
     int64_t c = (tiles + want - 1) / want;
-    c = c < 8 ? 8 : c;
+    c = c < 16 ? 16 : c;
     chunk = (int)c;
     blocks = (int)(tgroups * ((tiles + c - 1) / c));
 }

@@ -2184,7 +2184,7 @@ class RelGeom:
         p = self._plans.get(device)
         if p is None:
             ids = [self.bucket(d if not self.causal else min(d, 0)) for d in range(-self.far, self.far + 1)]
-            p = self._plans[device] = torch.tensor(ids + self.borders, dtype=torch.int32, device=device)
+            p = self._plans[device] = torch.tensor(ids, dtype=torch.int32, device=device)
         return p
 
 
@@ -2246,12 +2246,16 @@ def relattn_fwd(g, q, k, v, table, cu_q, cu_k=None, *, max_q=None, max_k=None, k
     [S + 1] on the device: sequence s owns rows cu[s] .. cu[s + 1] - 1 (cu_k = None: cu_q); max_q / max_k: the longest sequences, known on the host
     (they size the launch; without them the whole tensor is assumed).  key_mask bool [Tk]: False hides a key.  The last query of a sequence stands
     at its last key.  Returns (o bf16 [Tq, H * D], lse fp32 [H, Tq] or None).  Rows behind the last sequence are zero in a fresh output and left alone in `out`."""
+    return _relattn_fwd(g, q, k, v, table, cu_q, cu_k, max_q, max_k, key_mask, out, want_lse)[:2]
+
+
+def _relattn_fwd(g, q, k, v, table, cu_q, cu_k, max_q, max_k, key_mask, out, want_lse):
     o = torch.empty((q.shape[0], g.H * g.D), dtype=BF16, device=q.device) if out is None else out
     lse = torch.empty((g.H, q.shape[0]), dtype=F32, device=q.device) if want_lse else None
     a = _rel_fill(g, q, k, v, o, lse, table, cu_q, cu_k, max_q, max_k, key_mask)
     a.zero_tail = int(out is None)
     _lib.check(_lib.lib().stg_relattn_fwd(C.byref(a), _stream()), "stg_relattn_fwd")
-    return o, lse
+    return o, lse, a
 
 
 def relattn_bwd(g, q, k, v, table, cu_q, cu_k, o, lse, do, *, max_q=None, max_k=None, key_mask=None, want_table=True):
@@ -2261,15 +2265,22 @@ def relattn_bwd(g, q, k, v, table, cu_q, cu_k, o, lse, do, *, max_q=None, max_k=
         raise RuntimeError("relattn_bwd: needs the forward's lse")
     a = _rel_fill(g, q, k, v, o, lse, table, cu_q, cu_k, max_q, max_k, key_mask)
     _rel_chk(do, "do", BF16, g.H * g.D, q.device, rows=q.shape[0])
-    dq = torch.empty((q.shape[0], g.H * g.D), dtype=BF16, device=q.device)
-    dk = torch.empty((k.shape[0], g.Hkv * g.D), dtype=BF16, device=q.device)
-    dv = torch.empty_like(dk)
-    dtable = torch.empty_like(table) if want_table else None
+    return _relattn_bwd(a, q.device, do, want_table)
+
+
+def _relattn_bwd(a, dev, do, want_table):
+    """The backward of a checked description (every pointer in place)."""
+    hd, kd = a.H * a.D, a.Hkv * a.D
+    dq = torch.empty((a.Tq, hd), dtype=BF16, device=dev)
+    dk = torch.empty((a.Tk, kd), dtype=BF16, device=dev)
+    dv = torch.empty((a.Tk, kd), dtype=BF16, device=dev)
+    dtable = torch.empty((a.num_buckets, a.H), dtype=F32, device=dev) if want_table else None
     a.zero_tail = 1
-    n = _lib.lib().stg_relattn_bwd_ws_floats(C.byref(a), int(want_table))
-    ws = torch.empty((max(n, 1),), dtype=F32, device=q.device)
-    _lib.check(_lib.lib().stg_relattn_bwd(C.byref(a), _p(do), _ld(do), _p(dq), _ld(dq), _p(dk), _ld(dk), _p(dv), _ld(dv), _p(dtable), _p(ws), ws.numel(),
-                                          _stream()), "stg_relattn_bwd")
+    lib = _lib.lib()
+    ref = C.byref(a)
+    n = lib.stg_relattn_bwd_ws_floats(ref, int(want_table))
+    ws = torch.empty((max(n, 1),), dtype=F32, device=dev)
+    _lib.check(lib.stg_relattn_bwd(ref, _p(do), _ld(do), _p(dq), hd, _p(dk), kd, _p(dv), kd, _p(dtable), _p(ws), n, _stream()), "stg_relattn_bwd")
     return dq, dk, dv, dtable
 
 
@@ -2363,6 +2374,10 @@ def norm_join_fwd(x, h, gate, post_w, post_b, pre_w, pre_b, *, kind="layer", alp
     x fp32 / bf16 [rows, C] (the residual stream), h bf16 [rows, C] (the block's output); gate None, one fp32 value, [C], or [groups, C] with
     rows_per_group consecutive rows to a group; weights fp32 [C] (biases may be None); kind "layer" or "rms".  Returns (x_new in x's type,
     y bf16, stats fp32 [rows, 4] for norm_join_bwd or None)."""
+    return _norm_join_fwd(x, h, gate, post_w, post_b, pre_w, pre_b, kind, alpha, eps, rows_per_group, want_stats)[:3]
+
+
+def _norm_join_fwd(x, h, gate, post_w, post_b, pre_w, pre_b, kind, alpha, eps, rows_per_group, want_stats):
     _chk2d(x, "x", x.dtype)
     x_new = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     y = torch.empty(x.shape, dtype=BF16, device=x.device)
@@ -2372,7 +2387,7 @@ def norm_join_fwd(x, h, gate, post_w, post_b, pre_w, pre_b, *, kind="layer", alp
     a.y, a.ldy = _p(y), _ld(y)
     a.x, a.ldx = _p(x), _ld(x)
     _lib.check(_lib.lib().stg_norm_join_fwd(C.byref(a), _stream()), "stg_norm_join_fwd")
-    return x_new, y, stats
+    return x_new, y, stats, a
 
 
 def norm_join_bwd(x_new, h, gate, post_w, post_b, pre_w, pre_b, stats, dy, dx_new=None, *, kind="layer", alpha=1.0, eps=1e-5, rows_per_group=None,
@@ -2388,22 +2403,38 @@ def norm_join_bwd(x_new, h, gate, post_w, post_b, pre_w, pre_b, stats, dy, dx_ne
     _rel_chk(dy, "dy", BF16, Cw, x_new.device, rows=R)
     if dx_new is not None:
         _rel_chk(dx_new, "dx_new", x_new.dtype, Cw, x_new.device, rows=R)
-    dx = torch.empty((R, Cw), dtype=x_new.dtype, device=x_new.device)
-    dh = torch.empty((R, Cw), dtype=BF16, device=x_new.device)
+    dx, dh, g = _norm_join_bwd(a, x_new.device, x_new.dtype, dy, dx_new, [None if t is None else t.shape for t in (post_w, post_b, pre_w, pre_b, gate)], want_params,
+                               want_gate)
+    return dict(zip(("dx", "dh", "dpost_w", "dpost_b", "dpre_w", "dpre_b", "dgate"), (dx, dh) + tuple(g)))
+
+
+def _norm_join_bwd(a, dev, dtype, dy, dx_new, shapes, want_params, want_gate):
+    """The backward of a checked description (every pointer in place); shapes of post_w, post_b, pre_w, pre_b, gate or None.  (dx, dh, their gradients)."""
+    R, Cw = a.rows, a.C
+    dx = torch.empty((R, Cw), dtype=dtype, device=dev)
+    dh = torch.empty((R, Cw), dtype=BF16, device=dev)
     lib = _lib.lib()
+    ref = C.byref(a)
+    groups = a.gate_kind == 3
     params = want_params or (want_gate and a.gate_kind in (1, 2))
-    n = lib.stg_norm_join_param_floats(C.byref(a))
-    dpar = torch.empty(((n + 3) // 4 * 4,), dtype=F32, device=x_new.device) if params else None
-    dgate = torch.empty_like(gate) if want_gate and a.gate_kind == 3 else None
-    nws = lib.stg_norm_join_bwd_ws_floats(C.byref(a)) if params or dgate is not None else 0
-    ws = torch.empty((nws,), dtype=F32, device=x_new.device) if nws else None
-    _lib.check(lib.stg_norm_join_bwd(C.byref(a), _p(dy), _ld(dy), _p(dx_new), _ld(dx_new) if dx_new is not None else 0, _p(dx), _ld(dx), _p(dh), _ld(dh),
-                                     _p(dpar), _p(dgate), _p(ws), nws, _stream()), "stg_norm_join_bwd")
-    out = {"dx": dx, "dh": dh, "dpost_w": None, "dpost_b": None, "dpre_w": None, "dpre_b": None, "dgate": dgate}
+    dpar = dgate = ws = None
+    nws = 0
+    if params:
+        dpar = torch.empty(((lib.stg_norm_join_param_floats(ref) + 3) // 4 * 4,), dtype=F32, device=dev)
+    if want_gate and groups:
+        dgate = torch.empty(shapes[4], dtype=F32, device=dev)
+    if params or dgate is not None:
+        nws = lib.stg_norm_join_bwd_ws_floats(ref)
+        ws = torch.empty((nws,), dtype=F32, device=dev)
+    _lib.check(lib.stg_norm_join_bwd(ref, _p(dy), _ld(dy), _p(dx_new), _ld(dx_new) if dx_new is not None else 0, _p(dx), Cw, _p(dh), Cw, _p(dpar), _p(dgate), _p(ws),
+                                     nws, _stream()), "stg_norm_join_bwd")
+    out = [None, None, None, None, dgate]
     if params:
         at = 0
-        for name, t in (("dpost_w", post_w), ("dpost_b", post_b), ("dpre_w", pre_w), ("dpre_b", pre_b), ("dgate", gate if a.gate_kind in (1, 2) else None)):
-            if t is not None:
-                out[name] = dpar[at:at + t.numel()].view(t.shape)
-                at += t.numel()
-    return out
+        for i, sh in enumerate(shapes):
+            if sh is not None and not (i == 4 and groups):
+                n = sh[0] if len(sh) else 1
+                t = dpar[at:at + n]
+                out[i] = t if len(sh) == 1 else t.view(sh)
+                at += n
+    return dx, dh, out
