@@ -644,7 +644,7 @@ int stg_bn_bwd(const void* x, const void* dy, const float* mean, const float* rs
  *
  * x_ij = scale q_i.k_j + table[bucket(j - p_i)][h], p_i = i + (n_k - n_q) (the last query stands at the last key), P = softmax over the visible
  * keys, O = P V.  A key is hidden by key_mask (byte 0) and, with `causal`, when j > p_i; a query that sees no key yields a zero row and lse -inf.
- *   Q [Tq, H D], K / V [Tk, Hkv D] bf16 rows with leading dimensions in elements (multiples of 8; 16-byte aligned bases), head h at column h D,
+ *   Q [Tq, H D], K / V [Tk, Hkv D] bf16 rows with leading dimensions in elements (multiples of 8 up to 2^24; 16-byte aligned bases), head h at column h D,
  *   query head h reads key / value head h / (H / Hkv).  D in {32, 64, 96, 128}.
  *   cu_q / cu_k int32 [S + 1] on the device: sequence s owns rows cu[s] .. cu[s + 1] - 1 (cu[0] is taken as 0; offsets outside the tensors are
  *   clamped, so no content of theirs makes a kernel leave its operands).  max_q / max_k: the longest sequences, on the host; they size the grid

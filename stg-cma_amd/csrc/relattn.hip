@@ -42,8 +42,31 @@ struct RP {
     bf16_t* dK; int64_t lddk;
     bf16_t* dV; int64_t lddv;
     float* delta;                     // [H, Tq]
-    float* part;                      // [S * gridDim.x, H, NB] partial table gradients, or NULL
+    float* part;                      // partial table gradients: [S * tiles, H, 2] behind the borders / [S * blocks, H, NB] of the band; or NULL
+    int tiles;                        // blocks per (sequence, head)
 };
+
+// Which (tile, head, sequence) a block of the one-dimensional grid serves; the blocks that clear the rows behind the last sequence (s == S) come
+// last.  Without the causal rule tiles run fastest: neighbouring blocks share their keys in L2.  With it heads run fastest, then sequences, and the
+// heaviest tiles come first, so the long walks do not start last; the sequence is rotated by the tile, since consecutive blocks go to the
+// eight XCDs in turn and a fixed order would hand the long sequences to the same ones (measured with sequences fastest: 1.7 times slower).
+struct Who { int tile, h, s; };
+__device__ __forceinline__ Who who(const RP& a, int heads) {
+    const int id = blockIdx.x;
+    Who w;
+    if (a.causal) {
+        const int u = id / heads;
+        w.h = id % heads;
+        w.tile = a.S > 0 ? u / a.S : a.tiles;
+        if (w.tile < a.tiles) w.s = (u % a.S + w.tile) % a.S;
+        else { w.tile = u - a.tiles * a.S; w.s = a.S; }
+    } else {
+        w.tile = id % a.tiles;
+        w.h = id / a.tiles % heads;
+        w.s = id / a.tiles / heads;
+    }
+    return w;
+}
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef short s4_t __attribute__((ext_vector_type(4)));
@@ -126,49 +149,76 @@ __device__ __forceinline__ void fill_bias(const RP& a, int h, float* bv, int tid
     }
 }
 
-// Staging of two [64][D] tiles (K and V, or Q and dO) by NTHR threads in 16-byte pieces through registers.
+// Staging of two [64][D] tiles (K and V, or Q and dO) by NTHR threads in 16-byte pieces through registers.  A thread's pieces are rows
+// of one column piece: one 32-bit byte offset per tensor and scalar bases, so a full tile costs no address arithmetic.  (D = 96: 256 threads are no
+// whole number of rows; an offset per piece.)
 template <int N> using U4Arr = u32x4_t[N];
 template <int D, int NTHR> struct StageC {
     static constexpr int ROWP = D / 8;                       // pieces per row
-    static constexpr int TOTAL = 2 * 64 * ROWP;
-    static constexpr int PER = (TOTAL + NTHR - 1) / NTHR;
+    static constexpr int HALF = 64 * ROWP / NTHR;            // pieces of one tensor per thread
+    static constexpr int PER = 2 * HALF;
+    static constexpr int STEP = NTHR % ROWP == 0 ? NTHR / ROWP : 0;     // rows between a thread's pieces, 0: not one number
+    static constexpr int NOFF = STEP ? 1 : HALF;
     static constexpr int DP = D + 8;                         // padded pitch: conflict-free for row-wise and transposed reads
     static constexpr int TILE = 64 * DP;
-    static_assert(TOTAL % NTHR == 0, "every thread moves the same number of pieces");
+    static_assert(64 * ROWP % NTHR == 0, "every thread moves the same number of pieces");
 };
+template <int D, int NTHR> __device__ __forceinline__ int stage_row(int tid, int i) { return (tid + NTHR * i) / StageC<D, NTHR>::ROWP; }
+template <int D, int NTHR> __device__ __forceinline__ int stage_col(int tid, int i) { return 8 * ((tid + NTHR * i) % StageC<D, NTHR>::ROWP); }
 template <int D, int NTHR>
-__device__ __forceinline__ void stage_fetch(U4Arr<StageC<D, NTHR>::PER>& v, int tid, const bf16_t* t0, int64_t ld0, const bf16_t* t1, int64_t ld1,
-                                            int row0, int n) {
+__device__ __forceinline__ void stage_one(u32x4_t* v, int tid, const bf16_t* t, int64_t ld, const uint32_t* off, int row0, int n) {
     using C = StageC<D, NTHR>;
+    if (row0 + 64 <= n) {
+        const char* base = reinterpret_cast<const char*>(t + (int64_t)row0 * ld);
 #pragma unroll
-    for (int i = 0; i < C::PER; ++i) {
-        const int id = tid + NTHR * i;
-        const int which = id / (64 * C::ROWP), rem = id - which * 64 * C::ROWP;
-        const int r = rem / C::ROWP, c = rem - r * C::ROWP;
-        int row = row0 + r;
-        row = row < n ? row : n - 1;
-        v[i] = *reinterpret_cast<const u32x4_t*>((which ? t1 + (int64_t)row * ld1 : t0 + (int64_t)row * ld0) + 8 * c);
+        for (int i = 0; i < C::HALF; ++i) v[i] = *reinterpret_cast<const u32x4_t*>(base + (C::STEP ? (int64_t)i * C::STEP * ld * 2 : 0) + off[C::STEP ? 0 : i]);
+    } else {                                                 // the last tile: rows past the end read the last row (and are zeroed on the way into LDS)
+#pragma unroll
+        for (int i = 0; i < C::HALF; ++i) {
+            int row = row0 + stage_row<D, NTHR>(tid, i);
+            row = row < n ? row : n - 1;
+            v[i] = *reinterpret_cast<const u32x4_t*>(t + (int64_t)row * ld + stage_col<D, NTHR>(tid, i));
+        }
     }
 }
+template <int D, int NTHR> struct Stage {
+    using C = StageC<D, NTHR>;
+    uint32_t off0[C::NOFF], off1[C::NOFF];
+    __device__ __forceinline__ void plan(int tid, int64_t ld0, int64_t ld1) {
+#pragma unroll
+        for (int i = 0; i < C::NOFF; ++i) {
+            off0[i] = 2 * ((uint32_t)stage_row<D, NTHR>(tid, i) * (uint32_t)ld0 + stage_col<D, NTHR>(tid, i));
+            off1[i] = 2 * ((uint32_t)stage_row<D, NTHR>(tid, i) * (uint32_t)ld1 + stage_col<D, NTHR>(tid, i));
+        }
+    }
+    __device__ __forceinline__ void fetch(U4Arr<C::PER>& v, int tid, const bf16_t* t0, int64_t ld0, const bf16_t* t1, int64_t ld1, int row0, int n) const {
+        stage_one<D, NTHR>(v, tid, t0, ld0, off0, row0, n);
+        stage_one<D, NTHR>(v + C::HALF, tid, t1, ld1, off1, row0, n);
+    }
+};
 // `valid`: bit r set = row r of the tile takes part; other rows are written as zeros
 template <int D, int NTHR>
-__device__ __forceinline__ void stage_commit(bf16_t* s, const U4Arr<StageC<D, NTHR>::PER>& v, int tid, uint64_t valid) {
+__device__ __forceinline__ void stage_commit(bf16_t* s, U4Arr<StageC<D, NTHR>::PER>& v, int tid, uint64_t valid) {
     using C = StageC<D, NTHR>;
+    if (valid != ~0ull) {
+        asm volatile("");
 #pragma unroll
-    for (int i = 0; i < C::PER; ++i) {
-        const int id = tid + NTHR * i;
-        const int which = id / (64 * C::ROWP), rem = id - which * 64 * C::ROWP;
-        const int r = rem / C::ROWP, c = rem - r * C::ROWP;
-        u32x4_t w = v[i];
-        if (valid != ~0ull && !((valid >> r) & 1)) w = (u32x4_t){0u, 0u, 0u, 0u};
-        *reinterpret_cast<u32x4_t*>(s + which * C::TILE + r * C::DP + 8 * c) = w;
+        for (int i = 0; i < C::PER; ++i)
+            if (!((valid >> stage_row<D, NTHR>(tid, i % C::HALF)) & 1)) v[i] = (u32x4_t){0u, 0u, 0u, 0u};
     }
+#pragma unroll
+    for (int i = 0; i < C::PER; ++i)
+        *reinterpret_cast<u32x4_t*>(s + (i / C::HALF) * C::TILE + stage_row<D, NTHR>(tid, i % C::HALF) * C::DP + stage_col<D, NTHR>(tid, i % C::HALF)) = v[i];
 }
-// bits of the 64 keys kb .. kb + 63 of a sequence that exist and are not masked (wave-uniform)
-__device__ __forceinline__ uint64_t key_bits(const RP& a, const Seq& z, int kb, int lane) {
-    bool ok = kb + lane < z.nk;
-    if (a.kmask != nullptr && ok) ok = a.kmask[(int64_t)z.k0 + kb + lane] != 0;
-    const uint64_t b = __builtin_amdgcn_ballot_w64(ok);
+// The 64 keys kb .. kb + 63 of a sequence that exist and are not masked: key_load asks for the lane's own (the load stays in flight), key_bits makes
+// the wave-uniform bits of them.
+__device__ __forceinline__ int key_load(const RP& a, const Seq& z, int kb, int lane) {
+    const int key = kb + lane;
+    if (a.kmask == nullptr) return key < z.nk;
+    return key < z.nk ? a.kmask[(int64_t)z.k0 + key] : 0;
+}
+__device__ __forceinline__ uint64_t key_bits(int mine) {
+    const uint64_t b = __builtin_amdgcn_ballot_w64(mine != 0);
     return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
 }
 // start of a score accumulator: bias of rows kb + ACC_ROW(., hh) against the lane's query position (idx = bv index of row 0, hh included)
@@ -197,25 +247,28 @@ __device__ __forceinline__ int64_t tail_start(const int32_t* cu, int S, int64_t 
 // Scores are computed transposed (rows = keys, lane = query): the softmax statistics are lane-local and P feeds the second MFMA from
 // registers.
 template <int D, int NW>
-__global__ void __launch_bounds__(NW * 64, 2) relattn_fwd_kernel(RP a) {
+__global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
     using SC = StageC<D, NTHR>;
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];       // two buffers x {K, V} x [64][DP], then the bias by distance
     float* bv = reinterpret_cast<float*>(smem + 4 * SC::TILE);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // (wave-uniform for the compiler too)
     const int r = lane & 31, hh = lane >> 5;
-    const int h = blockIdx.y, hk = h / (a.H / a.Hkv);
-    if ((int)blockIdx.z == a.S) {                                       // the slice that clears the rows behind the last sequence
+    const Who w = who(a, a.H);
+    const int h = w.h, hk = h / (a.H / a.Hkv);
+    if (w.s == a.S) {                                       // the slice that clears the rows behind the last sequence
         const int64_t from = tail_start(a.cu_q, a.S, a.Tq);
-        const int step = gridDim.x * NTHR, off = blockIdx.x * NTHR + tid;
+        const int step = a.tiles * NTHR, off = w.tile * NTHR + tid;
         zero_rows(a.O, a.ldo, from, a.Tq, h * D, D, step, off);
         if (a.lse) for (int64_t i = from + off; i < a.Tq; i += step) a.lse[(int64_t)h * a.Tq + i] = -INFINITY;
         return;
     }
-    const Seq z = seq_of(a, blockIdx.z);
+    const Seq z = seq_of(a, w.s);
     const int shift = z.nk - z.nq;
+    Stage<D, NTHR> sg;
+    sg.plan(tid, a.ldk, a.ldv);
     bool filled = false;
-    for (int64_t tile = blockIdx.x; tile * 32 * NW < z.nq; tile += gridDim.x) {
+    for (int64_t tile = w.tile; tile * 32 * NW < z.nq; tile += a.tiles) {
         // heavy tiles first under the causal rule
         const int nt = (z.nq + 32 * NW - 1) / (32 * NW);
         const int qt = a.causal ? nt - 1 - (int)tile : (int)tile;
@@ -244,13 +297,17 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_fwd_kernel(RP a) {
         const bf16_t* Kb = a.K + (int64_t)z.k0 * a.ldk + hk * D;
         const bf16_t* Vb = a.V + (int64_t)z.k0 * a.ldv + hk * D;
         u32x4_t sv[SC::PER];
-        uint64_t bits = 0, nbits = 0;
+        uint64_t bits = 0;
+        int mk = 0;
         if (np > 0) {
-            stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, 0, z.nk);
-            bits = key_bits(a, z, 0, lane);
+            mk = key_load(a, z, 0, lane);
+            sg.fetch(sv, tid, Kb, a.ldk, Vb, a.ldv, 0, z.nk);
         }
         if (!filled) { fill_bias(a, h, bv, tid, NTHR); filled = true; }
-        if (np > 0) stage_commit<D, NTHR>(smem, sv, tid, bits);
+        if (np > 0) {
+            bits = key_bits(mk);
+            stage_commit<D, NTHR>(smem, sv, tid, bits);
+        }
         __syncthreads();
         const float cleft = bv[0], cright = bv[2 * (a.far + PAD)];
         for (int kp = 0; kp < np; ++kp) {
@@ -258,8 +315,8 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_fwd_kernel(RP a) {
             const bf16_t* sV = sK + SC::TILE;
             const int kb = 64 * kp;
             if (kp + 1 < np) {
-                stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, kb + 64, z.nk);
-                nbits = key_bits(a, z, kb + 64, lane);
+                mk = key_load(a, z, kb + 64, lane);
+                sg.fetch(sv, tid, Kb, a.ldk, Vb, a.ldv, kb + 64, z.nk);
             }
             if (live && bits != 0 && !(a.causal && kb > phi)) {
                 // St[key][q] of keys kb .. + 31 / + 32 .. + 63.  Behind a border the bias is one number: it joins the exponent's constant and
@@ -327,8 +384,10 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_fwd_kernel(RP a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[dt] = MFMA32(tr_frag<DP>(sV, dt, i, hh, r), pf[i], o[dt]);
             }
-            if (kp + 1 < np) stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, nbits);
-            bits = nbits;
+            if (kp + 1 < np) {
+                bits = key_bits(mk);
+                stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, bits);
+            }
             __syncthreads();
         }
         {
@@ -371,19 +430,22 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
     float* bv = reinterpret_cast<float*>(smem + 4 * SC::TILE);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // (wave-uniform for the compiler too)
     const int r = lane & 31, hh = lane >> 5;
-    const int h = blockIdx.y, hk = h / (a.H / a.Hkv);
-    if ((int)blockIdx.z == a.S) {
+    const Who w = who(a, a.H);
+    const int h = w.h, hk = h / (a.H / a.Hkv);
+    if (w.s == a.S) {
         const int64_t from = tail_start(a.cu_q, a.S, a.Tq);
-        zero_rows(a.dQ, a.lddq, from, a.Tq, h * D, D, gridDim.x * NTHR, blockIdx.x * NTHR + tid);
+        zero_rows(a.dQ, a.lddq, from, a.Tq, h * D, D, a.tiles * NTHR, w.tile * NTHR + tid);
         return;
     }
-    const Seq z = seq_of(a, blockIdx.z);
+    const Seq z = seq_of(a, w.s);
     const int shift = z.nk - z.nq;
     fill_bias(a, h, bv, tid, NTHR);
+    Stage<D, NTHR> sg;
+    sg.plan(tid, a.ldk, a.ldv);
     float tab_l = 0.f, tab_r = 0.f;                                     // the lane's sums behind the borders, corrected
     __syncthreads();
     const float cleft = bv[0] * a.scale2, cright = bv[blen - 1] * a.scale2;
-    for (int64_t tile = blockIdx.x; tile * 32 * NW < z.nq; tile += gridDim.x) {
+    for (int64_t tile = w.tile; tile * 32 * NW < z.nq; tile += a.tiles) {
         const int nt = (z.nq + 32 * NW - 1) / (32 * NW);
         const int qt = a.causal ? nt - 1 - (int)tile : (int)tile;
         const int qb = qt * 32 * NW, qw = qb + 32 * wave;
@@ -425,12 +487,16 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
         const bf16_t* Vb = a.V + (int64_t)z.k0 * a.ldv + hk * D;
         Comp all, sl, sr;                                               // the lane's share of its row: sum dS, behind the left / right border
         float br = 0.f, bn = 0.f;                                       // probability behind the right border, around the diagonal
-        const f32x16_t ndel = splat16(-delta);
+        // dP - delta: the accumulator starts at -delta, 16 registers held for that where there is room (D <= 64), else a subtraction
+        constexpr bool HOLD = D <= 64;
+        const f32x16_t ndel = splat16(HOLD ? -delta : 0.f);
         u32x4_t sv[SC::PER];
-        uint64_t bits = 0, nbits = 0;
+        uint64_t bits = 0;
+        int mk = 0;
         if (np > 0) {
-            stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, 0, z.nk);
-            bits = key_bits(a, z, 0, lane);
+            mk = key_load(a, z, 0, lane);
+            sg.fetch(sv, tid, Kb, a.ldk, Vb, a.ldv, 0, z.nk);
+            bits = key_bits(mk);
             stage_commit<D, NTHR>(smem, sv, tid, bits);
         }
         __syncthreads();
@@ -439,8 +505,8 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
             const bf16_t* sV = sK + SC::TILE;
             const int kb = 64 * kp;
             if (kp + 1 < np) {
-                stage_fetch<D, NTHR>(sv, tid, Kb, a.ldk, Vb, a.ldv, kb + 64, z.nk);
-                nbits = key_bits(a, z, kb + 64, lane);
+                mk = key_load(a, z, kb + 64, lane);
+                sg.fetch(sv, tid, Kb, a.ldk, Vb, a.ldv, kb + 64, z.nk);
             }
             const bool left = kb + 63 - plo <= -a.far, right = kb - phi >= a.far;
             if (live && bits != 0 && !(a.causal && kb > phi)) {
@@ -458,7 +524,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
                     const bf16_t* tK = sK + half * 32 * DP;
                     const bf16_t* tV = sV + half * 32 * DP;
                     const int idx = idx0 + 32 * half;
-                    f32x16_t sc, dp = MFMA32(nat_frag<DP>(tV, r, hh, 0), df[0], ndel);     // dP - delta: the accumulator starts at -delta
+                    f32x16_t sc, dp = MFMA32(nat_frag<DP>(tV, r, hh, 0), df[0], ndel);
                     if (left || right) sc = MFMA32(nat_frag<DP>(tK, r, hh, 0), qf[0], splat16(0.f));
                     else sc = MFMA32(nat_frag<DP>(tK, r, hh, 0), qf[0], bias16(bv, idx));
 #pragma unroll
@@ -470,7 +536,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
 #pragma unroll
                     for (int reg = 0; reg < 16; ++reg) {
                         p[reg] = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nf));
-                        ds[reg] = p[reg] * dp[reg];
+                        ds[reg] = p[reg] * (HOLD ? dp[reg] : dp[reg] - delta);
                     }
                     if (edge) {
                         asm volatile("");                           // (kept a branch: as selects these run in every tile)
@@ -503,8 +569,10 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
                     }
                 }
             }
-            if (kp + 1 < np) stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, nbits);
-            bits = nbits;
+            if (kp + 1 < np) {
+                bits = key_bits(mk);
+                stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, bits);
+            }
             __syncthreads();
         }
         bf16_t* dqp = a.dQ + ((int64_t)z.q0 + q) * a.lddq + h * D;
@@ -535,7 +603,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
             float t = 0.f;
 #pragma unroll
             for (int w = 0; w < NW; ++w) t += bv[2 * w + tid];
-            a.part[(((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * a.H + h) * 2 + tid] = t;
+            a.part[(((int64_t)w.s * a.tiles + w.tile) * a.H + h) * 2 + tid] = t;
         }
     }
 }
@@ -603,12 +671,13 @@ __global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups,
                 *reinterpret_cast<u32x4_t*>(s + half * TILE + rr * DP + 8 * c) = w;
             }
         };
-        auto kbits = [&](int kt) -> uint32_t {                          // keys of tile kt that exist and are not masked
+        auto kload = [&](int kt) -> int {                               // the lane's key of tile kt: exists and is not masked
             const int key = 32 * kt + (lane & 31);
-            bool ok = key >= 0 && key < z.nk;
-            if (a.kmask != nullptr && ok) ok = a.kmask[(int64_t)z.k0 + key] != 0;
-            return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)__builtin_amdgcn_ballot_w64(ok));
+            const bool ok = key >= 0 && key < z.nk;
+            if (a.kmask == nullptr) return ok;
+            return ok ? a.kmask[(int64_t)z.k0 + key] : 0;
         };
+        auto kbits = [&](int mk) -> uint32_t { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)__builtin_amdgcn_ballot_w64(mk != 0)); };
         auto qbits = [&](int i) -> uint32_t {
             const int left = z.nq - 32 * i;
             return left >= 32 ? ~0u : (1u << left) - 1;
@@ -616,27 +685,27 @@ __global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups,
         for (int first = ch * chunk; first < nqt; first += nch * chunk) {
             const int last = first + chunk < nqt ? first + chunk : nqt;
             // what a step stages is fetched two steps ahead (a step computes for ~600 cycles, an L2 or MALL load takes longer): two register sets
-            struct Next { u32x4_t kv[PER], qd[PER]; float l, d; uint32_t sbits, bits; } n0, n1;
+            struct Next { u32x4_t kv[PER], qd[PER]; float l, d; int smk, mk; } n0, n1;
             auto ahead = [&](int i, Next& n) {                          // query tile i, its new key tile, the wave's key bits
                 fetch(n.kv, Kb, a.ldk, Vb, a.ldv, 32 * (i + t0 + 3), z.nk);
                 fetch(n.qd, Qb, a.ldq, Db, a.lddo, 32 * i, z.nq);
                 const int q = 32 * i + r;
                 n.l = q < z.nq ? lseb[q] : -INFINITY;
                 n.d = q < z.nq ? delb[q] : 0.f;
-                n.sbits = kbits(i + t0 + 3);
-                n.bits = kbits(i + t);
+                n.smk = kload(i + t0 + 3);
+                n.mk = kload(i + t);
             };
             int slot = 0;                                               // ring slot of the block's first diagonal
             float nl, nd;
             uint32_t bits;
             auto enter = [&](int i, const Next& n, int kslot) {         // the step's tiles into LDS, its statistics into registers
-                commit(smem + kslot * 2 * TILE, n.kv, n.sbits);
+                commit(smem + kslot * 2 * TILE, n.kv, kbits(n.smk));
                 commit(sQ + ((i - first) & 1) * 2 * TILE, n.qd, qbits(i));
             };
             auto take = [&](const Next& n) {
                 nl = n.l == -INFINITY ? -INFINITY : -n.l * LOG2E;
                 nd = -n.d;
-                bits = n.bits;
+                bits = kbits(n.mk);
             };
             auto compute = [&](int i) {
                 const int kt = i + t, kb = (32 * kt) & ~63, plo = 32 * i + shift, phi = plo + 31;
@@ -672,12 +741,12 @@ __global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups,
             };
             {
                 u32x4_t w[3][PER];
-                uint32_t ok[3];
+                int ok[3];
                 for (int j = 0; j < 3; ++j) fetch(w[j], Kb, a.ldk, Vb, a.ldv, 32 * (first + t0 + j), z.nk);
                 ahead(first, n0);
-                for (int j = 0; j < 3; ++j) ok[j] = kbits(first + t0 + j);
+                for (int j = 0; j < 3; ++j) ok[j] = kload(first + t0 + j);
                 __syncthreads();
-                for (int j = 0; j < 3; ++j) commit(smem + j * 2 * TILE, w[j], ok[j]);
+                for (int j = 0; j < 3; ++j) commit(smem + j * 2 * TILE, w[j], kbits(ok[j]));
                 enter(first, n0, 3);
                 take(n0);
             }
@@ -763,23 +832,26 @@ template <int D, int NW>
 __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
     using SC = StageC<D, NTHR>;
-    constexpr int BUF = 2 * SC::TILE + 256;                             // Q and dO tiles + 128 floats of statistics
+    constexpr int BUF = 2 * SC::TILE + 512;                             // Q and dO tiles + 4 x 64 floats of statistics
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
     float* bv = reinterpret_cast<float*>(smem + 2 * BUF);
     const int blen = 2 * (a.far + PAD) + 1;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // (wave-uniform for the compiler too)
     const int r = lane & 31, hh = lane >> 5;
-    const int hk = blockIdx.y, rep = a.H / a.Hkv;
-    if ((int)blockIdx.z == a.S) {
+    const Who w = who(a, a.Hkv);
+    const int hk = w.h, rep = a.H / a.Hkv;
+    if (w.s == a.S) {
         const int64_t from = tail_start(a.cu_k, a.S, a.Tk);
-        const int step = gridDim.x * NTHR, off = blockIdx.x * NTHR + tid;
+        const int step = a.tiles * NTHR, off = w.tile * NTHR + tid;
         zero_rows(a.dK, a.lddk, from, a.Tk, hk * D, D, step, off);
         zero_rows(a.dV, a.lddv, from, a.Tk, hk * D, D, step, off);
         return;
     }
-    const Seq z = seq_of(a, blockIdx.z);
+    const Seq z = seq_of(a, w.s);
     const int shift = z.nk - z.nq;
-    for (int64_t tile = blockIdx.x; tile * 32 * NW < z.nk; tile += gridDim.x) {
+    Stage<D, NTHR> sg;
+    sg.plan(tid, a.ldq, a.lddo);
+    for (int64_t tile = w.tile; tile * 32 * NW < z.nk; tile += a.tiles) {
         const int kw = 32 * ((int)tile * NW + wave);
         const int key = kw + r;
         bool kok = key < z.nk;
@@ -812,29 +884,30 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
             const float* lseb = a.lse + (int64_t)h * a.Tq + z.q0;
             const float* delb = a.delta + (int64_t)h * a.Tq + z.q0;
             u32x4_t sv[SC::PER];
-            float nl = 0.f, nd = 0.f;
+            float nl = 0.f, nd = 0.f, cleft, cright;
             auto fetch_all = [&](int q0) {
-                stage_fetch<D, NTHR>(sv, tid, Qb, a.ldq, Db, a.lddo, q0, z.nq);
+                sg.fetch(sv, tid, Qb, a.ldq, Db, a.lddo, q0, z.nq);
                 if (tid < 64) {
                     const int qi = q0 + tid;
                     nl = qi < z.nq ? lseb[qi] : -INFINITY;
                     nd = qi < z.nq ? -delb[qi] : 0.f;
-                    nl = nl == -INFINITY ? -INFINITY : -nl * LOG2E;     // a row that saw nothing, or none at all: P = 0
+                    // lse in units of the raw score; a row that saw nothing, or none at all: P = 0
+                    nl = nl == -INFINITY ? -INFINITY : -nl * a.inv_scale;
                 }
             };
             auto commit_all = [&](bf16_t* buf, int q0) {
                 const int left = z.nq - q0;
                 stage_commit<D, NTHR>(buf, sv, tid, left >= 64 ? ~0ull : (1ull << left) - 1);
                 float* st = reinterpret_cast<float*>(buf + 2 * SC::TILE);
-                if (tid < 64) { st[tid] = nl; st[64 + tid] = nd; }
+                if (tid < 64) { st[tid] = nl; st[64 + tid] = nl + cleft; st[128 + tid] = nl + cright; st[192 + tid] = nd; }
             };
             fetch_all(64 * p0);
             fill_bias(a, h, bv, tid, NTHR);
+            __syncthreads();
+            cleft = bv[0];
+            cright = bv[blen - 1];
             commit_all(smem + (p0 & 1) * BUF, 64 * p0);
             __syncthreads();
-            const float cleft = bv[0], cright = bv[blen - 1];
-            f32x16_t cvec = splat16(cright);
-            int side = 2;
             for (int qp = p0; qp < np; ++qp) {
                 const bf16_t* sQ = smem + (qp & 1) * BUF;
                 const bf16_t* sD = sQ + SC::TILE;
@@ -844,42 +917,36 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                 if (live && !(a.causal && pb + 63 < kw)) {
                     const bool left = kw + 31 - pb <= -a.far, right = kw - (pb + 63) >= a.far;
                     const bool edge = a.causal && kw + 31 > pb;
-                    // behind a border the accumulator starts at one number: 16 registers that change twice in a walk
-                    if ((left || right) && side != (left ? 1 : 2)) {
-                        side = left ? 1 : 2;
-                        cvec = splat16(left ? cleft : cright);
-                    }
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const bf16_t* tQ = sQ + half * 32 * DP;
                         const bf16_t* tD = sD + half * 32 * DP;
                         const int rel = key - (pb + 32 * half) - 4 * hh;    // distance of accumulator row 0
+                        // the accumulators start at bias - lse (behind a border the two were added once per query) and at -delta
                         f32x16_t sc, dp;
-                        if (left || right) sc = MFMA32(nat_frag<DP>(tQ, r, hh, 0), kf[0], cvec);
-                        else {
-                            const float* bp = bv + rel + a.far + PAD;
-                            f32x16_t c;
-#pragma unroll
-                            for (int reg = 0; reg < 16; ++reg) c[reg] = bp[-ACC_ROW(reg, 0)];
-                            sc = MFMA32(nat_frag<DP>(tQ, r, hh, 0), kf[0], c);
-                        }
-                        float lv[16];
+                        const float* st = sL + 64 * (left ? 1 : (right ? 2 : 0)) + 32 * half + 4 * hh;
 #pragma unroll
                         for (int g4 = 0; g4 < 4; ++g4) {
-                            const float4 ls = *reinterpret_cast<const float4*>(sL + 32 * half + 8 * g4 + 4 * hh);
-                            const float4 de = *reinterpret_cast<const float4*>(sL + 64 + 32 * half + 8 * g4 + 4 * hh);
-                            lv[4 * g4] = ls.x; lv[4 * g4 + 1] = ls.y; lv[4 * g4 + 2] = ls.z; lv[4 * g4 + 3] = ls.w;
+                            const float4 ls = *reinterpret_cast<const float4*>(st + 8 * g4);
+                            const float4 de = *reinterpret_cast<const float4*>(sL + 192 + 32 * half + 8 * g4 + 4 * hh);
+                            sc[4 * g4] = ls.x; sc[4 * g4 + 1] = ls.y; sc[4 * g4 + 2] = ls.z; sc[4 * g4 + 3] = ls.w;
                             dp[4 * g4] = de.x; dp[4 * g4 + 1] = de.y; dp[4 * g4 + 2] = de.z; dp[4 * g4 + 3] = de.w;
+                        }
+                        if (!left && !right) {
+                            asm volatile("");
+                            const float* bp = bv + rel + a.far + PAD;
+#pragma unroll
+                            for (int reg = 0; reg < 16; ++reg) sc[reg] += bp[-ACC_ROW(reg, 0)];
                         }
 #pragma unroll
                         for (int s = 0; s < KS; ++s) {
-                            if (s > 0) sc = MFMA32(nat_frag<DP>(tQ, r, hh, s), kf[s], sc);
+                            sc = MFMA32(nat_frag<DP>(tQ, r, hh, s), kf[s], sc);
                             dp = MFMA32(nat_frag<DP>(tD, r, hh, s), vf[s], dp);
                         }
                         float pr[16], ds[16];
 #pragma unroll
                         for (int reg = 0; reg < 16; ++reg) {
-                            const float p = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, lv[reg]));
+                            const float p = __builtin_amdgcn_exp2f(sc[reg] * a.scale2);
                             pr[reg] = p;
                             ds[reg] = p * dp[reg];
                         }
@@ -1124,6 +1191,8 @@ __global__ void __launch_bounds__(256) relattn_parts_kernel(DP_ a) {
 // ------------------------------------------------------------------------------------------------ host side
 constexpr int MAX_FAR = 2048, MAX_NB = 256;      // the widest bias arrays (155 KB with the tiles at head dim 128) fit the 160 KB of LDS
 
+constexpr int64_t MAX_LD = 1 << 24;               // a tile's 64 rows are addressed with 32-bit byte offsets
+
 bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
 int check_bias(const char* who, const float* table, const int32_t* plan, int NB, int far, int causal, float scale) {
@@ -1145,6 +1214,7 @@ int check_args(const char* who, const stg_relattn_args* a) {
     const int64_t hd = (int64_t)a->H * a->D, kd = (int64_t)a->Hkv * a->D;
     STG_CHECK(a->ldq >= hd && a->ldo >= hd && a->ldk >= kd && a->ldv >= kd && a->ldq % 8 == 0 && a->ldk % 8 == 0 && a->ldv % 8 == 0 && a->ldo % 8 == 0, -3,
               "%s: leading dimensions must be multiples of 8 and hold every head", who);
+    STG_CHECK(a->ldq <= MAX_LD && a->ldk <= MAX_LD && a->ldv <= MAX_LD && a->ldo <= MAX_LD, -3, "%s: leading dimensions up to 2^24", who);
     STG_CHECK(!misaligned(a->Q) && !misaligned(a->K) && !misaligned(a->V) && !misaligned(a->O), -3, "%s: tensors must be 16-byte aligned", who);
     return check_bias(who, a->table, a->plan, a->num_buckets, a->far, a->causal, a->scale);
 }
@@ -1165,7 +1235,7 @@ RP make_rp(const stg_relattn_args* a) {
 
 int64_t lds_fwd(int D, int far) { return (int64_t)4 * 64 * (D + 8) * 2 + (2 * (far + PAD) + 1) * 4; }
 int64_t lds_band(int D) { return (int64_t)14 * 32 * (D + 8) * 2 + 320 * 4; }
-int64_t lds_dkv(int D, int far) { return (int64_t)2 * (2 * 64 * (D + 8) + 256) * 2 + (2 * (far + PAD) + 1) * 4; }
+int64_t lds_dkv(int D, int far) { return (int64_t)2 * (2 * 64 * (D + 8) + 512) * 2 + (2 * (far + PAD) + 1) * 4; }
 int64_t lds_dec(int D, int NB) { return (int64_t)8 * 32 * (D + 8) * 2 + (int64_t)NB * 32 * 4; }
 
 int grid_tiles(int max_n, int64_t T, int rows) {
@@ -1176,24 +1246,30 @@ int grid_tiles(int max_n, int64_t T, int rows) {
 }
 
 template <int D>
-int launch_fwd(const RP& p, int max_q, hipStream_t st) {
+int launch_fwd(const RP& p0, int max_q, hipStream_t st) {
     static std::atomic<uint64_t> done{0};
     auto k = relattn_fwd_kernel<D, 4>;
     STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_fwd: cannot reserve LDS");
-    const dim3 grid(grid_tiles(max_q, p.Tq, 128), p.H, p.S + (p.zero_tail ? 1 : 0));
-    if (grid.z == 0) return 0;
-    k<<<grid, 256, lds_fwd(D, p.far), st>>>(p);
+    RP p = p0;
+    p.tiles = grid_tiles(max_q, p.Tq, 128);
+    const int64_t blocks = (int64_t)p.tiles * p.H * (p.S + (p.zero_tail ? 1 : 0));
+    STG_CHECK(blocks <= INT32_MAX, -2, "relattn: too many blocks (max_q / max_k larger than the sequences?)");
+    if (blocks == 0) return 0;
+    k<<<dim3((unsigned)blocks), 256, lds_fwd(D, p.far), st>>>(p);
     STG_LAUNCH_CHECK();
     return 0;
 }
 template <int D, bool TAB>
-int launch_dq(const RP& p, int max_q, hipStream_t st) {
+int launch_dq(const RP& p0, int max_q, hipStream_t st) {
     static std::atomic<uint64_t> done{0};
     auto k = relattn_dq_kernel<D, 4, TAB>;
     STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_bwd: cannot reserve LDS");
-    const dim3 grid(grid_tiles(max_q, p.Tq, 128), p.H, p.S + (p.zero_tail ? 1 : 0));
-    if (grid.z == 0) return 0;
-    k<<<grid, 256, lds_fwd(D, p.far), st>>>(p);
+    RP p = p0;
+    p.tiles = grid_tiles(max_q, p.Tq, 128);
+    const int64_t blocks = (int64_t)p.tiles * p.H * (p.S + (p.zero_tail ? 1 : 0));
+    STG_CHECK(blocks <= INT32_MAX, -2, "relattn: too many blocks (max_q / max_k larger than the sequences?)");
+    if (blocks == 0) return 0;
+    k<<<dim3((unsigned)blocks), 256, lds_fwd(D, p.far), st>>>(p);
     STG_LAUNCH_CHECK();
     return 0;
 }
@@ -1208,13 +1284,16 @@ int launch_band(const RP& p, int blocks, int tgroups, int chunk, hipStream_t st)
     return 0;
 }
 template <int D>
-int launch_dkv(const RP& p, int max_k, hipStream_t st) {
+int launch_dkv(const RP& p0, int max_k, hipStream_t st) {
     static std::atomic<uint64_t> done{0};
     auto k = relattn_dkv_kernel<D, 4>;
     STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_bwd: cannot reserve LDS");
-    const dim3 grid(grid_tiles(max_k, p.Tk, 128), p.Hkv, p.S + (p.zero_tail ? 1 : 0));
-    if (grid.z == 0) return 0;
-    k<<<grid, 256, lds_dkv(D, p.far), st>>>(p);
+    RP p = p0;
+    p.tiles = grid_tiles(max_k, p.Tk, 128);
+    const int64_t blocks = (int64_t)p.tiles * p.Hkv * (p.S + (p.zero_tail ? 1 : 0));
+    STG_CHECK(blocks <= INT32_MAX, -2, "relattn: too many blocks (max_q / max_k larger than the sequences?)");
+    if (blocks == 0) return 0;
+    k<<<dim3((unsigned)blocks), 256, lds_dkv(D, p.far), st>>>(p);
     STG_LAUNCH_CHECK();
     return 0;
 }
@@ -1300,6 +1379,7 @@ extern "C" int stg_relattn_bwd(const stg_relattn_args* a, const void* dO, int64_
     if (rc) return rc;
     const int64_t hd = (int64_t)a->H * a->D, kd = (int64_t)a->Hkv * a->D;
     STG_CHECK((a->Tq == 0 || (dO && dQ && a->lse)) && (a->Tk == 0 || (dK && dV)) && ws, -1, "stg_relattn_bwd: null tensor");
+    STG_CHECK(lddo <= MAX_LD, -3, "stg_relattn_bwd: leading dimensions up to 2^24");
     STG_CHECK(lddo >= hd && lddq >= hd && lddk >= kd && lddv >= kd && lddo % 8 == 0 && lddq % 8 == 0 && lddk % 8 == 0 && lddv % 8 == 0, -3,
               "stg_relattn_bwd: leading dimensions must be multiples of 8 and hold every head");
     STG_CHECK(!misaligned(dO) && !misaligned(dQ) && !misaligned(dK) && !misaligned(dV), -3, "stg_relattn_bwd: tensors must be 16-byte aligned");

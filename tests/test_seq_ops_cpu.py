@@ -63,7 +63,7 @@ def _attn_args(**kw):
 
 
 BAD_ATTN = [dict(Q=None), dict(cu_q=None), dict(table=None), dict(plan=None), dict(D=48), dict(D=0), dict(H=3), dict(Hkv=0), dict(H=0), dict(S=-1), dict(S=70000), dict(Tq=-1),
-            dict(Tq=2 ** 31), dict(max_q=-1), dict(ldq=255), dict(ldq=128), dict(ldk=64), dict(ldv=132), dict(Q=4104), dict(O=4104), dict(scale=0.0), dict(scale=float("nan")),
+            dict(Tq=2 ** 31), dict(max_q=-1), dict(ldq=255), dict(ldq=128), dict(ldk=64), dict(ldv=132), dict(ldk=2 ** 24 + 8), dict(ldq=2 ** 31), dict(Q=4104), dict(O=4104), dict(scale=0.0), dict(scale=float("nan")),
             dict(num_buckets=31), dict(num_buckets=2), dict(num_buckets=1000), dict(far=0), dict(far=5000)]
 
 
