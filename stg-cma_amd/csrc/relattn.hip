@@ -1119,73 +1119,77 @@ __global__ void __launch_bounds__(256, 2) relattn_decode_kernel(DP_ a) {
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    // ---- the four waves meet: statistics, then the scaled outputs, one wave's after the other's so that the sum has one order
+    // ---- the four waves meet: statistics, then the scaled outputs, summed in one order
     __syncthreads();
-    float* st = reinterpret_cast<float*>(smem);                         // [4][32] maxima, [4][32] sums, then [D][32] outputs
+    float* st = reinterpret_cast<float*>(smem);                         // [4][32] maxima, [4][32] sums, then per wave [D][33] outputs
     float* so = st + 256;
+    static_assert(1024 + 4 * D * 33 * 4 <= 8 * TILE * 2, "the waves' tiles hold the statistics and the outputs");
     if (hh == 0) { st[32 * wave + r] = m; st[128 + 32 * wave + r] = l; }
     __syncthreads();
     float M = -INFINITY, L = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, st[32 * w + r]);
+    for (int w = 0; w < 4; ++w) M = fmax2(M, st[32 * w + r]);
     const float nM = M == -INFINITY ? 0.f : -M;
 #pragma unroll
     for (int w = 0; w < 4; ++w) L += st[128 + 32 * w + r] * __builtin_amdgcn_exp2f(st[32 * w + r] + nM);
-    const float f = __builtin_amdgcn_exp2f(m + nM);
-    for (int w = 0; w < 4; ++w) {
-        if (wave == w) {
+    const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
+    const float f = __builtin_amdgcn_exp2f(m + nM) * inv;
+    if (col) {
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                for (int reg = 0; reg < 16; ++reg) {
-                    const int d = 32 * dt + ACC_ROW(reg, hh);
-                    const float v = f == 0.f ? 0.f : o[dt][reg] * f;
-                    so[d * 33 + r] = w == 0 ? v : so[d * 33 + r] + v;
-                }
-        }
-        __syncthreads();
+            for (int reg = 0; reg < 16; ++reg) so[(wave * D + 32 * dt + ACC_ROW(reg, hh)) * 33 + r] = f == 0.f ? 0.f : o[dt][reg] * f;
     }
-    if (wave == 0 && hh == 0) st[r] = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
-    if (wave == 1 && hh == 0 && col && a.nsplit > 1)
+    if (wave == 0 && hh == 0 && col && a.nsplit > 1)
         a.pl[((int64_t)s * a.nsplit + sp) * a.H + h0 + r] = L == 0.f ? -INFINITY : M + __log2f(L);
     __syncthreads();
     for (int i = tid; i < ncol * D; i += 256) {
         const int c = i / D, d = i - c * D;
-        const float v = so[d * 33 + c] * st[c];
+        const float v = ((so[d * 33 + c] + so[(D + d) * 33 + c]) + so[(2 * D + d) * 33 + c]) + so[(3 * D + d) * 33 + c];
         if (a.nsplit == 1) a.O[(int64_t)s * a.ldo + (int64_t)(h0 + c) * D + d] = f2bf(v);
         else a.po[(((int64_t)s * a.nsplit + sp) * a.H + h0 + c) * D + d] = v;
     }
 }
 
-// joins the parts of a sequence: O = sum_p 2^(lse_p - M) O_p / sum_p 2^(lse_p - M); one wave per (sequence, head), parts in order
+// joins the parts of a sequence: O = sum_p 2^(lse_p - M) O_p / sum_p 2^(lse_p - M).  A block per (sequence, head): wave w takes parts w, w + 4, ..., eight
+// loads in flight, and the four sums meet in order.
 template <int D>
 __global__ void __launch_bounds__(256) relattn_parts_kernel(DP_ a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (item >= (int64_t)a.S * a.H) return;
-    const int s = (int)(item / a.H), h = (int)(item - (int64_t)s * a.H);
+    constexpr int N = (D + 63) / 64;
+    __shared__ float so[4][D], sw[4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int s = blockIdx.x / a.H, h = blockIdx.x - s * a.H;
     int len = a.lens[s];
     len = len < 0 ? 0 : (len > a.cap ? a.cap : len);
     const int np = len == 0 ? 1 : (len + a.chunk - 1) / a.chunk;
     const float* pl = a.pl + ((int64_t)s * a.nsplit) * a.H + h;
+    const float* po = a.po + ((int64_t)s * a.nsplit * a.H + h) * D;
     float M = -INFINITY;
-    for (int p = lane; p < np; p += 64) M = fmaxf(M, pl[(int64_t)p * a.H]);
-    M = wave_max<64>(M);
+    for (int p = lane; p < np; p += 64) M = fmax2(M, pl[(int64_t)p * a.H]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) M = fmax2(M, __shfl_xor(M, o, 64));
     const float nM = M == -INFINITY ? 0.f : -M;
-    float w = 0.f, acc[(D + 63) / 64] = {};
-    for (int p = 0; p < np; ++p) {
+    float w = 0.f, acc[N] = {};
+#pragma unroll 8
+    for (int p = wave; p < np; p += 4) {
         const float e = __builtin_amdgcn_exp2f(pl[(int64_t)p * a.H] + nM);
         w += e;
-        if (e == 0.f) continue;
-        const float* po = a.po + (((int64_t)s * a.nsplit + p) * a.H + h) * D;
 #pragma unroll
-        for (int i = 0; i < (D + 63) / 64; ++i)
-            if (lane + 64 * i < D) acc[i] = fmaf(e, po[lane + 64 * i], acc[i]);
+        for (int i = 0; i < N; ++i) {
+            const float v = lane + 64 * i < D ? po[(int64_t)p * a.H * D + lane + 64 * i] : 0.f;
+            acc[i] = fmaf(e, e == 0.f ? 0.f : v, acc[i]);
+        }
     }
-    const float inv = w == 0.f ? 0.f : 1.0f / w;
 #pragma unroll
-    for (int i = 0; i < (D + 63) / 64; ++i)
-        if (lane + 64 * i < D) a.O[(int64_t)s * a.ldo + (int64_t)h * D + lane + 64 * i] = f2bf(acc[i] * inv);
+    for (int i = 0; i < N; ++i)
+        if (lane + 64 * i < D) so[wave][lane + 64 * i] = acc[i];
+    if (lane == 0) sw[wave] = w;
+    __syncthreads();
+    if ((int)threadIdx.x < D) {
+        w = ((sw[0] + sw[1]) + sw[2]) + sw[3];
+        const float v = ((so[0][threadIdx.x] + so[1][threadIdx.x]) + so[2][threadIdx.x]) + so[3][threadIdx.x];
+        a.O[(int64_t)s * a.ldo + (int64_t)h * D + threadIdx.x] = f2bf(w == 0.f ? 0.f : v / w);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -1306,7 +1310,7 @@ int launch_decode(const DP_& p, hipStream_t st) {
     k<<<dim3(p.nsplit, p.Hkv * ncg, p.S), 256, lds_dec(D, p.NB), st>>>(p);
     STG_LAUNCH_CHECK();
     if (p.nsplit > 1) {
-        relattn_parts_kernel<D><<<dim3((unsigned)(((int64_t)p.S * p.H + 3) / 4)), 256, 0, st>>>(p);
+        relattn_parts_kernel<D><<<dim3((unsigned)(p.S * p.H)), 256, 0, st>>>(p);
         STG_LAUNCH_CHECK();
     }
     return 0;
@@ -1331,12 +1335,13 @@ int run_dkv(const RP& p, int D, int max_k, hipStream_t st) { BY_DIM(D, (launch_d
 int run_band(const RP& p, int D, int blocks, int tgroups, int chunk, hipStream_t st) { BY_DIM(D, (launch_band<DIM>(p, blocks, tgroups, chunk, st))); }
 int run_decode(const DP_& p, int D, hipStream_t st) { BY_DIM(D, (launch_decode<DIM>(p, st))); }
 
-// keys per block of the single-token form: enough blocks for the chip, at least 128 keys (one 32-key tile for each of the four waves)
+// Keys per block of the single-token form: about 1024 blocks at full length (two rounds of two per compute unit; 64 sequences of 1 .. 4096 tokens:
+// 132 us against 145 / 199 us for blocks of 1024 / 512 keys), at least 128 keys (a 32-key tile for each of the four waves), at most 2048.
 int decode_chunk(int S, int Hkv, int rep, int cap) {
     const int64_t groups = (int64_t)S * Hkv * ((rep + 31) / 32);
     const int64_t total = groups * cap;
     int64_t c = (total / 1024 + 127) / 128 * 128;
-    c = c < 128 ? 128 : (c > 1024 ? 1024 : c);
+    c = c < 128 ? 128 : (c > 2048 ? 2048 : c);
     while ((cap + c - 1) / c > 4096) c *= 2;
     return (int)c;
 }
@@ -1419,7 +1424,7 @@ extern "C" int stg_relattn_decode(const stg_relattn_decode_args* a, float* ws, i
     STG_CHECK(a != nullptr, -1, "stg_relattn_decode: null arguments");
     STG_CHECK(a->S >= 0 && a->S <= 65535 && a->cap >= 0 && a->cap <= INT32_MAX - 1024, -2, "stg_relattn_decode: S=%d (<= 65535), cap=%d", a->S, a->cap);
     STG_CHECK(a->D == 32 || a->D == 64 || a->D == 96 || a->D == 128, -2, "stg_relattn_decode: head dim %d (32, 64, 96 or 128)", a->D);
-    STG_CHECK(a->H > 0 && a->H <= 32768 && a->Hkv > 0 && a->H % a->Hkv == 0, -2, "stg_relattn_decode: %d heads over %d key / value heads", a->H, a->Hkv);
+    STG_CHECK(a->H > 0 && a->H <= 32768 && (int64_t)a->H * a->S <= INT32_MAX && a->Hkv > 0 && a->H % a->Hkv == 0, -2, "stg_relattn_decode: %d heads over %d key / value heads", a->H, a->Hkv);
     STG_CHECK(a->Q && a->O && a->lens && (a->cap == 0 || (a->K && a->V)), -1, "stg_relattn_decode: null tensor");
     const int64_t hd = (int64_t)a->H * a->D, kd = (int64_t)a->Hkv * a->D;
     STG_CHECK(a->ldq >= hd && a->ldo >= hd && a->ldk >= kd && a->ldv >= kd && a->ldq % 8 == 0 && a->ldk % 8 == 0 && a->ldv % 8 == 0 && a->bsk % 8 == 0 &&

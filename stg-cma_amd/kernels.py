@@ -2189,11 +2189,9 @@ class RelGeom:
 
 
 def _rel_chk(t, name, dtype, cols, dev, rows=None):
-    _chk2d(t, name, dtype)
+    _chk2d(t, name, dtype, cols, rows)
     if t.device != dev:
         raise RuntimeError(f"{name}: on {t.device}, expected {dev}")
-    if t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
-        raise RuntimeError(f"{name}: expected {'any number of' if rows is None else rows} rows x {cols} columns, got {tuple(t.shape)}")
     if _ld(t) % 8 or t.data_ptr() % 16:
         raise RuntimeError(f"{name}: rows must start 16-byte aligned (leading dimension {_ld(t)}, a multiple of 8)")
 
@@ -2228,14 +2226,10 @@ def _rel_fill(g, q, k, v, o, lse, table, cu_q, cu_k, max_q, max_k, key_mask):
             raise RuntimeError(f"key_mask: expected a contiguous bool / uint8 vector of {k.shape[0]} on {dev}, got {key_mask.dtype} {tuple(key_mask.shape)}")
     if lse is not None and (lse.dtype != F32 or tuple(lse.shape) != (g.H, q.shape[0]) or not lse.is_contiguous() or lse.device != dev):
         raise RuntimeError(f"lse: expected contiguous fp32 [{g.H}, {q.shape[0]}]")
-    a = _lib.RelAttnArgs()
-    a.Q, a.ldq, a.K, a.ldk, a.V, a.ldv, a.O, a.ldo = _p(q), _ld(q), _p(k), _ld(k), _p(v), _ld(v), _p(o), _ld(o)
-    a.lse, a.cu_q, a.cu_k, a.key_mask = _p(lse), _p(cu_q), _p(cu_k), _p(key_mask)
-    a.Tq, a.Tk, a.S, a.max_q, a.max_k = q.shape[0], k.shape[0], cu_q.shape[0] - 1, min(max_q, q.shape[0]), min(max_k, k.shape[0])
-    a.H, a.Hkv, a.D, a.scale, a.causal = g.H, g.Hkv, g.D, g.scale, int(g.causal)
-    a.plan, a.num_buckets, a.far = _p(g.plan(dev)), g.num_buckets, g.far
-    a.table = _p(table)
-    return a
+    Tq, Tk = q.shape[0], k.shape[0]
+    return _lib.RelAttnArgs(_p(q), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), o.data_ptr(), _ld(o), None if lse is None else lse.data_ptr(), cu_q.data_ptr(),
+                            cu_k.data_ptr(), None if key_mask is None else key_mask.data_ptr(), Tq, Tk, cu_q.shape[0] - 1, min(max_q, Tq), min(max_k, Tk), g.H, g.Hkv, g.D,
+                            g.scale, g.causal, table.data_ptr(), g.plan(dev).data_ptr(), g.num_buckets, g.far, 0)
 
 
 def relattn_fwd(g, q, k, v, table, cu_q, cu_k=None, *, max_q=None, max_k=None, key_mask=None, out=None, want_lse=True):
@@ -2289,33 +2283,31 @@ def relattn_decode(g, q, k_cache, v_cache, table, lens, out=None):
     row and sequence strides that are multiples of 8, so a larger cache's slice is fine), the new token's own key and value already in
     place; lens int32 [S] on the device: tokens in the cache, the new one included.  Returns o bf16 [S, H * D] (zero where lens is 0)."""
     S, dev = q.shape[0], q.device
-    _rel_chk(q, "q", BF16, g.H * g.D, dev)
+    hd, kd = g.H * g.D, g.Hkv * g.D
+    _rel_chk(q, "q", BF16, hd, dev)
+    cap = k_cache.shape[1] if k_cache.dim() == 3 else -1
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if not t.is_cuda or t.dtype != BF16 or t.dim() != 3 or t.shape[0] != S or t.shape[2] != g.Hkv * g.D or t.device != dev or t.shape[1] != k_cache.shape[1]:
-            raise RuntimeError(f"{name}: expected bf16 [{S}, cap, {g.Hkv * g.D}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-        if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and (t.stride(1) % 8 or t.stride(1) < t.shape[2])) or (S > 1 and t.stride(0) % 8)
-                          or t.data_ptr() % 16):
+        if t.dtype != BF16 or t.device != dev or tuple(t.shape) != (S, cap, kd):
+            raise RuntimeError(f"{name}: expected bf16 [{S}, cap, {kd}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        bs, ld, one = t.stride()
+        if t.numel() and (one != 1 or (cap > 1 and (ld % 8 or ld < kd)) or (S > 1 and (bs % 8 or bs < 0)) or t.data_ptr() % 16):
             raise RuntimeError(f"{name}: rows must be contiguous and start 16-byte aligned, strides {t.stride()}")
     _rel_table(g, table, dev)
-    _rel_int32(lens, "lens", S, dev) if S else None
     if out is None:
-        out = torch.empty((S, g.H * g.D), dtype=BF16, device=dev)
-    _rel_chk(out, "out", BF16, g.H * g.D, dev, rows=S)
+        out = torch.empty((S, hd), dtype=BF16, device=dev)
+    else:
+        _rel_chk(out, "out", BF16, hd, dev, rows=S)
     if S == 0:
         return out
-    a = _lib.RelAttnDecodeArgs()
-    cap = k_cache.shape[1]
-    a.Q, a.ldq, a.O, a.ldo = _p(q), _ld(q), _p(out), _ld(out)
-    for t, ptr, ld, bs in ((k_cache, "K", "ldk", "bsk"), (v_cache, "V", "ldv", "bsv")):
-        setattr(a, ptr, _p(t))
-        setattr(a, ld, t.stride(1) if cap > 1 else g.Hkv * g.D)
-        setattr(a, bs, t.stride(0) if S > 1 else 0)
-    a.lens, a.S, a.cap, a.H, a.Hkv, a.D, a.scale, a.causal = _p(lens), S, cap, g.H, g.Hkv, g.D, g.scale, int(g.causal)
-    a.plan, a.num_buckets, a.far = _p(g.plan(dev)), g.num_buckets, g.far
-    a.table = _p(table)
-    n = _lib.lib().stg_relattn_decode_ws_floats(S, cap, g.H, g.Hkv, g.D)
+    _rel_int32(lens, "lens", S, dev)
+    many = S > 1
+    a = _lib.RelAttnDecodeArgs(_p(q), _ld(q), k_cache.data_ptr(), k_cache.stride(1) if cap > 1 else kd, k_cache.stride(0) if many else 0,
+                               v_cache.data_ptr(), v_cache.stride(1) if cap > 1 else kd, v_cache.stride(0) if many else 0, out.data_ptr(), _ld(out),
+                               lens.data_ptr(), S, cap, g.H, g.Hkv, g.D, g.scale, g.causal, table.data_ptr(), g.plan(dev).data_ptr(), g.num_buckets, g.far)
+    lib = _lib.lib()
+    n = lib.stg_relattn_decode_ws_floats(S, cap, g.H, g.Hkv, g.D)
     ws = torch.empty((n,), dtype=F32, device=dev) if n else None
-    _lib.check(_lib.lib().stg_relattn_decode(C.byref(a), _p(ws), n, _stream()), "stg_relattn_decode")
+    _lib.check(lib.stg_relattn_decode(C.byref(a), None if ws is None else ws.data_ptr(), n, _stream()), "stg_relattn_decode")
     return out
 
 
