@@ -91,6 +91,12 @@ __device__ __forceinline__ void both_halves(float v, float& lo, float& hi) {
 }
 __device__ __forceinline__ float half_sum(float v) { float a, b; both_halves(v, a, b); return a + b; }
 __device__ __forceinline__ float half_max(float v) { float a, b; both_halves(v, a, b); return fmax2(a, b); }
+// Operands loaded in front of a loop have arrived before it is entered.  (Without a use here the wait-count bookkeeping takes them as possibly in flight on
+// some path into the loop, and every trip's first products then wait for the NEXT tile's loads, which were issued behind them.)
+template <int N> __device__ __forceinline__ void arrived(bf16x8_t (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
 __device__ __forceinline__ bf16x8_t zero_frag() { const u32x4_t z = {0u, 0u, 0u, 0u}; return __builtin_bit_cast(bf16x8_t, z); }
 __device__ __forceinline__ bf16x8_t pack8(const float* x) {
     const u32x4_t w = {pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7])};
@@ -210,15 +216,15 @@ __device__ __forceinline__ void stage_commit(bf16_t* s, U4Arr<StageC<D, NTHR>::P
     for (int i = 0; i < C::PER; ++i)
         *reinterpret_cast<u32x4_t*>(s + (i / C::HALF) * C::TILE + stage_row<D, NTHR>(tid, i % C::HALF) * C::DP + stage_col<D, NTHR>(tid, i % C::HALF)) = v[i];
 }
-// The 64 keys kb .. kb + 63 of a sequence that exist and are not masked: key_load asks for the lane's own (the load stays in flight), key_bits makes
-// the wave-uniform bits of them.
+// The 64 keys kb .. kb + 63 of a sequence that exist and are not masked: key_load asks for the lane's mask byte (nothing looks at it yet: the load stays
+// in flight), key_bits makes the wave-uniform bits of them.
 __device__ __forceinline__ int key_load(const RP& a, const Seq& z, int kb, int lane) {
-    const int key = kb + lane;
-    if (a.kmask == nullptr) return key < z.nk;
-    return key < z.nk ? a.kmask[(int64_t)z.k0 + key] : 0;
+    if (a.kmask == nullptr) return 1;
+    const int key = kb + lane < z.nk ? kb + lane : z.nk - 1;
+    return a.kmask[(int64_t)z.k0 + key];
 }
-__device__ __forceinline__ uint64_t key_bits(int mine) {
-    const uint64_t b = __builtin_amdgcn_ballot_w64(mine != 0);
+__device__ __forceinline__ uint64_t key_bits(const RP& a, const Seq& z, int byte, int kb, int lane) {
+    const uint64_t b = __builtin_amdgcn_ballot_w64((byte != 0 || a.kmask == nullptr) && kb + lane < z.nk);
     return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
 }
 // start of a score accumulator: bias of rows kb + ACC_ROW(., hh) against the lane's query position (idx = bv index of row 0, hh included)
@@ -305,11 +311,13 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
         }
         if (!filled) { fill_bias(a, h, bv, tid, NTHR); filled = true; }
         if (np > 0) {
-            bits = key_bits(mk);
+            bits = key_bits(a, z, mk, 0, lane);
             stage_commit<D, NTHR>(smem, sv, tid, bits);
         }
         __syncthreads();
-        const float cleft = bv[0], cright = bv[2 * (a.far + PAD)];
+        float cleft = bv[0], cright = bv[2 * (a.far + PAD)];
+        arrived(qf);
+        asm volatile("" : "+v"(cleft), "+v"(cright));
         for (int kp = 0; kp < np; ++kp) {
             const bf16_t* sK = smem + (kp & 1) * 2 * SC::TILE;
             const bf16_t* sV = sK + SC::TILE;
@@ -385,7 +393,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
                     for (int i = 0; i < 4; ++i) o[dt] = MFMA32(tr_frag<DP>(sV, dt, i, hh, r), pf[i], o[dt]);
             }
             if (kp + 1 < np) {
-                bits = key_bits(mk);
+                bits = key_bits(a, z, mk, kb + 64, lane);
                 stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, bits);
             }
             __syncthreads();
@@ -496,10 +504,12 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
         if (np > 0) {
             mk = key_load(a, z, 0, lane);
             sg.fetch(sv, tid, Kb, a.ldk, Vb, a.ldv, 0, z.nk);
-            bits = key_bits(mk);
+            bits = key_bits(a, z, mk, 0, lane);
             stage_commit<D, NTHR>(smem, sv, tid, bits);
         }
         __syncthreads();
+        arrived(qf);
+        arrived(df);
         for (int kp = 0; kp < np; ++kp) {
             const bf16_t* sK = smem + (kp & 1) * 2 * SC::TILE;
             const bf16_t* sV = sK + SC::TILE;
@@ -570,7 +580,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
                 }
             }
             if (kp + 1 < np) {
-                bits = key_bits(mk);
+                bits = key_bits(a, z, mk, kb + 64, lane);
                 stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, bits);
             }
             __syncthreads();
@@ -671,13 +681,17 @@ __global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups,
                 *reinterpret_cast<u32x4_t*>(s + half * TILE + rr * DP + 8 * c) = w;
             }
         };
-        auto kload = [&](int kt) -> int {                               // the lane's key of tile kt: exists and is not masked
-            const int key = 32 * kt + (lane & 31);
-            const bool ok = key >= 0 && key < z.nk;
-            if (a.kmask == nullptr) return ok;
-            return ok ? a.kmask[(int64_t)z.k0 + key] : 0;
+        // without a mask the byte comes from K's rows and does not count: one flow of loads, which the wait counts can follow
+        const uint8_t* mask = a.kmask != nullptr ? a.kmask + z.k0 : reinterpret_cast<const uint8_t*>(Kb);
+        auto kload = [&](int kt) -> int {                               // the lane's mask byte of tile kt (stays in flight)
+            int key = 32 * kt + (lane & 31);
+            key = key < 0 ? 0 : (key < z.nk ? key : z.nk - 1);
+            return mask[key];
         };
-        auto kbits = [&](int mk) -> uint32_t { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)__builtin_amdgcn_ballot_w64(mk != 0)); };
+        auto kbits = [&](int kt, int byte) -> uint32_t {                // keys of the tile that exist and are not masked
+            const int key = 32 * kt + (lane & 31);
+            return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)__builtin_amdgcn_ballot_w64((byte != 0 || a.kmask == nullptr) && key >= 0 && key < z.nk));
+        };
         auto qbits = [&](int i) -> uint32_t {
             const int left = z.nq - 32 * i;
             return left >= 32 ? ~0u : (1u << left) - 1;
@@ -689,9 +703,9 @@ __global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups,
             auto ahead = [&](int i, Next& n) {                          // query tile i, its new key tile, the wave's key bits
                 fetch(n.kv, Kb, a.ldk, Vb, a.ldv, 32 * (i + t0 + 3), z.nk);
                 fetch(n.qd, Qb, a.ldq, Db, a.lddo, 32 * i, z.nq);
-                const int q = 32 * i + r;
-                n.l = q < z.nq ? lseb[q] : -INFINITY;
-                n.d = q < z.nq ? delb[q] : 0.f;
+                const int q = 32 * i + r < z.nq ? 32 * i + r : z.nq - 1;
+                n.l = lseb[q];
+                n.d = delb[q];
                 n.smk = kload(i + t0 + 3);
                 n.mk = kload(i + t);
             };
@@ -699,13 +713,14 @@ __global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups,
             float nl, nd;
             uint32_t bits;
             auto enter = [&](int i, const Next& n, int kslot) {         // the step's tiles into LDS, its statistics into registers
-                commit(smem + kslot * 2 * TILE, n.kv, kbits(n.smk));
+                commit(smem + kslot * 2 * TILE, n.kv, kbits(i + t0 + 3, n.smk));
                 commit(sQ + ((i - first) & 1) * 2 * TILE, n.qd, qbits(i));
             };
-            auto take = [&](const Next& n) {
-                nl = n.l == -INFINITY ? -INFINITY : -n.l * LOG2E;
-                nd = -n.d;
-                bits = kbits(n.mk);
+            auto take = [&](int i, const Next& n) {
+                const bool ok = 32 * i + r < z.nq && n.l != -INFINITY;
+                nl = ok ? -n.l * LOG2E : -INFINITY;
+                nd = ok ? -n.d : 0.f;
+                bits = kbits(i + t, n.mk);
             };
             auto compute = [&](int i) {
                 const int kt = i + t, kb = (32 * kt) & ~63, plo = 32 * i + shift, phi = plo + 31;
@@ -746,18 +761,18 @@ __global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups,
                 ahead(first, n0);
                 for (int j = 0; j < 3; ++j) ok[j] = kload(first + t0 + j);
                 __syncthreads();
-                for (int j = 0; j < 3; ++j) commit(smem + j * 2 * TILE, w[j], kbits(ok[j]));
+                for (int j = 0; j < 3; ++j) commit(smem + j * 2 * TILE, w[j], kbits(first + t0 + j, ok[j]));
                 enter(first, n0, 3);
-                take(n0);
+                take(first, n0);
             }
-            if (first + 1 < last) ahead(first + 1, n1);
+            ahead(first + 1 < last ? first + 1 : first, n1);
             __syncthreads();
             auto step = [&](int i, Next& next, Next& after) {           // next: fetched for step i + 1; after: free
-                if (i + 2 < last) ahead(i + 2, after);
+                ahead(i + 2 < last ? i + 2 : i, after);                 // (always: a branch here would make the wait for `next` a wait for these)
                 compute(i);
                 if (i + 1 < last) {
                     enter(i + 1, next, slot + 4 < 5 ? slot + 4 : slot - 1);
-                    take(next);
+                    take(i + 1, next);
                 }
                 slot = slot + 1 < 5 ? slot + 1 : 0;
                 __syncthreads();
@@ -877,6 +892,8 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
         int qfirst = a.causal ? (int)tile * 32 * NW - shift : 0;
         qfirst = qfirst < 0 ? 0 : qfirst;
         const int p0 = qfirst >> 6, np = (z.nq + 63) >> 6;
+        arrived(kf);
+        arrived(vf);
         for (int g = 0; g < rep && p0 < np; ++g) {
             const int h = hk * rep + g;
             const bf16_t* Qb = a.Q + (int64_t)z.q0 * a.ldq + h * D;
@@ -888,18 +905,23 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
             auto fetch_all = [&](int q0) {
                 sg.fetch(sv, tid, Qb, a.ldq, Db, a.lddo, q0, z.nq);
                 if (tid < 64) {
-                    const int qi = q0 + tid;
-                    nl = qi < z.nq ? lseb[qi] : -INFINITY;
-                    nd = qi < z.nq ? -delb[qi] : 0.f;
-                    // lse in units of the raw score; a row that saw nothing, or none at all: P = 0
-                    nl = nl == -INFINITY ? -INFINITY : -nl * a.inv_scale;
+                    const int qi = q0 + tid < z.nq ? q0 + tid : z.nq - 1;
+                    nl = lseb[qi];
+                    nd = delb[qi];
                 }
             };
             auto commit_all = [&](bf16_t* buf, int q0) {
                 const int left = z.nq - q0;
                 stage_commit<D, NTHR>(buf, sv, tid, left >= 64 ? ~0ull : (1ull << left) - 1);
                 float* st = reinterpret_cast<float*>(buf + 2 * SC::TILE);
-                if (tid < 64) { st[tid] = nl; st[64 + tid] = nl + cleft; st[128 + tid] = nl + cright; st[192 + tid] = nd; }
+                if (tid < 64) {                                         // lse in units of the raw score; a row that saw nothing, or none at all: P = 0
+                    const bool ok = tid < left && nl != -INFINITY;
+                    const float l = ok ? -nl * a.inv_scale : -INFINITY;
+                    st[tid] = l;
+                    st[64 + tid] = l + cleft;
+                    st[128 + tid] = l + cright;
+                    st[192 + tid] = ok ? -nd : 0.f;
+                }
             };
             fetch_all(64 * p0);
             fill_bias(a, h, bv, tid, NTHR);
