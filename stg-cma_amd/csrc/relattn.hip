@@ -197,6 +197,10 @@ template <int D, int NTHR> struct Stage {
             off1[i] = 2 * ((uint32_t)stage_row<D, NTHR>(tid, i) * (uint32_t)ld1 + stage_col<D, NTHR>(tid, i));
         }
     }
+    // one of the two tensors into HALF registers
+    __device__ __forceinline__ void fetch1(U4Arr<C::HALF>& v, int tid, const bf16_t* t, int64_t ld, int which, int row0, int n) const {
+        stage_one<D, NTHR>(v, tid, t, ld, which ? off1 : off0, row0, n);
+    }
     __device__ __forceinline__ void fetch(U4Arr<C::PER>& v, int tid, const bf16_t* t0, int64_t ld0, const bf16_t* t1, int64_t ld1, int row0, int n) const {
         stage_one<D, NTHR>(v, tid, t0, ld0, off0, row0, n);
         stage_one<D, NTHR>(v + C::HALF, tid, t1, ld1, off1, row0, n);
@@ -204,17 +208,21 @@ template <int D, int NTHR> struct Stage {
 };
 // `valid`: bit r set = row r of the tile takes part; other rows are written as zeros
 template <int D, int NTHR>
-__device__ __forceinline__ void stage_commit(bf16_t* s, U4Arr<StageC<D, NTHR>::PER>& v, int tid, uint64_t valid) {
+__device__ __forceinline__ void commit_one(bf16_t* s, u32x4_t* v, int tid, uint64_t valid) {
     using C = StageC<D, NTHR>;
     if (valid != ~0ull) {
         asm volatile("");
 #pragma unroll
-        for (int i = 0; i < C::PER; ++i)
-            if (!((valid >> stage_row<D, NTHR>(tid, i % C::HALF)) & 1)) v[i] = (u32x4_t){0u, 0u, 0u, 0u};
+        for (int i = 0; i < C::HALF; ++i)
+            if (!((valid >> stage_row<D, NTHR>(tid, i)) & 1)) v[i] = (u32x4_t){0u, 0u, 0u, 0u};
     }
 #pragma unroll
-    for (int i = 0; i < C::PER; ++i)
-        *reinterpret_cast<u32x4_t*>(s + (i / C::HALF) * C::TILE + stage_row<D, NTHR>(tid, i % C::HALF) * C::DP + stage_col<D, NTHR>(tid, i % C::HALF)) = v[i];
+    for (int i = 0; i < C::HALF; ++i) *reinterpret_cast<u32x4_t*>(s + stage_row<D, NTHR>(tid, i) * C::DP + stage_col<D, NTHR>(tid, i)) = v[i];
+}
+template <int D, int NTHR>
+__device__ __forceinline__ void stage_commit(bf16_t* s, U4Arr<StageC<D, NTHR>::PER>& v, int tid, uint64_t valid) {
+    commit_one<D, NTHR>(s, v, tid, valid);
+    commit_one<D, NTHR>(s + StageC<D, NTHR>::TILE, v + StageC<D, NTHR>::HALF, tid, valid);
 }
 // The 64 keys kb .. kb + 63 of a sequence that exist and are not masked: key_load asks for the lane's mask byte (nothing looks at it yet: the load stays
 // in flight), key_bits makes the wave-uniform bits of them.
@@ -430,8 +438,9 @@ struct Comp {                                                           // compe
     }
 };
 template <int D, int NW, bool TAB>
-__global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP a) {
+__global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
+    constexpr bool SPLIT = D >= 96;
     using SC = StageC<D, NTHR>;
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
     const int blen = 2 * (a.far + PAD) + 1;
@@ -498,14 +507,24 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
         // dP - delta: the accumulator starts at -delta, 16 registers held for that where there is room (D <= 64), else a subtraction
         constexpr bool HOLD = D <= 64;
         const f32x16_t ndel = splat16(HOLD ? -delta : 0.f);
-        u32x4_t sv[SC::PER];
-        uint64_t bits = 0;
+        // Wide heads: K and V take turns in one half's staging registers (K arrives behind the first 32 keys' products, V behind the second's), which
+        // leaves room for two waves per SIMD.
+        u32x4_t sv[SPLIT ? SC::HALF : SC::PER];
+        uint64_t bits = 0, nbits = 0;
         int mk = 0;
         if (np > 0) {
             mk = key_load(a, z, 0, lane);
-            sg.fetch(sv, tid, Kb, a.ldk, Vb, a.ldv, 0, z.nk);
-            bits = key_bits(a, z, mk, 0, lane);
-            stage_commit<D, NTHR>(smem, sv, tid, bits);
+            if constexpr (SPLIT) {
+                sg.fetch1(sv, tid, Kb, a.ldk, 0, 0, z.nk);
+                bits = key_bits(a, z, mk, 0, lane);
+                commit_one<D, NTHR>(smem, sv, tid, bits);
+                sg.fetch1(sv, tid, Vb, a.ldv, 1, 0, z.nk);
+                commit_one<D, NTHR>(smem + SC::TILE, sv, tid, bits);
+            } else {
+                sg.fetch(sv, tid, Kb, a.ldk, Vb, a.ldv, 0, z.nk);
+                bits = key_bits(a, z, mk, 0, lane);
+                stage_commit<D, NTHR>(smem, sv, tid, bits);
+            }
         }
         __syncthreads();
         arrived(qf);
@@ -516,10 +535,13 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
             const int kb = 64 * kp;
             if (kp + 1 < np) {
                 mk = key_load(a, z, kb + 64, lane);
-                sg.fetch(sv, tid, Kb, a.ldk, Vb, a.ldv, kb + 64, z.nk);
+                if constexpr (SPLIT) sg.fetch1(sv, tid, Kb, a.ldk, 0, kb + 64, z.nk);
+                else sg.fetch(sv, tid, Kb, a.ldk, Vb, a.ldv, kb + 64, z.nk);
             }
+            bf16_t* nK = smem + ((kp + 1) & 1) * 2 * SC::TILE;
             const bool left = kb + 63 - plo <= -a.far, right = kb - phi >= a.far;
-            if (live && bits != 0 && !(a.causal && kb > phi)) {
+            const bool act = live && bits != 0 && !(a.causal && kb > phi);
+            {
                 const int idx0 = kb + 4 * hh - pos + a.far + PAD;
                 uint64_t vis = bits;
                 if (a.causal) {
@@ -531,57 +553,71 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dq_kernel(RP
                 const float nf = left ? nl + cleft : (right ? nl + cright : nl);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {              // the two 32-key tiles, one after the other (register budget)
-                    const bf16_t* tK = sK + half * 32 * DP;
-                    const bf16_t* tV = sV + half * 32 * DP;
-                    const int idx = idx0 + 32 * half;
-                    f32x16_t sc, dp = MFMA32(nat_frag<DP>(tV, r, hh, 0), df[0], ndel);
-                    if (left || right) sc = MFMA32(nat_frag<DP>(tK, r, hh, 0), qf[0], splat16(0.f));
-                    else sc = MFMA32(nat_frag<DP>(tK, r, hh, 0), qf[0], bias16(bv, idx));
+                    if (act) {
+                        const bf16_t* tK = sK + half * 32 * DP;
+                        const bf16_t* tV = sV + half * 32 * DP;
+                        const int idx = idx0 + 32 * half;
+                        f32x16_t sc, dp = MFMA32(nat_frag<DP>(tV, r, hh, 0), df[0], ndel);
+                        if (left || right) sc = MFMA32(nat_frag<DP>(tK, r, hh, 0), qf[0], splat16(0.f));
+                        else sc = MFMA32(nat_frag<DP>(tK, r, hh, 0), qf[0], bias16(bv, idx));
 #pragma unroll
-                    for (int s = 1; s < KS; ++s) {
-                        sc = MFMA32(nat_frag<DP>(tK, r, hh, s), qf[s], sc);
-                        dp = MFMA32(nat_frag<DP>(tV, r, hh, s), df[s], dp);
-                    }
-                    float p[16], ds[16];
-#pragma unroll
-                    for (int reg = 0; reg < 16; ++reg) {
-                        p[reg] = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nf));
-                        ds[reg] = p[reg] * (HOLD ? dp[reg] : dp[reg] - delta);
-                    }
-                    if (edge) {
-                        asm volatile("");                           // (kept a branch: as selects these run in every tile)
+                        for (int s = 1; s < KS; ++s) {
+                            sc = MFMA32(nat_frag<DP>(tK, r, hh, s), qf[s], sc);
+                            dp = MFMA32(nat_frag<DP>(tV, r, hh, s), df[s], dp);
+                        }
+                        float p[16], ds[16];
 #pragma unroll
                         for (int reg = 0; reg < 16; ++reg) {
-                            const bool on = (vis >> (32 * half + ACC_ROW(reg, 0))) & 1;
-                            p[reg] = on ? p[reg] : 0.f;
-                            ds[reg] = on ? ds[reg] : 0.f;
+                            p[reg] = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nf));
+                            ds[reg] = p[reg] * (HOLD ? dp[reg] : dp[reg] - delta);
+                        }
+                        if (edge) {
+                            asm volatile("");                           // (kept a branch: as selects these run in every tile)
+#pragma unroll
+                            for (int reg = 0; reg < 16; ++reg) {
+                                const bool on = (vis >> (32 * half + ACC_ROW(reg, 0))) & 1;
+                                p[reg] = on ? p[reg] : 0.f;
+                                ds[reg] = on ? ds[reg] : 0.f;
+                            }
+                        }
+                        if (TAB) {
+                            float t = 0.f;
+#pragma unroll
+                            for (int reg = 0; reg < 16; ++reg) t += ds[reg];
+                            all.add(t);
+                            if (left) sl.add(t);
+                            if (right) sr.add(t);
+                            if (!left) {                            // the probability behind the left border is what is left of one
+                                float b = 0.f;
+#pragma unroll
+                                for (int reg = 0; reg < 16; ++reg) b += p[reg];
+                                if (right) br += b; else bn += b;
+                            }
+                        }
+                        const bf16x8_t d0 = pack8(ds), d1 = pack8(ds + 8);
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) {
+                            dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 0, hh, r), d0, dq[dt]);
+                            dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 1, hh, r), d1, dq[dt]);
                         }
                     }
-                    if (TAB) {
-                        float t = 0.f;
-#pragma unroll
-                        for (int reg = 0; reg < 16; ++reg) t += ds[reg];
-                        all.add(t);
-                        if (left) sl.add(t);
-                        if (right) sr.add(t);
-                        if (!left) {                            // the probability behind the left border is what is left of one
-                            float b = 0.f;
-#pragma unroll
-                            for (int reg = 0; reg < 16; ++reg) b += p[reg];
-                            if (right) br += b; else bn += b;
+                    if constexpr (SPLIT) {
+                        if (half == 0 && kp + 1 < np) {
+                            nbits = key_bits(a, z, mk, kb + 64, lane);
+                            commit_one<D, NTHR>(nK, sv, tid, nbits);
+                            sg.fetch1(sv, tid, Vb, a.ldv, 1, kb + 64, z.nk);
                         }
-                    }
-                    const bf16x8_t d0 = pack8(ds), d1 = pack8(ds + 8);
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 0, hh, r), d0, dq[dt]);
-                        dq[dt] = MFMA32(tr_frag<DP>(tK, dt, 1, hh, r), d1, dq[dt]);
                     }
                 }
             }
             if (kp + 1 < np) {
-                bits = key_bits(a, z, mk, kb + 64, lane);
-                stage_commit<D, NTHR>(smem + ((kp + 1) & 1) * 2 * SC::TILE, sv, tid, bits);
+                if constexpr (SPLIT) {
+                    commit_one<D, NTHR>(nK + SC::TILE, sv, tid, nbits);
+                    bits = nbits;
+                } else {
+                    bits = key_bits(a, z, mk, kb + 64, lane);
+                    stage_commit<D, NTHR>(nK, sv, tid, bits);
+                }
             }
             __syncthreads();
         }
@@ -846,6 +882,7 @@ __global__ void __launch_bounds__(256) relattn_dtable_kernel(const float* band, 
 template <int D, int NW>
 __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
+    constexpr bool WIDE = D >= 96;
     using SC = StageC<D, NTHR>;
     constexpr int BUF = 2 * SC::TILE + 512;                             // Q and dO tiles + 4 x 64 floats of statistics
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
@@ -960,11 +997,22 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
 #pragma unroll
                             for (int reg = 0; reg < 16; ++reg) sc[reg] += bp[-ACC_ROW(reg, 0)];
                         }
+                        // one wave per SIMD (D >= 96): nothing else hides the LDS latency, so the operands of a whole phase are asked for at once
+                        bf16x8_t qa[KS], da[KS];
+#pragma unroll
+                        for (int s = 0; s < KS; ++s) { qa[s] = nat_frag<DP>(tQ, r, hh, s); da[s] = nat_frag<DP>(tD, r, hh, s); }
+                        if (WIDE) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                         for (int s = 0; s < KS; ++s) {
-                            sc = MFMA32(nat_frag<DP>(tQ, r, hh, s), kf[s], sc);
-                            dp = MFMA32(nat_frag<DP>(tD, r, hh, s), vf[s], dp);
+                            sc = MFMA32(qa[s], kf[s], sc);
+                            dp = MFMA32(da[s], vf[s], dp);
                         }
+                        bf16x8_t to[2][4];                              // transposed operands of one 32-column block: dO, dO, Q, Q
+                        auto trans = [&](int dt) {
+                            to[dt & 1][0] = tr_frag<DP>(tD, dt, 0, hh, r); to[dt & 1][1] = tr_frag<DP>(tD, dt, 1, hh, r);
+                            to[dt & 1][2] = tr_frag<DP>(tQ, dt, 0, hh, r); to[dt & 1][3] = tr_frag<DP>(tQ, dt, 1, hh, r);
+                        };
+                        if (WIDE) { trans(0); __builtin_amdgcn_sched_barrier(0); }
                         float pr[16], ds[16];
 #pragma unroll
                         for (int reg = 0; reg < 16; ++reg) {
@@ -981,12 +1029,15 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                             }
                         }
                         const bf16x8_t a0 = pack8(pr), a1 = pack8(pr + 8), d0 = pack8(ds), d1 = pack8(ds + 8);
+                        if (!WIDE) trans(0);
 #pragma unroll
                         for (int dt = 0; dt < DT; ++dt) {
-                            dv[dt] = MFMA32(tr_frag<DP>(tD, dt, 0, hh, r), a0, dv[dt]);
-                            dv[dt] = MFMA32(tr_frag<DP>(tD, dt, 1, hh, r), a1, dv[dt]);
-                            dk[dt] = MFMA32(tr_frag<DP>(tQ, dt, 0, hh, r), d0, dk[dt]);
-                            dk[dt] = MFMA32(tr_frag<DP>(tQ, dt, 1, hh, r), d1, dk[dt]);
+                            if (dt + 1 < DT) trans(dt + 1);
+                            if (WIDE) __builtin_amdgcn_sched_barrier(0);
+                            dv[dt] = MFMA32(to[dt & 1][0], a0, dv[dt]);
+                            dk[dt] = MFMA32(to[dt & 1][2], d0, dk[dt]);
+                            dv[dt] = MFMA32(to[dt & 1][1], a1, dv[dt]);
+                            dk[dt] = MFMA32(to[dt & 1][3], d1, dk[dt]);
                         }
                     }
                 }
