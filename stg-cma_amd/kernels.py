@@ -2196,6 +2196,19 @@ def _rel_chk(t, name, dtype, cols, dev, rows=None):
         raise RuntimeError(f"{name}: rows must start 16-byte aligned (leading dimension {_ld(t)}, a multiple of 8)")
 
 
+def _rel_rows(t, name, dtype, cols, dev, rows=None):
+    """Leading dimension of a row tensor the kernels can take (one pass over its attributes; _rel_chk says what is wrong otherwise)."""
+    shape = t.shape
+    if len(shape) == 2 and t.dtype is dtype and t.device == dev and dev.type == "cuda" and shape[1] == cols and (rows is None or shape[0] == rows):
+        ld, one = t.stride()
+        if shape[0] <= 1:
+            ld = cols
+        if one == 1 and ld >= cols and not ld % 8 and not t.data_ptr() % 16:
+            return ld
+    _rel_chk(t, name, dtype, cols, dev, rows)
+    return _ld(t)
+
+
 def _rel_int32(t, name, n, dev):
     if t.device != dev or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n) or t.shape[0] < 1:
         raise RuntimeError(f"{name}: expected a contiguous int32 vector{'' if n is None else f' of {n}'} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
@@ -2208,26 +2221,27 @@ def _rel_table(g, table, dev):
 
 def _rel_fill(g, q, k, v, o, lse, table, cu_q, cu_k, max_q, max_k, key_mask):
     dev = q.device
-    _rel_chk(q, "q", BF16, g.H * g.D, dev)
-    _rel_chk(k, "k", BF16, g.Hkv * g.D, dev)
-    _rel_chk(v, "v", BF16, g.Hkv * g.D, dev, rows=k.shape[0])
-    _rel_chk(o, "o", BF16, g.H * g.D, dev, rows=q.shape[0])
+    hd, kd = g.H * g.D, g.Hkv * g.D
+    Tq, Tk = q.shape[0], k.shape[0]
+    ldq, ldk = _rel_rows(q, "q", BF16, hd, dev), _rel_rows(k, "k", BF16, kd, dev)
+    ldv, ldo = _rel_rows(v, "v", BF16, kd, dev, Tk), _rel_rows(o, "o", BF16, hd, dev, Tq)
     _rel_table(g, table, dev)
     self_attn = cu_k is None or cu_k is cu_q
-    cu_k = cu_q if cu_k is None else cu_k
     _rel_int32(cu_q, "cu_q", None, dev)
-    _rel_int32(cu_k, "cu_k", cu_q.shape[0], dev)
-    max_q = q.shape[0] if max_q is None else int(max_q)
-    max_k = (max_q if self_attn else k.shape[0]) if max_k is None else int(max_k)
+    if self_attn:
+        cu_k = cu_q
+    else:
+        _rel_int32(cu_k, "cu_k", cu_q.shape[0], dev)
+    max_q = Tq if max_q is None else int(max_q)
+    max_k = (max_q if self_attn else Tk) if max_k is None else int(max_k)
     if max_q < 0 or max_k < 0:
         raise RuntimeError(f"relattn: max_q={max_q}, max_k={max_k}")
     if key_mask is not None:
-        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.dim() != 1 or key_mask.shape[0] != k.shape[0] or not key_mask.is_contiguous() or key_mask.device != dev:
-            raise RuntimeError(f"key_mask: expected a contiguous bool / uint8 vector of {k.shape[0]} on {dev}, got {key_mask.dtype} {tuple(key_mask.shape)}")
-    if lse is not None and (lse.dtype != F32 or tuple(lse.shape) != (g.H, q.shape[0]) or not lse.is_contiguous() or lse.device != dev):
-        raise RuntimeError(f"lse: expected contiguous fp32 [{g.H}, {q.shape[0]}]")
-    Tq, Tk = q.shape[0], k.shape[0]
-    return _lib.RelAttnArgs(_p(q), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), o.data_ptr(), _ld(o), None if lse is None else lse.data_ptr(), cu_q.data_ptr(),
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.dim() != 1 or key_mask.shape[0] != Tk or not key_mask.is_contiguous() or key_mask.device != dev:
+            raise RuntimeError(f"key_mask: expected a contiguous bool / uint8 vector of {Tk} on {dev}, got {key_mask.dtype} {tuple(key_mask.shape)}")
+    if lse is not None and (lse.dtype != F32 or tuple(lse.shape) != (g.H, Tq) or not lse.is_contiguous() or lse.device != dev):
+        raise RuntimeError(f"lse: expected contiguous fp32 [{g.H}, {Tq}]")
+    return _lib.RelAttnArgs(_p(q), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(), ldo, None if lse is None else lse.data_ptr(), cu_q.data_ptr(),
                             cu_k.data_ptr(), None if key_mask is None else key_mask.data_ptr(), Tq, Tk, cu_q.shape[0] - 1, min(max_q, Tq), min(max_k, Tk), g.H, g.Hkv, g.D,
                             g.scale, g.causal, table.data_ptr(), g.plan(dev).data_ptr(), g.num_buckets, g.far, 0)
 
@@ -2274,7 +2288,8 @@ def _relattn_bwd(a, dev, do, want_table):
     ref = C.byref(a)
     n = lib.stg_relattn_bwd_ws_floats(ref, int(want_table))
     ws = torch.empty((max(n, 1),), dtype=F32, device=dev)
-    _lib.check(lib.stg_relattn_bwd(ref, _p(do), _ld(do), _p(dq), hd, _p(dk), kd, _p(dv), kd, _p(dtable), _p(ws), n, _stream()), "stg_relattn_bwd")
+    _lib.check(lib.stg_relattn_bwd(ref, _p(do), _ld(do), dq.data_ptr(), hd, dk.data_ptr(), kd, dv.data_ptr(), kd, dtable.data_ptr() if want_table else None,
+                                   ws.data_ptr(), n, _stream()), "stg_relattn_bwd")
     return dq, dk, dv, dtable
 
 
@@ -2314,50 +2329,55 @@ def relattn_decode(g, q, k_cache, v_cache, table, lens, out=None):
 _NORM_KINDS = {"layer": 0, "rms": 1}
 
 
-def _norm_join_args(x_new, h, gate, post_w, post_b, pre_w, pre_b, kind, alpha, eps, rows_per_group, stats):
-    dev = x_new.device
-    if x_new.dtype not in (BF16, F32):
-        raise RuntimeError(f"norm_join: the stream is bf16 or fp32, got {x_new.dtype}")
-    if kind not in _NORM_KINDS:
+def _norm_join_args(x, x_new, h, y, gate, weights, kind, alpha, eps, rows_per_group, stats):
+    """The checked description: weights = post_w, post_b, pre_w, pre_b; x and y may be None (the backward does not read them)."""
+    dev, dtype = x_new.device, x_new.dtype
+    if dtype is not BF16 and dtype is not F32:
+        raise RuntimeError(f"norm_join: the stream is bf16 or fp32, got {dtype}")
+    rms = _NORM_KINDS.get(kind)
+    if rms is None:
         raise RuntimeError(f"norm_join: kind {kind!r} (layer or rms)")
     R, Cw = x_new.shape
     if Cw % 8 or Cw > 8192 or Cw == 0:
         raise RuntimeError(f"norm_join: width {Cw} (a multiple of 8 up to 8192)")
-    _rel_chk(h, "h", BF16, Cw, dev, rows=R)
-    for t, name, must in ((post_w, "post_w", True), (post_b, "post_b", False), (pre_w, "pre_w", True), (pre_b, "pre_b", False)):
+    ldxo, ldh = _rel_rows(x_new, "x", dtype, Cw, dev), _rel_rows(h, "h", BF16, Cw, dev, R)
+    if weights[0] is None or weights[2] is None:
+        raise RuntimeError("norm_join: post_w and pre_w are needed")
+    ptrs = []
+    for t, name in zip(weights, ("post_w", "post_b", "pre_w", "pre_b")):
         if t is None:
-            if must:
-                raise RuntimeError(f"norm_join: {name} is needed")
+            ptrs.append(None)
             continue
-        _chk1d(t, name, F32, Cw)
-        if t.device != dev or t.data_ptr() % 16:
-            raise RuntimeError(f"{name}: expected a 16-byte aligned vector on {dev}")
-    a = _lib.NormJoinArgs()
-    a.gate_kind, a.rows_per_group = 0, 0
+        p = t.data_ptr()
+        if t.dtype is not F32 or t.device != dev or p % 16 or t.dim() != 1 or t.shape[0] != Cw or not t.is_contiguous():
+            raise RuntimeError(f"{name}: expected a contiguous, 16-byte aligned fp32 vector of {Cw} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        ptrs.append(p)
+    gk = rpg = 0
     if gate is not None:
-        if gate.device != dev or gate.dtype != F32 or not gate.is_contiguous() or gate.data_ptr() % 16:
+        if gate.device != dev or gate.dtype is not F32 or not gate.is_contiguous() or gate.data_ptr() % 16:
             raise RuntimeError(f"gate: expected a contiguous, 16-byte aligned fp32 tensor on {dev}")
-        if gate.dim() == 2:
+        sh = gate.shape
+        if len(sh) == 2:
             if not rows_per_group or int(rows_per_group) < 1:
                 raise RuntimeError("norm_join: a gate by row groups needs rows_per_group")
-            a.gate_kind, a.rows_per_group = 3, int(rows_per_group)
-            if tuple(gate.shape) != (-(-R // a.rows_per_group), Cw):
-                raise RuntimeError(f"gate: expected [{-(-R // a.rows_per_group)}, {Cw}], got {tuple(gate.shape)}")
-        elif gate.numel() == 1 and gate.dim() <= 1:
-            a.gate_kind = 1
-        elif gate.dim() == 1 and gate.shape[0] == Cw:
-            a.gate_kind = 2
+            gk, rpg = 3, int(rows_per_group)
+            if tuple(sh) != (-(-R // rpg), Cw):
+                raise RuntimeError(f"gate: expected [{-(-R // rpg)}, {Cw}], got {tuple(sh)}")
+        elif len(sh) == 0 or tuple(sh) == (1,):
+            gk = 1
+        elif tuple(sh) == (Cw,):
+            gk = 2
         else:
-            raise RuntimeError(f"gate: expected one value, [{Cw}] or [groups, {Cw}], got {tuple(gate.shape)}")
-    if stats is not None and (stats.dtype != F32 or tuple(stats.shape) != (R, 4) or not stats.is_contiguous() or stats.device != dev):
+            raise RuntimeError(f"gate: expected one value, [{Cw}] or [groups, {Cw}], got {tuple(sh)}")
+    if stats is not None and (stats.dtype is not F32 or tuple(stats.shape) != (R, 4) or not stats.is_contiguous() or stats.device != dev):
         raise RuntimeError(f"norm_join: stats must be contiguous fp32 [{R}, 4]")
-    a.x_dtype = _dt(x_new)
-    a.h, a.ldh, a.gate = _p(h), _ld(h), _p(gate)
-    a.w1, a.b1, a.w2, a.b2 = _p(post_w), _p(post_b), _p(pre_w), _p(pre_b)
-    a.alpha, a.eps, a.rms = float(alpha), float(eps), _NORM_KINDS[kind]
-    a.stats, a.rows, a.C = _p(stats), R, Cw
-    a.xo, a.ldxo = _p(x_new), _ld(x_new)
-    return a
+    xp = yp = None
+    ldx = 0
+    if x is not None:
+        ldx = _rel_rows(x, "x", dtype, Cw, dev, R)
+        xp, yp = x.data_ptr(), y.data_ptr()
+    return _lib.NormJoinArgs(xp, ldx, STG_BF16 if dtype is BF16 else STG_F32, _p(h), ldh, None if gate is None else gate.data_ptr(), gk, rpg, *ptrs, alpha, eps, rms,
+                             x_new.data_ptr(), ldxo, yp, Cw, None if stats is None else stats.data_ptr(), R, Cw)
 
 
 def norm_join_fwd(x, h, gate, post_w, post_b, pre_w, pre_b, *, kind="layer", alpha=1.0, eps=1e-5, rows_per_group=None, want_stats=True):
@@ -2366,18 +2386,17 @@ def norm_join_fwd(x, h, gate, post_w, post_b, pre_w, pre_b, *, kind="layer", alp
     x fp32 / bf16 [rows, C] (the residual stream), h bf16 [rows, C] (the block's output); gate None, one fp32 value, [C], or [groups, C] with
     rows_per_group consecutive rows to a group; weights fp32 [C] (biases may be None); kind "layer" or "rms".  Returns (x_new in x's type,
     y bf16, stats fp32 [rows, 4] for norm_join_bwd or None)."""
-    return _norm_join_fwd(x, h, gate, post_w, post_b, pre_w, pre_b, kind, alpha, eps, rows_per_group, want_stats)[:3]
+    return _norm_join_fwd(x, h, gate, (post_w, post_b, pre_w, pre_b), kind, alpha, eps, rows_per_group, want_stats)[:3]
 
 
-def _norm_join_fwd(x, h, gate, post_w, post_b, pre_w, pre_b, kind, alpha, eps, rows_per_group, want_stats):
-    _chk2d(x, "x", x.dtype)
-    x_new = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y = torch.empty(x.shape, dtype=BF16, device=x.device)
-    stats = torch.empty((x.shape[0], 4), dtype=F32, device=x.device) if want_stats else None
-    a = _norm_join_args(x_new, h, gate, post_w, post_b, pre_w, pre_b, kind, alpha, eps, rows_per_group, stats)
-    _rel_chk(x, "x", x.dtype, x.shape[1], x.device)
-    a.y, a.ldy = _p(y), _ld(y)
-    a.x, a.ldx = _p(x), _ld(x)
+def _norm_join_fwd(x, h, gate, weights, kind, alpha, eps, rows_per_group, want_stats):
+    dev, shape = x.device, x.shape
+    if len(shape) != 2 or dev.type != "cuda":
+        _chk2d(x, "x", x.dtype)
+    x_new = torch.empty(shape, dtype=x.dtype, device=dev)
+    y = torch.empty(shape, dtype=BF16, device=dev)
+    stats = torch.empty((shape[0], 4), dtype=F32, device=dev) if want_stats else None
+    a = _norm_join_args(x, x_new, h, y, gate, weights, kind, alpha, eps, rows_per_group, stats)
     _lib.check(_lib.lib().stg_norm_join_fwd(C.byref(a), _stream()), "stg_norm_join_fwd")
     return x_new, y, stats, a
 
@@ -2390,43 +2409,47 @@ def norm_join_bwd(x_new, h, gate, post_w, post_b, pre_w, pre_b, stats, dy, dx_ne
     R, Cw = x_new.shape
     if stats is None:
         raise RuntimeError("norm_join_bwd: needs the forward's stats")
-    a = _norm_join_args(x_new, h, gate, post_w, post_b, pre_w, pre_b, kind, alpha, eps, rows_per_group, stats)
-    _rel_chk(x_new, "x_new", x_new.dtype, Cw, x_new.device)
-    _rel_chk(dy, "dy", BF16, Cw, x_new.device, rows=R)
+    weights = (post_w, post_b, pre_w, pre_b)
+    a = _norm_join_args(None, x_new, h, None, gate, weights, kind, alpha, eps, rows_per_group, stats)
+    _rel_rows(dy, "dy", BF16, Cw, x_new.device, R)
     if dx_new is not None:
-        _rel_chk(dx_new, "dx_new", x_new.dtype, Cw, x_new.device, rows=R)
-    dx, dh, g = _norm_join_bwd(a, x_new.device, x_new.dtype, dy, dx_new, [None if t is None else t.shape for t in (post_w, post_b, pre_w, pre_b, gate)], want_params,
-                               want_gate)
-    return dict(zip(("dx", "dh", "dpost_w", "dpost_b", "dpre_w", "dpre_b", "dgate"), (dx, dh) + tuple(g)))
+        _rel_rows(dx_new, "dx_new", x_new.dtype, Cw, x_new.device, R)
+    g = _norm_join_bwd(a, x_new.device, x_new.dtype, dy, dx_new, weights, gate, want_params, want_gate)
+    return dict(zip(("dx", "dh", "dpost_w", "dpost_b", "dpre_w", "dpre_b", "dgate"), g))
 
 
-def _norm_join_bwd(a, dev, dtype, dy, dx_new, shapes, want_params, want_gate):
-    """The backward of a checked description (every pointer in place); shapes of post_w, post_b, pre_w, pre_b, gate or None.  (dx, dh, their gradients)."""
-    R, Cw = a.rows, a.C
+def _norm_join_bwd(a, dev, dtype, dy, dx_new, weights, gate, want_params, want_gate):
+    """The backward of a checked description (every pointer in place): dx, dh, then the gradients of the weights and the gate (None where there are none)."""
+    R, Cw, gk = a.rows, a.C, a.gate_kind
     dx = torch.empty((R, Cw), dtype=dtype, device=dev)
     dh = torch.empty((R, Cw), dtype=BF16, device=dev)
-    lib = _lib.lib()
-    ref = C.byref(a)
-    groups = a.gate_kind == 3
-    params = want_params or (want_gate and a.gate_kind in (1, 2))
+    params = want_params or (want_gate and gk in (1, 2))
+    out = [None, None, None, None, None]
     dpar = dgate = ws = None
     nws = 0
-    if params:
-        dpar = torch.empty(((lib.stg_norm_join_param_floats(ref) + 3) // 4 * 4,), dtype=F32, device=dev)
-    if want_gate and groups:
-        dgate = torch.empty(shapes[4], dtype=F32, device=dev)
+    lib = _lib.lib()
+    ref = C.byref(a)
+    if params:                                                # one buffer, in the C call's order
+        which = [i for i in range(4) if weights[i] is not None]
+        sizes = [Cw] * len(which)
+        if gk in (1, 2):
+            which.append(4)
+            sizes.append(1 if gk == 1 else Cw)
+        n = sum(sizes)
+        if n % 4:
+            sizes.append(4 - n % 4)
+            n += 4 - n % 4
+        dpar = torch.empty((n,), dtype=F32, device=dev)
+        for i, t in zip(which, dpar.split(sizes)):
+            out[i] = t
+        if gk == 1 and gate.dim() == 0:
+            out[4] = out[4].view(())
+    if gk == 3 and want_gate:
+        dgate = out[4] = torch.empty(gate.shape, dtype=F32, device=dev)
     if params or dgate is not None:
         nws = lib.stg_norm_join_bwd_ws_floats(ref)
         ws = torch.empty((nws,), dtype=F32, device=dev)
-    _lib.check(lib.stg_norm_join_bwd(ref, _p(dy), _ld(dy), _p(dx_new), _ld(dx_new) if dx_new is not None else 0, _p(dx), Cw, _p(dh), Cw, _p(dpar), _p(dgate), _p(ws),
-                                     nws, _stream()), "stg_norm_join_bwd")
-    out = [None, None, None, None, dgate]
-    if params:
-        at = 0
-        for i, sh in enumerate(shapes):
-            if sh is not None and not (i == 4 and groups):
-                n = sh[0] if len(sh) else 1
-                t = dpar[at:at + n]
-                out[i] = t if len(sh) == 1 else t.view(sh)
-                at += n
-    return dx, dh, out
+    ptr = lambda t: None if t is None else t.data_ptr()
+    _lib.check(lib.stg_norm_join_bwd(ref, _p(dy), _ld(dy), ptr(dx_new), _ld(dx_new) if dx_new is not None else 0, dx.data_ptr(), Cw, dh.data_ptr(), Cw, ptr(dpar),
+                                     ptr(dgate), ptr(ws), nws, _stream()), "stg_norm_join_bwd")
+    return [dx, dh] + out

@@ -43,9 +43,8 @@ class RelAttentionFn(torch.autograd.Function):
         q, k, v, o, lse, table, cu_q, cu_k, key_mask, plan = ctx.saved_tensors
         need = ctx.needs_input_grad
         a = type(ctx.call).from_buffer_copy(ctx.call)
-        for t, name in ((q, "q"), (k, "k"), (v, "v"), (o, "o")):
-            setattr(a, name.upper(), t.data_ptr())
-            setattr(a, "ld" + name, K._ld(t))                  # (hooks may have stored a dense copy)
+        a.Q, a.K, a.V, a.O = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr()
+        a.ldq, a.ldk, a.ldv, a.ldo = K._ld(q), K._ld(k), K._ld(v), K._ld(o)      # (hooks may have stored a dense copy)
         a.lse, a.table, a.cu_q, a.plan = lse.data_ptr(), table.data_ptr(), cu_q.data_ptr(), plan.data_ptr()
         a.cu_k = a.cu_q if cu_k is None else cu_k.data_ptr()
         a.key_mask = None if key_mask is None else key_mask.data_ptr()
@@ -63,7 +62,7 @@ class NormJoinFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, h, gate, post_w, post_b, pre_w, pre_b, kind, alpha, eps, rows_per_group):
         train = any(ctx.needs_input_grad[:7])
-        x_new, y, stats, a = K._norm_join_fwd(x, h, gate, post_w, post_b, pre_w, pre_b, kind, alpha, eps, rows_per_group, train)
+        x_new, y, stats, a = K._norm_join_fwd(x, h, gate, (post_w, post_b, pre_w, pre_b), kind, alpha, eps, rows_per_group, train)
         if train:
             ctx.save_for_backward(x_new, h, stats, gate, post_w, post_b, pre_w, pre_b)
             ctx.call = a                                       # the checked sizes and strides; its pointers are taken again from the saved tensors
@@ -80,13 +79,19 @@ class NormJoinFn(torch.autograd.Function):
         a = type(ctx.call).from_buffer_copy(ctx.call)
         a.xo, a.h, a.stats, a.w1, a.w2 = x_new.data_ptr(), h.data_ptr(), stats.data_ptr(), post_w.data_ptr(), pre_w.data_ptr()
         a.ldxo, a.ldh = K._ld(x_new), K._ld(h)
-        a.gate, a.b1, a.b2 = (None if t is None else t.data_ptr() for t in (gate, post_b, pre_b))
+        if gate is not None:
+            a.gate = gate.data_ptr()
+        if post_b is not None:
+            a.b1 = post_b.data_ptr()
+        if pre_b is not None:
+            a.b2 = pre_b.data_ptr()
         dy = torch.zeros(h.shape, dtype=BF16, device=h.device) if dy is None else _ready(dy, BF16)
         if dx_new is not None:
             dx_new = _ready(dx_new, x_new.dtype)
-        shapes = [None if t is None else t.shape for t in (post_w, post_b, pre_w, pre_b, gate)]
-        dx, dh, (dw1, db1, dw2, db2, dg) = K._norm_join_bwd(a, h.device, x_new.dtype, dy, dx_new, shapes, any(need[3:7]), need[2])
-        return tuple(g if n else None for g, n in zip((dx, dh, dg, dw1, db1, dw2, db2), need)) + (None,) * 4
+        dx, dh, dw1, db1, dw2, db2, dg = K._norm_join_bwd(a, h.device, x_new.dtype, dy, dx_new, (post_w, post_b, pre_w, pre_b), gate, any(need[3:7]), need[2])
+        if not all(need[:7]):
+            dx, dh, dg, dw1, db1, dw2, db2 = (g if n else None for g, n in zip((dx, dh, dg, dw1, db1, dw2, db2), need))
+        return dx, dh, dg, dw1, db1, dw2, db2, None, None, None, None
 
 
 def norm_join(x, h, gate, post_w, post_b, pre_w, pre_b, *, kind="layer", alpha=1.0, eps=1e-5, rows_per_group=None):
