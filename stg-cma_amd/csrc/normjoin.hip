@@ -52,223 +52,335 @@ __device__ __forceinline__ void store8(float* p, const float* v) {
 __device__ __forceinline__ void round_as(float*, const float*) {}                     // fp32 stream: stored as computed
 __device__ __forceinline__ void round_as(bf16_t*, float* v) { const u4_t u = packed8(v); unpack8(u, v); }
 
-// sums over the W waves that share a row (WPR waves; every wave of the block calls it the same number of times)
-template <int WPR>
-__device__ __forceinline__ float row_sum(float v, float* red, int wave) {
-    v = wave_sum<64>(v);
-    if (WPR == 1) return v;
+// sum over the TPR threads that share a row (every wave of the block calls it the same number of times)
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+    v = wave_sum<(TPR < 64 ? TPR : 64)>(v);
+    if (TPR <= 64) return v;
+    const int wave = threadIdx.x >> 6, w0 = wave / (TPR / 64) * (TPR / 64);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[wave] = v;
     __syncthreads();
-    const int w0 = wave / WPR * WPR;
     float t = 0.f;
 #pragma unroll
-    for (int w = 0; w < WPR; ++w) t += red[w0 + w];
+    for (int w = 0; w < TPR / 64; ++w) t += red[w0 + w];
     return t;
 }
-template <int WPR>
-__device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int wave) {
-    a = wave_sum<64>(a);
-    b = wave_sum<64>(b);
-    if (WPR == 1) return;
+template <int TPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* red) {
+    a = wave_sum<(TPR < 64 ? TPR : 64)>(a);
+    b = wave_sum<(TPR < 64 ? TPR : 64)>(b);
+    if (TPR <= 64) return;
+    const int wave = threadIdx.x >> 6, w0 = wave / (TPR / 64) * (TPR / 64);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) { red[wave] = a; red[16 + wave] = b; }
+    if ((threadIdx.x & 63) == 0) { red[wave] = a; red[8 + wave] = b; }
     __syncthreads();
-    const int w0 = wave / WPR * WPR;
     a = b = 0.f;
 #pragma unroll
-    for (int w = 0; w < WPR; ++w) { a += red[w0 + w]; b += red[16 + w0 + w]; }
+    for (int w = 0; w < TPR / 64; ++w) { a += red[w0 + w]; b += red[8 + w0 + w]; }
 }
 
-// A lane owns 8 columns of the row (WPR waves of 64 lanes cover 512 WPR columns) and keeps their weights in registers over its rows.
-template <typename XT, int WPR>
-__global__ void __launch_bounds__(WPR <= 4 ? 256 : 64 * WPR) norm_join_fwd_kernel(JP a) {
-    constexpr int NW = WPR <= 4 ? 4 : WPR, RG = NW / WPR;               // waves of the block, rows in flight
-    __shared__ float red[32];
-    const int wave = threadIdx.x >> 6;
-    const int col = 8 * ((wave % WPR) * 64 + (threadIdx.x & 63));
-    const bool on = col < a.C;
+// Eight elements as they lie in memory: a row's loads are asked for one row ahead, so they stay raw until their turn.
+template <typename T> struct Raw8 { u4_t a, b; };
+template <> struct Raw8<bf16_t> { u4_t a; };
+__device__ __forceinline__ void ask(Raw8<bf16_t>& r, const bf16_t* p) { r.a = *reinterpret_cast<const u4_t*>(p); }
+__device__ __forceinline__ void ask(Raw8<float>& r, const float* p) { r.a = *reinterpret_cast<const u4_t*>(p); r.b = *reinterpret_cast<const u4_t*>(p + 4); }
+__device__ __forceinline__ void none(Raw8<bf16_t>& r) { r.a = (u4_t){0u, 0u, 0u, 0u}; }
+__device__ __forceinline__ void none(Raw8<float>& r) { r.a = r.b = (u4_t){0u, 0u, 0u, 0u}; }
+__device__ __forceinline__ void open8(const Raw8<bf16_t>& r, float* v) { unpack8(r.a, v); }
+__device__ __forceinline__ void open8(const Raw8<float>& r, float* v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(r.a[i]); v[4 + i] = __uint_as_float(r.b[i]); }
+}
+
+// TPR threads own a row, 8 NCH columns each (16 .. 512 threads: rows of up to 128 columns go four to a wave), and keep the columns' weights in registers over
+// their rows; a block of NT threads has RG rows in flight.
+template <int TPR> struct Blk { static constexpr int NT = TPR <= 256 ? 256 : TPR, RG = NT / TPR; };
+
+template <typename XT, int TPR, int NCH>
+__global__ void __launch_bounds__(Blk<TPR>::NT) norm_join_fwd_kernel(JP a) {
+    constexpr int RG = Blk<TPR>::RG;
+    __shared__ float red[16];
+    const int rg = threadIdx.x / TPR, col0 = 8 * (threadIdx.x % TPR);
     const float invC = 1.0f / (float)a.C;
-    float w1[8] = {}, b1[8] = {}, w2[8] = {}, b2[8] = {}, g[8];
+    float w1[NCH][8], b1[NCH][8], w2[NCH][8], b2[NCH][8], g[NCH][8];
+    bool on[NCH];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = 1.f;
-    if (on) {
-        load8(a.w1 + col, w1);
-        load8(a.w2 + col, w2);
-        if (a.b1) load8(a.b1 + col, b1);
-        if (a.b2) load8(a.b2 + col, b2);
-        if (a.gate_kind == 2) load8(a.gate + col, g);
-    }
-    if (a.gate_kind == 1) {
-        const float s = a.gate[0];
+    for (int c = 0; c < NCH; ++c) {
+        const int col = col0 + 8 * TPR * c;
+        on[c] = col < a.C;
+        const float s = a.gate_kind == 1 ? a.gate[0] : 1.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = s;
+        for (int i = 0; i < 8; ++i) { w1[c][i] = b1[c][i] = w2[c][i] = b2[c][i] = 0.f; g[c][i] = s; }
+        if (on[c]) {
+            load8(a.w1 + col, w1[c]);
+            load8(a.w2 + col, w2[c]);
+            if (a.b1) load8(a.b1 + col, b1[c]);
+            if (a.b2) load8(a.b2 + col, b2[c]);
+            if (a.gate_kind == 2) load8(a.gate + col, g[c]);
+        }
     }
+    Raw8<bf16_t> rh[NCH];
+    Raw8<XT> rx[NCH];
+    auto fetch = [&](int64_t row) {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const int col = col0 + 8 * TPR * c;
+            none(rh[c]);
+            none(rx[c]);
+            if (on[c] && row < a.rows) {
+                ask(rh[c], a.h + row * a.ldh + col);
+                ask(rx[c], (const XT*)a.x + row * a.ldx + col);
+            }
+        }
+    };
     const int64_t step = (int64_t)gridDim.x * RG;
+    fetch((int64_t)blockIdx.x * RG + rg);
     for (int64_t base = (int64_t)blockIdx.x * RG; base < a.rows; base += step) {
-        const int64_t row = base + wave / WPR;
-        const bool ok = on && row < a.rows;
-        float h[8] = {}, x[8] = {};
-        if (ok) {
-            load8(a.h + row * a.ldh + col, h);
-            load8((const XT*)a.x + row * a.ldx + col, x);
-            if (a.gate_kind == 3) load8(a.gate + (row / a.rpg) * a.C + col, g);
-        }
+        const int64_t row = base + rg;
+        float h[NCH][8], x[NCH][8];
         float m1 = 0.f, m2 = 0.f, s = 0.f;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            open8(rh[c], h[c]);
+            open8(rx[c], x[c]);
+            if (a.gate_kind == 3 && on[c] && row < a.rows) load8(a.gate + (row / a.rpg) * a.C + col0 + 8 * TPR * c, g[c]);
+        }
+        fetch(row + step);
         if (!a.rms) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += h[i];
-            m1 = row_sum<WPR>(s, red, wave) * invC;
+            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s += h[c][i];
+            m1 = row_sum<TPR>(s, red) * invC;
         }
         s = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { h[i] = on ? h[i] - m1 : 0.f; s = fmaf(h[i], h[i], s); }
-        const float r1 = rsqrtf(row_sum<WPR>(s, red, wave) * invC + a.eps);
+        for (int c = 0; c < NCH; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float n = fmaf(h[i] * r1, w1[i], b1[i]);
-            x[i] = fmaf(g[i], n, a.alpha * x[i]);
-        }
-        round_as((XT*)nullptr, x);
-        if (ok) store8((XT*)a.xo + row * a.ldxo + col, x);
-        s = 0.f;
-        if (!a.rms) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s += on ? x[i] : 0.f;
-            m2 = row_sum<WPR>(s, red, wave) * invC;
-        }
+            for (int i = 0; i < 8; ++i) { h[c][i] = on[c] ? h[c][i] - m1 : 0.f; s = fmaf(h[c][i], h[c][i], s); }
+        const float r1 = rsqrtf(row_sum<TPR>(s, red) * invC + a.eps);
         s = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { x[i] = on ? x[i] - m2 : 0.f; s = fmaf(x[i], x[i], s); }
-        const float r2 = rsqrtf(row_sum<WPR>(s, red, wave) * invC + a.eps);
+        for (int c = 0; c < NCH; ++c) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i] * r2, w2[i], b2[i]);
-        if (ok) store8(a.y + row * a.ldy + col, x);
-        if (a.stats && row < a.rows && col == 0) *reinterpret_cast<f4_t*>(a.stats + 4 * row) = (f4_t){m1, r1, m2, r2};
+            for (int i = 0; i < 8; ++i) {
+                const float n = fmaf(h[c][i] * r1, w1[c][i], b1[c][i]);
+                x[c][i] = fmaf(g[c][i], n, a.alpha * x[c][i]);
+            }
+            round_as((XT*)nullptr, x[c]);
+            if (on[c] && row < a.rows) store8((XT*)a.xo + row * a.ldxo + col0 + 8 * TPR * c, x[c]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += on[c] ? x[c][i] : 0.f;
+        }
+        if (!a.rms) m2 = row_sum<TPR>(s, red) * invC;
+        s = 0.f;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { x[c][i] = on[c] ? x[c][i] - m2 : 0.f; s = fmaf(x[c][i], x[c][i], s); }
+        const float r2 = rsqrtf(row_sum<TPR>(s, red) * invC + a.eps);
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[c][i] = fmaf(x[c][i] * r2, w2[c][i], b2[c][i]);
+            if (on[c] && row < a.rows) store8(a.y + row * a.ldy + col0 + 8 * TPR * c, x[c]);
+        }
+        if (a.stats && row < a.rows && col0 == 0) *reinterpret_cast<f4_t*>(a.stats + 4 * row) = (f4_t){m1, r1, m2, r2};
     }
 }
 
 // partial row of one parameter: the RG row groups of the block are summed in LDS, in order
-template <int RG>
-__device__ __forceinline__ void flush8(const float* v, float* s, float* out, int C, int rg, int col, bool on) {
+template <int TPR, int NCH>
+__device__ __forceinline__ void flush8(const float (&v)[NCH][8], float* s, float* out, int C, const bool (&on)[NCH]) {
+    constexpr int RG = Blk<TPR>::RG;
+    const int rg = threadIdx.x / TPR, col0 = 8 * (threadIdx.x % TPR);
     if (RG > 1) {
         __syncthreads();
-        if (on) store8(s + rg * C + col, v);
+        if (on[0]) store8(s + rg * C + col0, v[0]);
         __syncthreads();
-        if (on && rg == 0) {
+        if (on[0] && rg == 0) {
             float t[8], u[8];
-            load8(s + col, t);
+            load8(s + col0, t);
 #pragma unroll
             for (int k = 1; k < RG; ++k) {
-                load8(s + k * C + col, u);
+                load8(s + k * C + col0, u);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) t[i] += u[i];
             }
-            store8(out + col, t);
+            store8(out + col0, t);
         }
-    } else if (on) store8(out + col, v);
+    } else {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+            if (on[c]) store8(out + col0 + 8 * TPR * c, v[c]);
+    }
 }
 
-template <typename XT, int WPR>
-__global__ void __launch_bounds__(WPR <= 4 ? 256 : 64 * WPR) norm_join_bwd_kernel(JP a) {
-    constexpr int NW = WPR <= 4 ? 4 : WPR, RG = NW / WPR;
-    __shared__ float red[32];
+// The rows of a block: `gpw` row groups (gate_kind 3; otherwise all rows are one group), or the piece `blockIdx % W` of one.  SOLO (at least RG groups to a
+// block): each of the RG row groups of threads takes whole gate groups and writes their gate gradients itself; otherwise the RG work on one
+// group together and meet in LDS at its end.
+template <typename XT, int TPR, int NCH, bool SOLO>
+__global__ void __launch_bounds__(Blk<TPR>::NT) norm_join_bwd_kernel(JP a) {
+    constexpr int RG = Blk<TPR>::RG, NW = Blk<TPR>::NT / 64;
+    static_assert(NCH == 1 || RG == 1, "flush8");
+    // 16 columns a thread leave no room for their weights and a row ahead beside the five sums: the weights come from L2 each time
+    constexpr bool HOLD = NCH == 1;
+    __shared__ float red[16];
     __shared__ __attribute__((aligned(16))) float sum[RG > 1 ? 2048 : 4];     // RG * C <= 2048
-    const int wave = threadIdx.x >> 6, rg = wave / WPR;
-    const int col = 8 * ((wave % WPR) * 64 + (threadIdx.x & 63));
-    const bool on = col < a.C;
+    const int rg = threadIdx.x / TPR, col0 = 8 * (threadIdx.x % TPR);
     const float invC = 1.0f / (float)a.C;
-    float w1[8] = {}, b1[8] = {}, w2[8] = {}, g[8];
+    float w1[HOLD ? NCH : 1][8], b1[HOLD ? NCH : 1][8], w2[HOLD ? NCH : 1][8], g[HOLD ? NCH : 1][8];
+    float aw1[NCH][8], ab1[NCH][8], aw2[NCH][8], ab2[NCH][8], ag[NCH][8];
+    bool on[NCH];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = 1.f;
-    if (on) {
-        load8(a.w1 + col, w1);
-        load8(a.w2 + col, w2);
-        if (a.b1) load8(a.b1 + col, b1);
-        if (a.gate_kind == 2) load8(a.gate + col, g);
-    }
-    if (a.gate_kind == 1) {
-        const float s = a.gate[0];
+    for (int c = 0; c < NCH; ++c) {
+        const int col = col0 + 8 * TPR * c;
+        on[c] = col < a.C;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = s;
+        for (int i = 0; i < 8; ++i) aw1[c][i] = ab1[c][i] = aw2[c][i] = ab2[c][i] = ag[c][i] = 0.f;
     }
-    float aw1[8] = {}, ab1[8] = {}, aw2[8] = {}, ab2[8] = {}, ag[8] = {};
+    const float gate0 = a.gate_kind == 1 ? a.gate[0] : 1.f;
+    auto set = [&](int c, int k, int64_t gr, bool fresh) {              // weights and gate of chunk c into slot k; fresh: the group's gate alone
+        const int col = col0 + 8 * TPR * c;
+        if (!fresh) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { w1[k][i] = b1[k][i] = w2[k][i] = 0.f; g[k][i] = gate0; }
+            if (on[c]) {
+                load8(a.w1 + col, w1[k]);
+                load8(a.w2 + col, w2[k]);
+                if (a.b1) load8(a.b1 + col, b1[k]);
+                if (a.gate_kind == 2) load8(a.gate + col, g[k]);
+            }
+        }
+        if (a.gate_kind == 3 && on[c] && gr < a.G) load8(a.gate + gr * a.C + col, g[k]);
+    };
+    if (HOLD) set(0, 0, a.G, false);
     const int64_t part = blockIdx.x % a.W, g0 = blockIdx.x / a.W * a.gpw;
     const int64_t g1 = g0 + a.gpw < a.G ? g0 + a.gpw : a.G;
-    for (int64_t gr = g0; gr < g1; ++gr) {
-        const int64_t first = gr * a.rpg + part * a.piece;
-        int64_t last = first + a.piece, gend = (gr + 1) * a.rpg;
-        gend = gend < a.rows ? gend : a.rows;
-        last = last < gend ? last : gend;
-        if (a.gate_kind == 3 && on) load8(a.gate + gr * a.C + col, g);
-        for (int64_t base = first; base < last; base += RG) {
-            const int64_t row = base + rg;
-            const bool in = row < last, ok = on && in;
-            float dy[8] = {}, t[8] = {}, z[8] = {}, h[8] = {};
-            f4_t st = {0.f, 0.f, 0.f, 0.f};
-            if (in) st = *reinterpret_cast<const f4_t*>(a.stats + 4 * row);
-            if (ok) {
-                load8(a.dy + row * a.lddy + col, dy);
-                load8((const XT*)a.xo + row * a.ldxo + col, z);
-                load8(a.h + row * a.ldh + col, h);
-                if (a.dxo) load8((const XT*)a.dxo + row * a.lddxo + col, t);
+    const int64_t turns = SOLO ? (g1 - g0 + RG - 1) / RG : g1 - g0;     // groups (of RG) in turn, `count` rows each: the same for every wave
+    const int64_t count = SOLO ? a.rpg : (a.piece + RG - 1) / RG;
+    auto row_of = [&](int64_t turn, int64_t i) -> int64_t {             // the row, or -1
+        const int64_t gr = SOLO ? g0 + turn * RG + rg : g0 + turn;
+        const int64_t in = SOLO ? i : part * a.piece + i * RG + rg;     // inside the group
+        const int64_t row = gr * a.rpg + in;
+        const bool ok = gr < g1 && in < a.rpg && (SOLO || i * RG + rg < a.piece) && row < a.rows;
+        return ok ? row : -1;
+    };
+    Raw8<bf16_t> rdy[NCH], rh[NCH];
+    Raw8<XT> rz[NCH], rt[NCH];
+    f4_t rs;
+    auto fetch = [&](int64_t row) {
+        rs = (f4_t){0.f, 0.f, 0.f, 0.f};
+        if (row >= 0) rs = *reinterpret_cast<const f4_t*>(a.stats + 4 * row);
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const int col = col0 + 8 * TPR * c;
+            none(rdy[c]);
+            none(rh[c]);
+            none(rz[c]);
+            none(rt[c]);
+            if (on[c] && row >= 0) {
+                ask(rdy[c], a.dy + row * a.lddy + col);
+                ask(rz[c], (const XT*)a.xo + row * a.ldxo + col);
+                ask(rh[c], a.h + row * a.ldh + col);
+                if (a.dxo) ask(rt[c], (const XT*)a.dxo + row * a.lddxo + col);
             }
+        }
+    };
+    if (HOLD && turns > 0 && count > 0) fetch(row_of(0, 0));
+    for (int64_t turn = 0; turn < turns; ++turn) {
+        const int64_t gr = SOLO ? g0 + turn * RG + rg : g0 + turn;
+        if (HOLD && gr < g1) set(0, 0, gr, true);
+        for (int64_t i = 0; i < count; ++i) {
+            const int64_t row = row_of(turn, i);
+            float dy[NCH][8], t[NCH][8], z[NCH][8], h[NCH][8];
+            if (!HOLD) fetch(row);
+            const f4_t st = rs;
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) { open8(rdy[c], dy[c]); open8(rt[c], t[c]); open8(rz[c], z[c]); open8(rh[c], h[c]); }
+            if (HOLD) fetch(i + 1 < count ? row_of(turn, i + 1) : (turn + 1 < turns ? row_of(turn + 1, 0) : -1));
             float c1 = 0.f, c2 = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                z[i] = ok ? (z[i] - st[2]) * st[3] : 0.f;               // second norm's normalised row
-                aw2[i] = fmaf(dy[i], z[i], aw2[i]);
-                ab2[i] += dy[i];
-                dy[i] *= w2[i];
-                c1 += dy[i];
-                c2 = fmaf(dy[i], z[i], c2);
+            for (int c = 0; c < NCH; ++c) {
+                const bool ok = on[c] && row >= 0;
+                const int u = HOLD ? c : 0;
+                if (!HOLD) set(c, 0, gr, false);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    z[c][k] = ok ? (z[c][k] - st[2]) * st[3] : 0.f;     // second norm's normalised row
+                    aw2[c][k] = fmaf(dy[c][k], z[c][k], aw2[c][k]);
+                    ab2[c][k] += dy[c][k];
+                    dy[c][k] *= w2[u][k];
+                    c1 += dy[c][k];
+                    c2 = fmaf(dy[c][k], z[c][k], c2);
+                }
             }
-            row_sum2<WPR>(c1, c2, red, wave);
+            row_sum2<TPR>(c1, c2, red);
             c1 = a.rms ? 0.f : c1 * invC;
             c2 *= invC;
             float e1 = 0.f, e2 = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                t[i] = fmaf(st[3], dy[i] - fmaf(z[i], c2, c1), t[i]);   // gradient of x'
-                h[i] = ok ? (h[i] - st[0]) * st[1] : 0.f;
-                t[i] = ok ? t[i] : 0.f;
-                ag[i] = fmaf(t[i], fmaf(h[i], w1[i], b1[i]), ag[i]);
-                const float dn = t[i] * g[i];
-                aw1[i] = fmaf(dn, h[i], aw1[i]);
-                ab1[i] += dn;
-                dy[i] = dn * w1[i];
-                e1 += dy[i];
-                e2 = fmaf(dy[i], h[i], e2);
-                t[i] *= a.alpha;
+            for (int c = 0; c < NCH; ++c) {
+                const bool ok = on[c] && row >= 0;
+                const int u = HOLD ? c : 0;
+                if (!HOLD) set(c, 0, gr, false);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    t[c][k] = fmaf(st[3], dy[c][k] - fmaf(z[c][k], c2, c1), t[c][k]);     // gradient of x'
+                    h[c][k] = ok ? (h[c][k] - st[0]) * st[1] : 0.f;
+                    t[c][k] = ok ? t[c][k] : 0.f;
+                    ag[c][k] = fmaf(t[c][k], fmaf(h[c][k], w1[u][k], b1[u][k]), ag[c][k]);
+                    const float dn = t[c][k] * g[u][k];
+                    aw1[c][k] = fmaf(dn, h[c][k], aw1[c][k]);
+                    ab1[c][k] += dn;
+                    dy[c][k] = dn * w1[u][k];
+                    e1 += dy[c][k];
+                    e2 = fmaf(dy[c][k], h[c][k], e2);
+                    t[c][k] *= a.alpha;
+                }
+                if (ok) store8((XT*)a.dx + row * a.lddx + col0 + 8 * TPR * c, t[c]);
             }
-            if (ok) store8((XT*)a.dx + row * a.lddx + col, t);
-            row_sum2<WPR>(e1, e2, red, wave);
+            row_sum2<TPR>(e1, e2, red);
             e1 = a.rms ? 0.f : e1 * invC;
             e2 *= invC;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[i] = st[1] * (dy[i] - fmaf(h[i], e2, e1));
-            if (ok) store8(a.dh + row * a.lddh + col, h);
+            for (int c = 0; c < NCH; ++c) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) h[c][k] = st[1] * (dy[c][k] - fmaf(h[c][k], e2, e1));
+                if (on[c] && row >= 0) store8(a.dh + row * a.lddh + col0 + 8 * TPR * c, h[c]);
+            }
         }
         if (a.gate_kind == 3 && a.gpart) {
-            flush8<RG>(ag, sum, a.gpart + (gr * a.W + part) * a.C, a.C, rg, col, on);
+            if (SOLO) {
+                if (gr < g1) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ag[i] = 0.f;
+                    for (int c = 0; c < NCH; ++c)
+                        if (on[c]) store8(a.gpart + gr * a.C + col0 + 8 * TPR * c, ag[c]);
+                }
+            } else flush8<TPR, NCH>(ag, sum, a.gpart + (gr * a.W + part) * a.C, a.C, on);
+#pragma unroll
+            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) ag[c][k] = 0.f;
         }
     }
     if (a.part) {
         float* out = a.part + (int64_t)blockIdx.x * a.pcols;
-        flush8<RG>(aw1, sum, out, a.C, rg, col, on); out += a.C;
-        if (a.b1) { flush8<RG>(ab1, sum, out, a.C, rg, col, on); out += a.C; }
-        flush8<RG>(aw2, sum, out, a.C, rg, col, on); out += a.C;
-        if (a.b2) { flush8<RG>(ab2, sum, out, a.C, rg, col, on); out += a.C; }
-        if (a.gate_kind == 2) flush8<RG>(ag, sum, out, a.C, rg, col, on);
+        flush8<TPR, NCH>(aw1, sum, out, a.C, on); out += a.C;
+        if (a.b1) { flush8<TPR, NCH>(ab1, sum, out, a.C, on); out += a.C; }
+        flush8<TPR, NCH>(aw2, sum, out, a.C, on); out += a.C;
+        if (a.b2) { flush8<TPR, NCH>(ab2, sum, out, a.C, on); out += a.C; }
+        if (a.gate_kind == 2) flush8<TPR, NCH>(ag, sum, out, a.C, on);
         if (a.gate_kind == 1) {
             float v = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v += ag[i];
+            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v += ag[c][k];
             v = wave_sum<64>(v);
             __syncthreads();
-            if ((threadIdx.x & 63) == 0) red[wave] = v;
+            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
             __syncthreads();
             if (threadIdx.x == 0) {
                 float s = 0.f;
@@ -328,35 +440,35 @@ int check(const char* who, const stg_norm_join_args* a) {
 JP make(const stg_norm_join_args* a) {
     JP p{};
     p.x = a->x; p.ldx = a->ldx; p.h = (const bf16_t*)a->h; p.ldh = a->ldh;
-    p.gate = a->gate; p.gate_kind = a->gate_kind; p.rpg = a->gate_kind == 3 ? a->rows_per_group : (a->rows > 0 ? a->rows : 1);
+    p.gate = a->gate; p.gate_kind = a->gate_kind; p.rpg = a->rows > 0 ? a->rows : 1;
+    if (a->gate_kind == 3 && a->rows_per_group < p.rpg) p.rpg = a->rows_per_group;
     p.w1 = a->w1; p.b1 = a->b1; p.w2 = a->w2; p.b2 = a->b2; p.alpha = a->alpha; p.eps = a->eps;
     p.xo = a->xo; p.ldxo = a->ldxo; p.y = (bf16_t*)a->y; p.ldy = a->ldy; p.stats = a->stats;
     p.rows = a->rows; p.C = a->C; p.rms = a->rms != 0;
     return p;
 }
 
-int waves_per_row(int C) { return C <= 512 ? 1 : C <= 1024 ? 2 : C <= 2048 ? 4 : C <= 4096 ? 8 : 16; }
+// threads of a row: 8 columns each up to 4096, 16 beyond (with 1024 threads a row the backward's 170 registers spilled: 600 us instead of 225 us
+// at 8192 x 5120)
+int threads_per_row(int C) { return C <= 128 ? 16 : C <= 256 ? 32 : C <= 512 ? 64 : C <= 1024 ? 128 : C <= 2048 ? 256 : 512; }
+int rows_in_flight(int C) { const int t = threads_per_row(C); return t <= 256 ? 256 / t : 1; }
 
-// How the backward's blocks share the rows.  Few rows: one block per compute unit, down to one row for each of its wave groups (latency).  Many: at
-// least 8 rows for each (a block's partial row costs as much traffic as a few rows) and at most 1024 blocks.  Groups (gate_kind 3) longer than
-// a block's share are split W ways, shorter ones go several to a block.
+// How the backward's blocks share the rows: as many blocks as stay resident together (two of 256 threads or one of 512 per compute unit at 200
+// registers; a few more would cost a second round), since every further block leaves another partial row of up to 5 C floats (8192 x 4096, bf16 stream:
+// 130 us with 1024 blocks, 115 us with 256); fewer when a block's row groups would be left without a row.  More gate groups than blocks: several
+// groups to a block; fewer: a group is split W ways.
 void plan_bwd(JP& p) {
-    const int wpr = waves_per_row(p.C), rgn = wpr <= 4 ? 4 / wpr : 1;
-    int64_t share = (p.rows + 255) / 256;
-    share = share < 8 * rgn ? share : 8 * rgn;
-    const int64_t most = (p.rows + 1023) / 1024;
-    share = share > most ? share : most;
-    share = share > rgn ? share : rgn;
-    share = (share + rgn - 1) / rgn * rgn;
+    const int64_t rgn = rows_in_flight(p.C), target = threads_per_row(p.C) <= 256 ? 512 : 256;
     p.G = (p.rows + p.rpg - 1) / p.rpg;
-    if (p.rpg > share) {
-        p.W = (int)((p.rpg + share - 1) / share);
+    p.W = 1;
+    p.gpw = 1;
+    p.piece = p.rpg;
+    if (p.G >= target) p.gpw = (p.G + target - 1) / target;
+    else if (p.G > 0) {
+        const int64_t most = (p.rpg + rgn - 1) / rgn, w = target / p.G;
+        p.W = (int)(w < most ? w : most);
         p.piece = ((p.rpg + p.W - 1) / p.W + rgn - 1) / rgn * rgn;
-        p.gpw = 1;
-    } else {
-        p.W = 1;
-        p.piece = p.rpg;
-        p.gpw = share / p.rpg;
+        p.W = (int)((p.rpg + p.piece - 1) / p.piece);
     }
 }
 int64_t blocks_of(const JP& p) { return (p.G + p.gpw - 1) / p.gpw * p.W; }
@@ -366,32 +478,33 @@ int64_t part_cols(const JP& p) {
 // the partial rows start 16-byte aligned
 int64_t part_pitch(const JP& p) { return (part_cols(p) + 3) / 4 * 4; }
 
+bool solo(const JP& p) { return p.W == 1 && p.gate_kind == 3 && p.gpw >= rows_in_flight(p.C); }
+
+#define BY_WIDTH(CALL)                                                          \
+    switch (threads_per_row(p.C)) {                                             \
+        case 16: { constexpr int T = 16, N = 1; CALL; break; }                  \
+        case 32: { constexpr int T = 32, N = 1; CALL; break; }                  \
+        case 64: { constexpr int T = 64, N = 1; CALL; break; }                  \
+        case 128: { constexpr int T = 128, N = 1; CALL; break; }                \
+        case 256: { constexpr int T = 256, N = 1; CALL; break; }                \
+        default:                                                                \
+            if (p.C <= 4096) { constexpr int T = 512, N = 1; CALL; }            \
+            else { constexpr int T = 512, N = 2; CALL; }                        \
+    }
+
 template <typename XT>
 int launch_fwd(const JP& p, hipStream_t st) {
-    const int wpr = waves_per_row(p.C), rgn = wpr <= 4 ? 4 / wpr : 1;
-    int64_t n = (p.rows + rgn - 1) / rgn;
+    int64_t n = (p.rows + rows_in_flight(p.C) - 1) / rows_in_flight(p.C);
     n = n < 2048 ? n : 2048;
-    const dim3 g((unsigned)n);
-    switch (wpr) {
-        case 1: norm_join_fwd_kernel<XT, 1><<<g, 256, 0, st>>>(p); break;
-        case 2: norm_join_fwd_kernel<XT, 2><<<g, 256, 0, st>>>(p); break;
-        case 4: norm_join_fwd_kernel<XT, 4><<<g, 256, 0, st>>>(p); break;
-        case 8: norm_join_fwd_kernel<XT, 8><<<g, 512, 0, st>>>(p); break;
-        default: norm_join_fwd_kernel<XT, 16><<<g, 1024, 0, st>>>(p); break;
-    }
+    BY_WIDTH((norm_join_fwd_kernel<XT, T, N><<<dim3((unsigned)n), Blk<T>::NT, 0, st>>>(p)));
     STG_LAUNCH_CHECK();
     return 0;
 }
 template <typename XT>
 int launch_bwd(const JP& p, hipStream_t st) {
     const dim3 g((unsigned)blocks_of(p));
-    switch (waves_per_row(p.C)) {
-        case 1: norm_join_bwd_kernel<XT, 1><<<g, 256, 0, st>>>(p); break;
-        case 2: norm_join_bwd_kernel<XT, 2><<<g, 256, 0, st>>>(p); break;
-        case 4: norm_join_bwd_kernel<XT, 4><<<g, 256, 0, st>>>(p); break;
-        case 8: norm_join_bwd_kernel<XT, 8><<<g, 512, 0, st>>>(p); break;
-        default: norm_join_bwd_kernel<XT, 16><<<g, 1024, 0, st>>>(p); break;
-    }
+    if (solo(p)) { BY_WIDTH((norm_join_bwd_kernel<XT, T, N, true><<<g, Blk<T>::NT, 0, st>>>(p))); }
+    else { BY_WIDTH((norm_join_bwd_kernel<XT, T, N, false><<<g, Blk<T>::NT, 0, st>>>(p))); }
     STG_LAUNCH_CHECK();
     return 0;
 }

@@ -2363,6 +2363,7 @@ def _norm_join_args(x, x_new, h, y, gate, weights, kind, alpha, eps, rows_per_gr
             gk, rpg = 3, int(rows_per_group)
             if tuple(sh) != (-(-R // rpg), Cw):
                 raise RuntimeError(f"gate: expected [{-(-R // rpg)}, {Cw}], got {tuple(sh)}")
+            rpg = min(rpg, max(R, 1))
         elif len(sh) == 0 or tuple(sh) == (1,):
             gk = 1
         elif tuple(sh) == (Cw,):
