@@ -427,7 +427,7 @@ int check(const char* who, const stg_norm_join_args* a) {
     STG_CHECK(a != nullptr, -1, "%s: null arguments", who);
     STG_CHECK(a->x_dtype == STG_F32 || a->x_dtype == STG_BF16, -2, "%s: the stream is fp32 or bf16", who);
     STG_CHECK(a->rows >= 0 && a->C > 0 && a->C % 8 == 0 && a->C <= 8192, -2, "%s: rows=%lld, width %d (a multiple of 8 up to 8192)", who, (long long)a->rows, a->C);
-    STG_CHECK(a->gate_kind >= 0 && a->gate_kind <= 3 && (a->gate_kind == 0) == (a->gate == nullptr), -2, "%s: gate kind %d (0..3, 0 without a gate)", who, a->gate_kind);
+    STG_CHECK(a->gate_kind >= 0 && a->gate_kind <= 3 && ((a->gate_kind == 0) == (a->gate == nullptr) || (a->gate_kind == 3 && a->rows == 0)), -2, "%s: gate kind %d (0..3, 0 without a gate)", who, a->gate_kind);
     STG_CHECK(a->gate_kind != 3 || a->rows_per_group > 0, -2, "%s: a gate by group needs rows_per_group > 0", who);
     STG_CHECK(a->w1 && a->w2 && (a->rows == 0 || (a->h && a->xo)), -1, "%s: null tensor", who);
     STG_CHECK(a->ldh >= a->C && a->ldxo >= a->C && a->ldh % 8 == 0 && a->ldxo % 8 == 0, -3, "%s: leading dimensions must be multiples of 8 and >= the width", who);

@@ -1315,12 +1315,19 @@ int64_t lds_band(int D) { return (int64_t)14 * 32 * (D + 8) * 2 + 320 * 4; }
 int64_t lds_dkv(int D, int far) { return (int64_t)2 * (2 * 64 * (D + 8) + 512) * 2 + (2 * (far + PAD) + 1) * 4; }
 int64_t lds_dec(int D, int NB) { return (int64_t)8 * 32 * (D + 8) * 2 + (int64_t)NB * 32 * 4; }
 
-int grid_tiles(int max_n, int64_t T, int rows) {
+int64_t cover(int max_n, int64_t T, int rows) {
     int64_t n = max_n > 0 ? max_n : 1;
     n = n < T ? n : (T > 0 ? T : 1);
-    const int64_t t = (n + rows - 1) / rows;
-    return (int)(t < 1 ? 1 : t);
+    return (n + rows - 1) / rows;
 }
+// Blocks per (sequence, head): one per 128-row tile of the longest sequence, but no more than 2^18 over all of them (a hundred rounds on
+// the chip); beyond, a block strides over several tiles.  Many short sequences without a length hint would otherwise launch tiles for sequences
+// as long as the whole batch (1000 of 14 .. 100 rows, 16 heads: 7 million empty blocks).
+int grid_tiles(int max_n, int64_t T, int64_t heads) {
+    const int64_t t = cover(max_n, T, 128), most = ((int64_t)1 << 18) / (heads > 0 ? heads : 1);
+    return (int)(t <= most ? t : (most < 1 ? 1 : most));
+}
+constexpr int64_t MAX_BLOCKS = (1 << 24) - 1;     // of 256 threads: a launch's threads are counted in 32 bits
 
 template <int D>
 int launch_fwd(const RP& p0, int max_q, hipStream_t st) {
@@ -1328,9 +1335,9 @@ int launch_fwd(const RP& p0, int max_q, hipStream_t st) {
     auto k = relattn_fwd_kernel<D, 4>;
     STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_fwd: cannot reserve LDS");
     RP p = p0;
-    p.tiles = grid_tiles(max_q, p.Tq, 128);
+    p.tiles = grid_tiles(max_q, p.Tq, (int64_t)p.S * p.H);
     const int64_t blocks = (int64_t)p.tiles * p.H * (p.S + (p.zero_tail ? 1 : 0));
-    STG_CHECK(blocks <= INT32_MAX, -2, "relattn: too many blocks (max_q / max_k larger than the sequences?)");
+    STG_CHECK(blocks <= MAX_BLOCKS, -2, "relattn: %d sequences of %d heads are more than 2^24 blocks", p.S, p.H);
     if (blocks == 0) return 0;
     k<<<dim3((unsigned)blocks), 256, lds_fwd(D, p.far), st>>>(p);
     STG_LAUNCH_CHECK();
@@ -1342,9 +1349,9 @@ int launch_dq(const RP& p0, int max_q, hipStream_t st) {
     auto k = relattn_dq_kernel<D, 4, TAB>;
     STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_bwd: cannot reserve LDS");
     RP p = p0;
-    p.tiles = grid_tiles(max_q, p.Tq, 128);
+    p.tiles = grid_tiles(max_q, p.Tq, (int64_t)p.S * p.H);
     const int64_t blocks = (int64_t)p.tiles * p.H * (p.S + (p.zero_tail ? 1 : 0));
-    STG_CHECK(blocks <= INT32_MAX, -2, "relattn: too many blocks (max_q / max_k larger than the sequences?)");
+    STG_CHECK(blocks <= MAX_BLOCKS, -2, "relattn: %d sequences of %d heads are more than 2^24 blocks", p.S, p.H);
     if (blocks == 0) return 0;
     k<<<dim3((unsigned)blocks), 256, lds_fwd(D, p.far), st>>>(p);
     STG_LAUNCH_CHECK();
@@ -1366,9 +1373,9 @@ int launch_dkv(const RP& p0, int max_k, hipStream_t st) {
     auto k = relattn_dkv_kernel<D, 4>;
     STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_bwd: cannot reserve LDS");
     RP p = p0;
-    p.tiles = grid_tiles(max_k, p.Tk, 128);
+    p.tiles = grid_tiles(max_k, p.Tk, (int64_t)p.S * p.Hkv);
     const int64_t blocks = (int64_t)p.tiles * p.Hkv * (p.S + (p.zero_tail ? 1 : 0));
-    STG_CHECK(blocks <= INT32_MAX, -2, "relattn: too many blocks (max_q / max_k larger than the sequences?)");
+    STG_CHECK(blocks <= MAX_BLOCKS, -2, "relattn: %d sequences of %d heads are more than 2^24 blocks", p.S, p.H);
     if (blocks == 0) return 0;
     k<<<dim3((unsigned)blocks), 256, lds_dkv(D, p.far), st>>>(p);
     STG_LAUNCH_CHECK();
@@ -1433,7 +1440,7 @@ extern "C" int stg_relattn_fwd(const stg_relattn_args* a, void* stream) {
 static void band_grid(const stg_relattn_args* a, int& tgroups, int& chunk, int& blocks) {
     const int nt = ((a->causal ? a->far + 62 + 31 : 2 * a->far + 124) >> 5) + 2;
     tgroups = (nt + 3) / 4;
-    const int64_t tiles = grid_tiles(a->max_q, a->Tq, 32), want = 2048 / ((int64_t)tgroups * a->H * (a->S > 0 ? a->S : 1)) + 1;
+    const int64_t tiles = cover(a->max_q, a->Tq, 32), want = 2048 / ((int64_t)tgroups * a->H * (a->S > 0 ? a->S : 1)) + 1;
     int64_t c = (tiles + want - 1) / want;
     c = c < 16 ? 16 : c;
     chunk = (int)c;
@@ -1446,7 +1453,7 @@ extern "C" int64_t stg_relattn_bwd_ws_floats(const stg_relattn_args* a, int want
     if (want_table) {
         int tg, chunk, blocks;
         band_grid(a, tg, chunk, blocks);
-        n += (int64_t)a->S * a->H * ((int64_t)grid_tiles(a->max_q, a->Tq, 128) * 2 + (int64_t)blocks * a->num_buckets);
+        n += (int64_t)a->S * a->H * ((int64_t)grid_tiles(a->max_q, a->Tq, (int64_t)a->S * a->H) * 2 + (int64_t)blocks * a->num_buckets);
     }
     return n > 0 ? n : 1;
 }
@@ -1468,7 +1475,7 @@ extern "C" int stg_relattn_bwd(const stg_relattn_args* a, const void* dO, int64_
     p.dK = (bf16_t*)dK; p.lddk = lddk; p.dV = (bf16_t*)dV; p.lddv = lddv;
     p.delta = ws;
     // table gradient: the dQ kernel's rows (two sums each), then the band's rows
-    const int nbehind = grid_tiles(a->max_q, a->Tq, 128) * a->S;
+    const int nbehind = grid_tiles(a->max_q, a->Tq, (int64_t)a->S * a->H) * a->S;
     float* behind = ws + (int64_t)a->H * a->Tq;
     float* band = behind + (int64_t)nbehind * a->H * 2;
     int tgroups = 0, chunk = 0, blocks = 0;
@@ -1497,7 +1504,7 @@ extern "C" int stg_relattn_decode(const stg_relattn_decode_args* a, float* ws, i
     STG_CHECK(a != nullptr, -1, "stg_relattn_decode: null arguments");
     STG_CHECK(a->S >= 0 && a->S <= 65535 && a->cap >= 0 && a->cap <= INT32_MAX - 1024, -2, "stg_relattn_decode: S=%d (<= 65535), cap=%d", a->S, a->cap);
     STG_CHECK(a->D == 32 || a->D == 64 || a->D == 96 || a->D == 128, -2, "stg_relattn_decode: head dim %d (32, 64, 96 or 128)", a->D);
-    STG_CHECK(a->H > 0 && a->H <= 32768 && (int64_t)a->H * a->S <= INT32_MAX && a->Hkv > 0 && a->H % a->Hkv == 0, -2, "stg_relattn_decode: %d heads over %d key / value heads", a->H, a->Hkv);
+    STG_CHECK(a->H > 0 && a->H <= 32768 && (int64_t)a->H * a->S <= MAX_BLOCKS && a->Hkv > 0 && a->H % a->Hkv == 0, -2, "stg_relattn_decode: %d heads over %d key / value heads", a->H, a->Hkv);
     STG_CHECK(a->Q && a->O && a->lens && (a->cap == 0 || (a->K && a->V)), -1, "stg_relattn_decode: null tensor");
     const int64_t hd = (int64_t)a->H * a->D, kd = (int64_t)a->Hkv * a->D;
     STG_CHECK(a->ldq >= hd && a->ldo >= hd && a->ldk >= kd && a->ldv >= kd && a->ldq % 8 == 0 && a->ldk % 8 == 0 && a->ldv % 8 == 0 && a->bsk % 8 == 0 &&

@@ -10,6 +10,7 @@ With u = 2^-8 (half a bf16 step, relative) and e = the relative error of a proba
 e: the score is a sum of D products in fp32 plus the bias, so its error is at most (D + 8) 2^-24 A with A = scale sum |q||k| + |bias| + |lse|, the
 exponential and the row sum of n terms add (n + 8) 2^-24.
 """
+import functools
 import math
 
 import torch
@@ -18,6 +19,7 @@ U = 2.0 ** -8
 E32 = 2.0 ** -24
 
 
+@functools.lru_cache(None)
 def bucket(distance, buckets, far, causal):
     half = buckets if causal else buckets // 2
     first = half // 2

@@ -30,6 +30,16 @@ CASES = [
     (2500, 192, "layer", F32, "group", 7, True, True, 1.0, True),
     (5000, 96, "rms", BF16, "group", 2048, False, False, 1.0, True),
     (3, 8184, "layer", F32, "channel", None, True, True, -1.0, True),
+    (1, 8, "rms", BF16, "group", 5, True, True, 1.0, True),              # a group larger than the batch
+    (77, 16, "layer", F32, "channel", None, True, False, 1.0, True),
+    (4099, 128, "layer", F32, "group", 1, True, True, 1.0, True),        # a group to every row; more groups than blocks
+    (9001, 136, "rms", BF16, "group", 4, False, True, 1.0, True),
+    (6000, 256, "layer", BF16, "group", 3, True, False, 0.5, True),
+    (2049, 512, "rms", F32, "group", 2, True, True, 1.0, False),
+    (700, 264, "layer", F32, "one", None, False, False, 1.0, True),
+    (1300, 1024, "rms", BF16, "none", None, True, True, 1.0, True),
+    (520, 4096, "layer", BF16, "channel", None, True, True, 1.0, True),
+    (600, 5120, "rms", F32, "group", 2, False, False, 1.0, True),
 ]
 
 
@@ -181,3 +191,100 @@ def test_block_of_attention_and_join(stg, gpu):
     assert float((y.double() - yr).norm() / yr.norm()) < tol and float((xn.double() - xr).norm() / xr.norm()) < tol
     for k in P:
         assert float((P[k].grad.double() - Q[k].grad).norm() / Q[k].grad.norm()) < tol, k
+
+
+@pytest.mark.parametrize("gate", ["none", "one", "channel", "group"])
+def test_no_rows(stg, gpu, gate):
+    from stgcma import ops_seq
+    C = 64
+    t = _make(gpu, 0, C, "layer", F32, gate, 4 if gate == "group" else None, True, True, 5)
+    leaf = {n: v.detach().requires_grad_(True) for n, v in t.items() if v is not None and n not in ("dy", "dxn")}
+    xn, y = ops_seq.norm_join(*[leaf.get(n) for n in ("x", "h", "gate", "w1", "b1", "w2", "b2")], rows_per_group=4 if gate == "group" else None)
+    assert xn.shape == y.shape == (0, C)
+    for v, g in zip(leaf.values(), torch.autograd.grad([xn, y], list(leaf.values()), [t["dxn"], t["dy"]])):
+        assert g.shape == v.shape and bool((g == 0).all())
+
+
+def test_offsets_beyond_32_bits(stg, gpu):
+    """Rows 2^23 elements apart (the last of 300 stands 2.5 * 10^9 elements behind the first) equal the dense call."""
+    from stgcma import kernels as K
+    rows, C = 300, 512
+    t = _make(gpu, rows, C, "layer", BF16, "channel", None, True, True, 6)
+    big = torch.empty(rows, 1 << 23, dtype=BF16, device=gpu)
+    wide = {}
+    for i, n in enumerate(("x", "h", "dy", "dxn")):
+        wide[n] = big[:, 1024 * i:1024 * i + C]
+        wide[n].copy_(t[n])
+    w = [t[n] for n in ("gate", "w1", "b1", "w2", "b2")]
+    out = []
+    for s in (t, wide):
+        xn, y, st = K.norm_join_fwd(s["x"], s["h"], *w)
+        g = K.norm_join_bwd(xn, s["h"], *w, st, s["dy"], s["dxn"])
+        out.append([xn, y, st] + list(g.values()))
+    wide["x"].copy_(xn)                                        # the stored stream in rows as far apart
+    out.append(out[0][:3] + list(K.norm_join_bwd(wide["x"], wide["h"], *w, st, wide["dy"], wide["dxn"]).values()))
+    for other in out[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(out[0], other))
+
+
+def test_autograd_corners(stg, gpu):
+    """Saved tensors that hooks move and pack densely, single wanted gradients, only one of the two outputs used, strided incoming gradients, no second
+    derivative."""
+    from stgcma import ops_seq
+    t = _make(gpu, 90, 96, "layer", F32, "group", 40, True, True, 12)
+    names = ["x", "h", "gate", "w1", "b1", "w2", "b2"]
+    run = lambda leaf: ops_seq.norm_join(*leaf, rows_per_group=40)
+    leaf = [t[n].detach().requires_grad_(True) for n in names]
+    want = torch.autograd.grad(run(leaf), leaf, [t["dxn"], t["dy"]])
+    with torch.autograd.graph.saved_tensors_hooks(lambda a: a.cpu().contiguous(), lambda a: a.to(gpu)):
+        out = run(leaf)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(out, leaf, [t["dxn"], t["dy"]])))
+    turned = [t[n].t().contiguous().t() for n in ("dxn", "dy")]
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(run(leaf), leaf, turned)))
+    for i in range(7):
+        one = [t[n].detach().requires_grad_(i == j) for j, n in enumerate(names)]
+        got, = torch.autograd.grad(run(one), [one[i]], [t["dxn"], t["dy"]])
+        assert torch.equal(got, want[i]), names[i]
+    ref = R.norm_join(*[t[n] for n in names], "layer", 1.0, 1e-5, 40, torch.zeros_like(t["dy"]), t["dxn"])
+    xn, y = run(leaf)
+    got = dict(zip(names, torch.autograd.grad(xn, leaf, t["dxn"], allow_unused=True)))       # the second norm's output unused
+    k32 = (96 + 16) * E32
+    _close(got["x"], ref["dx"], "dx", 2 * E32, k32 * ref["dx"].abs().amax(1, keepdim=True) * 4)
+    assert bool((got["w2"] == 0).all()) and bool((got["b2"] == 0).all())
+    out = run(leaf)
+    (dx,) = torch.autograd.grad(out, leaf[:1], [t["dxn"], t["dy"]], create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(run(leaf), out))
+    scalar = torch.tensor(0.7, device=gpu, requires_grad=True)  # a gate without dimensions
+    one = torch.tensor([0.7], device=gpu, requires_grad=True)
+    g0, g1 = (torch.autograd.grad(ops_seq.norm_join(*[t[n] for n in names[:2]], g, *[t[n] for n in names[3:]]), [g], [t["dxn"], t["dy"]])[0] for g in (scalar, one))
+    assert g0.shape == () and g1.shape == (1,) and torch.equal(g0, g1[0])
+
+
+def test_refusals_on_the_gpu(stg, gpu):
+    from stgcma import kernels as K
+    t = _make(gpu, 20, 64, "layer", F32, "channel", None, True, True, 3)
+    a = [t[n] for n in ("x", "h", "gate", "w1", "b1", "w2", "b2")]
+    xn, y, st = K.norm_join_fwd(*a)
+    off = torch.zeros(65, device=gpu)[1:]
+
+    def with_(**kw):
+        b = dict(zip(("x", "h", "gate", "w1", "b1", "w2", "b2"), a))
+        b.update(kw)
+        return list(b.values())
+    for bad in (with_(x=t["x"].half()), with_(h=t["h"].float()), with_(h=t["h"][:-1]), with_(h=t["h"][:, :56]), with_(x=t["x"].t().contiguous().t()), with_(x=t["x"][:, 1:]),
+                with_(w1=None), with_(w2=None), with_(w1=off), with_(w1=t["w1"].to(BF16)), with_(b1=t["b1"][:56]), with_(w2=t["w2"].cpu()), with_(gate=t["gate"][:8]),
+                with_(gate=t["gate"].to(BF16)), with_(gate=torch.ones(20, 64, device=gpu)), with_(gate=torch.ones(1, device="cpu")), with_(x=t["x"][0]),
+                with_(x=t["x"][:, :60].contiguous(), h=t["h"][:, :60].contiguous())):
+        with pytest.raises(RuntimeError):
+            K.norm_join_fwd(*bad)
+    for kw in (dict(kind="batch"), dict(rows_per_group=0, kind="none")):
+        with pytest.raises(RuntimeError):
+            K.norm_join_fwd(*a, **kw)
+    with pytest.raises(RuntimeError):
+        K.norm_join_fwd(*with_(gate=torch.ones(5, 64, device=gpu)), rows_per_group=3)
+    for st_, dy, dxn in ((st, t["dy"].float(), None), (st[:-1], t["dy"], None), (None, t["dy"], None), (st, t["dy"], t["dxn"].to(BF16)), (st, t["dy"][:-1], None)):
+        with pytest.raises(RuntimeError):
+            K.norm_join_bwd(xn, *a[1:], st_, dy, dxn)

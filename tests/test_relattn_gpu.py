@@ -336,3 +336,182 @@ def test_decode_capture(stg, gpu):
         torch.cuda.synchronize()
         got = out.clone()
         assert torch.equal(got, K.relattn_decode(geom, q, kc, vc, table, lens))
+
+
+def _all(K, geom, q, k, v, table, cu_q, cu_k, do, **kw):
+    """Forward and every gradient through the direct calls."""
+    o, lse = K.relattn_fwd(geom, q, k, v, table, cu_q, cu_k, **kw)
+    return (o, lse) + K.relattn_bwd(geom, q, k, v, table, cu_q, cu_k, o, lse, do, **kw)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_empty_tensors(stg, gpu, causal):
+    from stgcma import kernels as K
+    H, Hkv, D = 4, 2, 64
+    geom = K.RelGeom(H, D, kv_heads=Hkv, causal=causal, device=gpu)
+    table = torch.randn(32, H, device=gpu)
+    e = lambda n, h: torch.randn(n, h * D, device=gpu).to(BF16)
+    for tq, tk, offs_q, offs_k in ((0, 0, [0, 0], None), (5, 5, [0], None), (4, 0, [0, 4], [0, 0]), (0, 6, [0, 0], [0, 6]), (0, 0, [0], None)):
+        cu_q = torch.tensor(offs_q, dtype=torch.int32, device=gpu)
+        cu_k = None if offs_k is None else torch.tensor(offs_k, dtype=torch.int32, device=gpu)
+        got = _all(K, geom, e(tq, H), e(tk, Hkv), e(tk, Hkv), table, cu_q, cu_k, e(tq, H))
+        assert [tuple(t.shape) for t in got] == [(tq, H * D), (H, tq), (tq, H * D), (tk, Hkv * D), (tk, Hkv * D), (32, H)]
+        assert all(bool((t == 0).all()) for i, t in enumerate(got) if i != 1) and bool((got[1] == -float("inf")).all())
+    none = K.relattn_decode(geom, e(3, H), e(3, Hkv).view(3, 1, -1)[:, :0], e(3, Hkv).view(3, 1, -1)[:, :0], table, torch.ones(3, dtype=torch.int32, device=gpu))
+    assert bool((none == 0).all())
+    assert K.relattn_decode(geom, e(0, H), e(0, Hkv).view(0, 1, Hkv * D), e(0, Hkv).view(0, 1, Hkv * D), table, torch.ones(0, dtype=torch.int32, device=gpu)).shape == (0, H * D)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_offsets_beyond_32_bits(stg, gpu, causal):
+    """Rows 2^24 elements apart: the last of 200 stands 3.3 * 10^9 elements behind the first, and everything equals the dense call."""
+    from stgcma import kernels as K
+    n, H, D = 200, 2, 64
+    q, k, v, table, do = _make(gpu, [n], [n], H, H, D, 32, 61)
+    geom = K.RelGeom(H, D, causal=causal, device=gpu)
+    big = torch.empty(n, 1 << 24, dtype=BF16, device=gpu)
+    wide = [big[:, i * H * D:(i + 1) * H * D] for i in range(4)]
+    for w, t in zip(wide, (q, k, v, do)):
+        w.copy_(t)
+    cu = _cu([n], gpu)
+    want, got = (_all(K, geom, a, b, c, table, cu, None, d) for a, b, c, d in ((q, k, v, do), wide))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    lens = torch.tensor([n], dtype=torch.int32, device=gpu)
+    assert torch.equal(K.relattn_decode(geom, q[:1], k[None], v[None], table, lens), K.relattn_decode(geom, q[:1], wide[1][None], wide[2][None], table, lens))
+    two = big.view(2, n // 2, 1 << 24)                          # sequences 1.7 * 10^9 elements apart
+    lens = torch.tensor([n // 2, 37], dtype=torch.int32, device=gpu)
+    dense = [t.reshape(2, n // 2, H * D) for t in (k, v)]
+    assert torch.equal(K.relattn_decode(geom, q[:2], *dense, table, lens), K.relattn_decode(geom, q[:2], two[:, :, H * D:2 * H * D], two[:, :, 2 * H * D:3 * H * D], table, lens))
+
+
+MORE = [
+    # lens_q, lens_k, H, Hkv, D, buckets, far, causal, mask
+    ([130, 3, 64], [40, 200, 0], 2, 1, 64, 32, 128, False, None),        # more queries than keys without the causal rule
+    ([2300], [2300], 1, 1, 128, 256, 2048, True, None),                  # the widest table and LDS arrays
+    ([2300], [2300], 1, 1, 128, 256, 2048, False, "random"),
+    ([2100, 1], [2101, 300], 2, 2, 32, 250, 2040, False, None),
+    ([400, 129], [400, 129], 65, 5, 32, 4, 3, True, None),               # many heads, thirteen to a group
+    ([513], [513], 2, 2, 96, 32, 128, True, "first"),
+]
+
+
+@pytest.mark.parametrize("case", range(len(MORE)))
+def test_wide_tables_and_lengths(stg, gpu, case):
+    from stgcma import kernels as K
+    lens_q, lens_k, H, Hkv, D, nb, far, causal, mk = MORE[case]
+    q, k, v, table, do = _make(gpu, lens_q, lens_k, H, Hkv, D, nb, 400 + case, fused=False)
+    mask = _mask(mk, lens_k, gpu, case, 0)
+    geom = K.RelGeom(H, D, kv_heads=Hkv, num_buckets=nb, max_distance=far, causal=causal, device=gpu)
+    ref = R.attention(q, k, v, table, lens_q, lens_k, H, Hkv, D, nb, far, causal, D ** -0.5, mask, do)
+    got = _all(K, geom, q, k, v, table, _cu(lens_q, gpu), _cu(lens_k, gpu), do, max_q=max(lens_q), max_k=max(lens_k), key_mask=mask)
+    for name, t in zip(("o", "lse", "dq", "dk", "dv", "dtable"), got):
+        R.within(t, ref[name], name, 1e-6)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_many_sequences_without_a_hint(stg, gpu, causal):
+    """20 000 sequences, nearly all empty, one of 1500 rows: fewer blocks than the longest sequence has tiles, each striding over several."""
+    from stgcma import kernels as K
+    S, H, D = 20000, 2, 32
+    lens = [0] * S
+    lens[17], lens[4000], lens[4001], lens[19998] = 33, 1500, 700, 129
+    q, k, v, table, do = _make(gpu, lens, lens, H, H, D, 32, 71, tail=3)
+    geom = K.RelGeom(H, D, causal=causal, device=gpu)
+    ref = R.attention(q, k, v, table, lens, lens, H, H, D, 32, 128, causal, D ** -0.5, None, do)
+    got = _all(K, geom, q, k, v, table, _cu(lens, gpu), None, do)
+    for name, t in zip(("o", "lse", "dq", "dk", "dv", "dtable"), got):
+        R.within(t, ref[name], name, 1e-6)
+
+
+def test_autograd_corners(stg, gpu):
+    """Saved tensors that hooks move and pack densely, single wanted gradients, a strided incoming gradient, and no second derivative."""
+    from stgcma import kernels as K, ops_seq
+    lens, H, Hkv, D = [70, 41], 4, 2, 64
+    q, k, v, table, do = _make(gpu, lens, lens, H, Hkv, D, 32, 81)
+    geom = K.RelGeom(H, D, kv_heads=Hkv, device=gpu)
+    cu, mask = _cu(lens, gpu), _mask("random", lens, gpu, 2, 0)
+    run = lambda *a: ops_seq.rel_attention(*a, geom, cu, max_q=70, key_mask=mask)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, table)]
+    want = torch.autograd.grad(run(*leaves), leaves, do)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu().contiguous(), lambda t: t.to(gpu)):
+        o = run(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(o, leaves, do)))
+    for i in (0, 1, 3):
+        a = [t.detach().requires_grad_(i == j) for j, t in enumerate((q, k, v, table))]
+        got, = torch.autograd.grad(run(*a), [a[i]], do)
+        name = ("dq", "dk", "dv", "dtable")[i]
+        R.within(got, R.attention(q, k, v, table, lens, lens, H, Hkv, D, 32, 128, False, D ** -0.5, mask, do, table_grad=i == 3)[name], name, 1e-6)
+    o = run(*leaves)
+    turned = do.t().contiguous().t()
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(o, leaves, turned)))
+    o = run(*leaves)
+    (dq,) = torch.autograd.grad(o, leaves[:1], do, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dq.float().sum().backward()
+    with torch.no_grad():
+        assert torch.equal(run(*leaves), o)
+    leaves[0].data.fill_(1.0)                                  # .data escapes the version check; an in-place change does not
+    o = run(*leaves)
+    with torch.no_grad():
+        leaves[3].add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(o, leaves, do)
+
+
+def test_refusals_on_the_gpu(stg, gpu):
+    from stgcma import kernels as K
+    lens, H, Hkv, D = [9, 4], 4, 2, 64
+    q, k, v, table, do = _make(gpu, lens, lens, H, Hkv, D, 32, 91, fused=False)
+    geom = K.RelGeom(H, D, kv_heads=Hkv, device=gpu)
+    cu = _cu(lens, gpu)
+    o, lse = K.relattn_fwd(geom, q, k, v, table, cu)
+    shifted = torch.zeros(q.numel() + 1, dtype=BF16, device=gpu)[1:].view(q.shape)
+    odd = torch.zeros(13, H * D + 4, dtype=BF16, device=gpu)[:, :H * D]
+    fwd = [(q.half(), k, v, table, cu), (q.float(), k, v, table, cu), (q[:, :-64], k, v, table, cu), (q, k[:-1], v, table, cu), (q, k, v.t(), table, cu),
+           (shifted, k, v, table, cu), (odd, k, v, table, cu), (q, k, v, table.half(), cu), (q, k, v, table[:-1], cu), (q, k, v, table.t(), cu), (q, k, v, table, cu.long()),
+           (q, k, v, table, cu.cpu()), (q, k, v, table.cpu(), cu), (q, k, v, table, cu[:0]), (q, k, v, table, cu, cu[:2].clone()), (q, q, q, table, cu)]
+    for bad in fwd:
+        with pytest.raises(RuntimeError):
+            K.relattn_fwd(geom, *bad)
+    for mask in (torch.ones(12, dtype=torch.bool, device=gpu), torch.ones(13, device=gpu), torch.ones(13, dtype=torch.bool), torch.ones(26, dtype=torch.bool, device=gpu)[::2]):
+        with pytest.raises(RuntimeError):
+            K.relattn_fwd(geom, q, k, v, table, cu, key_mask=mask)
+    with pytest.raises(RuntimeError):
+        K.relattn_fwd(geom, q, k, v, table, cu, out=torch.empty_like(q, dtype=F32))
+    with pytest.raises(RuntimeError):
+        K.relattn_fwd(geom, q, k, v, table, cu, max_q=-1)
+    for bad in ((o, lse, do.float()), (o, lse[:, :-1], do), (o, None, do), (o, lse, do[:-1]), (o.float(), lse, do)):
+        with pytest.raises(RuntimeError):
+            K.relattn_bwd(geom, q, k, v, table, cu, None, *bad)
+    kc, vc = k[None].expand(3, -1, -1), v[None].expand(3, -1, -1)
+    n3 = torch.tensor([13, 5, 1], dtype=torch.int32, device=gpu)
+    shared = K.relattn_decode(geom, q[:3], kc, vc, table, n3)   # one cache for every sequence
+    assert torch.equal(shared, K.relattn_decode(geom, q[:3], kc.contiguous(), vc.contiguous(), table, n3))
+    wide = torch.full((3, 2 * H * D), 5.0, dtype=BF16, device=gpu)
+    assert torch.equal(K.relattn_decode(geom, q[:3], kc, vc, table, n3, out=wide[:, :H * D]), shared) and bool((wide[:, H * D:] == 5.0).all())
+    for bad in ((q[:3].float(), kc, vc, table, n3), (q[:2], kc, vc, table, n3), (q[:3], kc[:, :-1], vc, table, n3), (q[:3], kc, vc.half(), table, n3), (q[:3], kc, vc, table, n3[:2]),
+                (q[:3], kc, vc, table, n3.cpu()), (q[:3], k, v, table, n3), (q[:3], kc, vc.contiguous().flatten()[:-1], table, n3)):
+        with pytest.raises(RuntimeError):
+            K.relattn_decode(geom, *bad)
+
+
+def test_two_streams_at_once(stg, gpu):
+    """Calls in flight on two streams together keep their own workspaces."""
+    from stgcma import kernels as K
+    lens, H, Hkv, D = [700, 300], 8, 2, 64
+    geom = K.RelGeom(H, D, kv_heads=Hkv, device=gpu)
+    cu = _cu(lens, gpu)
+    sets = [_make(gpu, lens, lens, H, Hkv, D, 32, 95 + i) for i in range(2)]
+    n = torch.tensor([1000, 1], dtype=torch.int32, device=gpu)
+    decode = lambda s: K.relattn_decode(geom, s[0][:2], s[1][None].expand(2, -1, -1), s[2][None].expand(2, -1, -1), s[3], n)
+    want = [_all(K, geom, *s[:4], cu, None, s[4], max_q=700) + (decode(s),) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for _ in range(3):
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(_all(K, geom, *s[:4], cu, None, s[4], max_q=700) + (decode(s),))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
