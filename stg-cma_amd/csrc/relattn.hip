@@ -235,6 +235,13 @@ __device__ __forceinline__ uint64_t key_bits(const RP& a, const Seq& z, int byte
     const uint64_t b = __builtin_amdgcn_ballot_w64((byte != 0 || a.kmask == nullptr) && kb + lane < z.nk);
     return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
 }
+// A sequence in which at most one key is visible: a row's only probability is one and dS is zero, not what its terms' roundings leave of them.
+__device__ __forceinline__ bool lone_key(const RP& a, const Seq& z, int lane) {
+    if (z.nk <= 1) return true;
+    if (a.kmask == nullptr || z.nk > 64) return false;
+    const uint64_t b = key_bits(a, z, key_load(a, z, 0, lane), 0, lane);
+    return (b & (b - 1)) == 0;
+}
 // start of a score accumulator: bias of rows kb + ACC_ROW(., hh) against the lane's query position (idx = bv index of row 0, hh included)
 __device__ __forceinline__ f32x16_t bias16(const float* bv, int idx) {
     f32x16_t c;
@@ -429,6 +436,8 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
 // row: r = rowsum(P dP) - delta, the exact delta's distance from the rounded one (sum P = 1).  Tiles behind the last border are summed here, in
 // compensated fp32, and corrected by r times their probability; the band of tiles around the diagonal is left to relattn_band_kernel, which has
 // the exact delta.  Each block leaves its sums in its own row of `part`, added up in a fixed order by relattn_dtable_kernel.
+// dQ and dK lose little by the rounded delta where many keys share a row; where a wave's queries see no more than one tile of keys, a first
+// pass over the tile (already in LDS) takes the exact one.
 struct Comp {                                                           // compensated running sum
     float s = 0.f, c = 0.f;
     __device__ __forceinline__ void add(float v) {
@@ -456,6 +465,7 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
     }
     const Seq z = seq_of(a, w.s);
     const int shift = z.nk - z.nq;
+    const bool lone = lone_key(a, z, lane);
     fill_bias(a, h, bv, tid, NTHR);
     Stage<D, NTHR> sg;
     sg.plan(tid, a.ldk, a.ldv);
@@ -504,9 +514,6 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
         const bf16_t* Vb = a.V + (int64_t)z.k0 * a.ldv + hk * D;
         Comp all, sl, sr;                                               // the lane's share of its row: sum dS, behind the left / right border
         float br = 0.f, bn = 0.f;                                       // probability behind the right border, around the diagonal
-        // dP - delta: the accumulator starts at -delta, 16 registers held for that where there is room (D <= 64), else a subtraction
-        constexpr bool HOLD = D <= 64;
-        const f32x16_t ndel = splat16(HOLD ? -delta : 0.f);
         // Wide heads: K and V take turns in one half's staging registers (K arrives behind the first 32 keys' products, V behind the second's), which
         // leaves room for two waves per SIMD.
         u32x4_t sv[SPLIT ? SC::HALF : SC::PER];
@@ -529,6 +536,44 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
         __syncthreads();
         arrived(qf);
         arrived(df);
+        auto visible = [&](int kb, uint64_t in) -> uint64_t {           // the keys of a tile that the lane's query sees, from its half-wave's first on
+            if (a.causal) {
+                const int c = pos - kb;
+                in = c < 0 ? 0 : (c >= 63 ? in : in & ((2ull << c) - 1));
+            }
+            return in >> (4 * hh);
+        };
+        const int span = a.causal && phi < z.nk ? phi + 1 : z.nk;       // keys the wave's queries see at most
+        if (live && bits != 0 && span > 0 && span <= 64) {              // few keys: delta = rowsum(P dP) first (see above)
+            float t = 0.f, l = 0.f;
+            const uint64_t vis = visible(0, bits);
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+                const bf16_t* tK = smem + half * 32 * DP;
+                f32x16_t sc, dp = splat16(0.f);
+                if (63 - plo <= -a.far) sc = splat16(bv[0]);
+                else if (-phi >= a.far) sc = splat16(bv[blen - 1]);
+                else sc = bias16(bv, 4 * hh - pos + a.far + PAD + 32 * half);
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    sc = MFMA32(nat_frag<DP>(tK, r, hh, s), qf[s], sc);
+                    dp = MFMA32(nat_frag<DP>(tK + SC::TILE, r, hh, s), df[s], dp);
+                }
+#pragma unroll
+                for (int reg = 0; reg < 16; ++reg) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nl));
+                    const bool on = (vis >> (32 * half + ACC_ROW(reg, 0))) & 1;
+                    l += on ? e : 0.f;
+                    t += on ? e * dp[reg] : 0.f;
+                }
+            }
+            t = half_sum(t);
+            l = half_sum(l);
+            delta = l > 0.f ? t / l : 0.f;
+        }
+        // dP - delta: the accumulator starts at -delta, 16 registers held for that where there is room (D <= 64), else a subtraction
+        constexpr bool HOLD = D <= 64;
+        const f32x16_t ndel = splat16(HOLD ? -delta : 0.f);
         for (int kp = 0; kp < np; ++kp) {
             const bf16_t* sK = smem + (kp & 1) * 2 * SC::TILE;
             const bf16_t* sV = sK + SC::TILE;
@@ -543,12 +588,7 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
             const bool act = live && bits != 0 && !(a.causal && kb > phi);
             {
                 const int idx0 = kb + 4 * hh - pos + a.far + PAD;
-                uint64_t vis = bits;
-                if (a.causal) {
-                    const int c = pos - kb;
-                    vis = c < 0 ? 0 : (c >= 63 ? vis : vis & ((2ull << c) - 1));
-                }
-                vis >>= 4 * hh;
+                const uint64_t vis = visible(kb, bits);
                 const bool edge = bits != ~0ull || (a.causal && kb + 63 > plo);
                 const float nf = left ? nl + cleft : (right ? nl + cright : nl);
 #pragma unroll
@@ -623,8 +663,8 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
         }
         bf16_t* dqp = a.dQ + ((int64_t)z.q0 + q) * a.lddq + h * D;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) store_tile32(dqp + 32 * dt, dq[dt], a.scale, hh, qok);
-        if (TAB) {
+        for (int dt = 0; dt < DT; ++dt) store_tile32(dqp + 32 * dt, dq[dt], lone ? 0.f : a.scale, hh, qok);
+        if (TAB && !lone) {
             const float rs = half_sum(all.s - all.c);
             br = half_sum(br);
             bn = half_sum(bn);
@@ -678,7 +718,7 @@ __global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups,
     const int t0 = ((shift - a.far - 62) >> 5) + 4 * tg, t = t0 + wave;
     const int tmax = a.causal ? (shift + 31) >> 5 : (shift + a.far + 62) >> 5;
     f32x16_t acc = splat16(0.f);
-    if (t0 <= tmax && z.nk > 0) {
+    if (t0 <= tmax && !lone_key(a, z, lane)) {
         const bool mine = t <= tmax;
         // bias of the wave's 63 distances, key - query = 32 t - shift + ACC_ROW - r: one lookup per lane, then 16 registers per lane
         f32x16_t cb;
@@ -901,6 +941,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
     }
     const Seq z = seq_of(a, w.s);
     const int shift = z.nk - z.nq;
+    const bool lone = lone_key(a, z, lane);
     Stage<D, NTHR> sg;
     sg.plan(tid, a.ldq, a.lddo);
     for (int64_t tile = w.tile; tile * 32 * NW < z.nk; tile += a.tiles) {
@@ -1050,7 +1091,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             if (!kok) { dk[dt] = splat16(0.f); dv[dt] = splat16(0.f); }     // a masked key has no gradient
-            store_tile32(kp + 32 * dt, dk[dt], a.scale, hh, stored);
+            store_tile32(kp + 32 * dt, dk[dt], lone ? 0.f : a.scale, hh, stored);
             store_tile32(vp + 32 * dt, dv[dt], 1.0f, hh, stored);
         }
         __syncthreads();

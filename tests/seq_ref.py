@@ -5,7 +5,8 @@ With u = 2^-8 (half a bf16 step, relative) and e = the relative error of a proba
     |o - ref|  <= u |ref| + (u + 2 e) sum_j p |v|
     |dv - ref| <= u |ref| + (u + 2 e) sum_i p |do|
     |dS - ref| <= 2 e p (|dP| + |delta|) + p E_i =: s_ij     E_i = error of delta_i: o's error where delta comes from the stored o (dq, and
-                                                       dk without a table gradient), fp32's where it is summed again (dtable, dk)
+                                                       dk without a table gradient, of sequences of more than 64 keys), fp32's where it
+                                                       is summed again (dtable, dk, short sequences)
     |dq - ref| <= u |ref| + scale sum_j (u |dS| + (1 + u) s_ij) |k|,   dk alike,   dtable <= sum s_ij over the bucket + its own fp32 summation.
 e: the score is a sum of D products in fp32 plus the bias, so its error is at most (D + 8) 2^-24 A with A = scale sum |q||k| + |bias| + |lse|, the
 exponential and the row sum of n terms add (n + 8) 2^-24.
@@ -92,10 +93,10 @@ def attention(q, k, v, table, lens_q, lens_k, H, Hkv, D, buckets, far, causal, s
                 s = 2 * e * p * (dP.abs() + delta.abs()) + p * (E + dperr)
                 return s, U * dS.abs() + (1 + U) * s
             rounded = U * O.abs() + (U + 2 * e) * pv
-            s, w = size(rounded)
+            s, w = size(2 * e * pv if nk <= 64 else rounded)
             out["dq"][0][rq, cq] = scale * dS @ Kk
             out["dq"][1][rq, cq] = U * (scale * dS @ Kk).abs() + scale * w @ Kk.abs()
-            s, w = size(2 * e * pv if table_grad else rounded)
+            s, w = size(2 * e * pv if table_grad or nk <= 64 else rounded)
             out["dk"][0][rk, ck] += scale * dS.t() @ Q
             out["dk"][1][rk, ck] += scale * w.t() @ Q.abs()
             out["dv"][0][rk, ck] += p.t() @ G

@@ -515,3 +515,30 @@ def test_two_streams_at_once(stg, gpu):
     torch.cuda.synchronize()
     for i, g in enumerate(got):
         assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_of_one_key_have_no_score_gradient(stg, gpu, causal, D):
+    """A softmax over one key is constant: dq, dk and dtable are zero, not the roundings of dP - delta, and dv is do."""
+    from stgcma import kernels as K
+    H, Hkv = 4, 2
+    geom = K.RelGeom(H, D, kv_heads=Hkv, causal=causal, device=gpu)
+    for lens, shown in (([1, 0, 1, 1], None), ([40, 1, 64], (7, 40, 60))):
+        q, k, v, table, do = _make(gpu, lens, lens, H, Hkv, D, 32, 131)
+        mask = None
+        if shown:
+            mask = torch.zeros(sum(lens), dtype=torch.bool, device=gpu)
+            mask[list(shown)] = True
+        for want_table in (True, False):
+            o, lse = K.relattn_fwd(geom, q, k, v, table, _cu(lens, gpu), max_q=max(lens), key_mask=mask)
+            dq, dk, dv, dt = K.relattn_bwd(geom, q, k, v, table, _cu(lens, gpu), None, o, lse, do, max_q=max(lens), key_mask=mask, want_table=want_table)
+            assert not dq.any() and not dk.any() and (dt is None or not dt.any())
+            ref = R.attention(q, k, v, table, lens, lens, H, Hkv, D, 32, 128, causal, D ** -0.5, mask, do)
+            R.within(dv, ref["dv"], "dv", 1e-6)
+    lens = [200]                                               # the first causal row, and the rows behind it that see few keys
+    q, k, v, table, do = _make(gpu, lens, lens, H, Hkv, D, 32, 132)
+    if causal:
+        dq = _all(K, geom, q, k, v, table, _cu(lens, gpu), None, do)[2]
+        ref = R.attention(q[:64], k[:64], v[:64], table, [64], [64], H, Hkv, D, 32, 128, True, D ** -0.5, None, do[:64])["dq"]
+        R.within(dq[:64], ref, "dq of the first rows", 1e-6)
