@@ -859,13 +859,23 @@ __global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups,
             }
         }
     }
-    // ---- distances: the wave's instructions stay in order, so each sum has one order
+    // ---- distances: the wave's 32 x 32 sums through LDS (rows of 33: no bank conflicts), lane u adds up the diagonal key - query = u - 31 (16 LDS
+    // additions at shared addresses instead took 7 us per block)
     __syncthreads();
-    sums[tid] = 0.f;
-    __syncthreads();
+    {
+        float* m = reinterpret_cast<float*>(smem) + 32 * 33 * wave;
+        static_assert(4 * 32 * 33 * 4 <= 10 * TILE * 2, "the sums fit where the K / V ring was");
 #pragma unroll
-    for (int reg = 0; reg < 16; ++reg)
-        __hip_atomic_fetch_add(sums + 64 * wave + ACC_ROW(reg, hh) - r + 31, acc[reg], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        for (int reg = 0; reg < 16; ++reg) m[ACC_ROW(reg, hh) * 33 + r] = acc[reg];
+        __syncthreads();
+        float t = 0.f;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+            const int row = lane - 31 + c;
+            t += row >= 0 && row < 32 ? m[(row & 31) * 33 + c] : 0.f;
+        }
+        sums[tid] = t;
+    }
     __syncthreads();
     // slot u of the block's 160 holds distance 32 t0 - shift - 31 + u, from two neighbouring diagonals; a thread per bucket collects its slots in order
     float v = 0.f;
