@@ -42,7 +42,7 @@ struct RP {
     bf16_t* dK; int64_t lddk;
     bf16_t* dV; int64_t lddv;
     float* delta;                     // [H, Tq]
-    float* part;                      // partial table gradients: [S * tiles, H, 2] behind the borders / [S * blocks, H, NB] of the band; or NULL
+    float* part;                      // partial table gradients: [S * tiles, H, 2] behind the borders / [S * tiles, H, NB] of the band; or NULL
     int tiles;                        // blocks per (sequence, head)
 };
 
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
 // TAB, the table's gradient: dtable[b] = sum of dS over a bucket's distances.  A row of dS sums to zero, so these sums cancel to a small part of
 // their terms, and delta = rowsum(dO O) from the bf16 output would leave 2^-9 of it in them.  The walk over the keys therefore also sums dS by
 // row: r = rowsum(P dP) - delta, the exact delta's distance from the rounded one (sum P = 1).  Tiles behind the last border are summed here, in
-// compensated fp32, and corrected by r times their probability; the band of tiles around the diagonal is left to relattn_band_kernel, which has
+// compensated fp32, and corrected by r times their probability; the band of tiles around the diagonal is left to relattn_dkv_kernel, which has
 // the exact delta.  Each block leaves its sums in its own row of `part`, added up in a fixed order by relattn_dtable_kernel.
 // dQ and dK lose little by the rounded delta where many keys share a row; where a wave's queries see no more than one tile of keys, a first
 // pass over the tile (already in LDS) takes the exact one.
@@ -694,220 +694,6 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
     }
 }
 
-// ------------------------------------------------------------------------------------------------ backward: table gradient, the band
-// The tiles that relattn_dq_kernel does not count as lying behind a border.  A wave walks ALONG a diagonal of 32 x 32 tiles (query tile i, key tile
-// i + t, t fixed): an accumulator register then holds one distance for the whole walk, so summing dS by distance costs one addition per element
-// and the bias is 16 registers loaded once; only at the end do the 16 x 64 sums fold into 63 distances.  A block = four neighbouring diagonals
-// and `chunk` query tiles of one (sequence, head): per step it stages one new query tile (Q, dO) and one new key tile (K, V; a ring of five).
-// Bound by the LDS reads of the four operands (nothing is reused across steps); measured against LDS additions per element in the dQ
-// kernel, which took four times as long.
-template <int D>
-__global__ void __launch_bounds__(256, 2) relattn_band_kernel(RP a, int tgroups, int chunk) {
-    constexpr int KS = D / 16, DP = D + 8, ROWP = D / 8, TILE = 32 * DP, PER = 32 * ROWP / 128;     // pieces per thread of one pair of tiles
-    extern __shared__ __attribute__((aligned(16))) bf16_t smem[];       // K / V ring [5][2][32][DP], Q / dO [2][2][32][DP], sums [4][64]
-    bf16_t* sQ = smem + 10 * TILE;
-    float* sums = reinterpret_cast<float*>(sQ + 4 * TILE);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 31, hh = lane >> 5;
-    const int h = blockIdx.y, hk = h / (a.H / a.Hkv);
-    const int tg = blockIdx.x % tgroups, ch = blockIdx.x / tgroups, nch = gridDim.x / tgroups;
-    const Seq z = seq_of(a, blockIdx.z);
-    const int shift = z.nk - z.nq;
-    const int nqt = (z.nq + 31) >> 5;
-    // diagonals that can hold an element counted here: from t_min on, four to a block
-    const int t0 = ((shift - a.far - 62) >> 5) + 4 * tg, t = t0 + wave;
-    const int tmax = a.causal ? (shift + 31) >> 5 : (shift + a.far + 62) >> 5;
-    f32x16_t acc = splat16(0.f);
-    if (t0 <= tmax && !lone_key(a, z, lane)) {
-        const bool mine = t <= tmax;
-        // bias of the wave's 63 distances, key - query = 32 t - shift + ACC_ROW - r: one lookup per lane, then 16 registers per lane
-        f32x16_t cb;
-        {
-            int d = 32 * t - shift + lane - 31;
-            d = d < -a.far ? -a.far : (d > a.far ? a.far : d);
-            int b = a.plan[d + a.far];
-            b = b < 0 ? 0 : (b < a.NB ? b : a.NB - 1);
-            sums[64 * wave + lane] = raw_bias(a.table[(int64_t)b * a.H + h], a.inv_scale);
-            __syncthreads();
-#pragma unroll
-            for (int reg = 0; reg < 16; ++reg) cb[reg] = sums[64 * wave + ACC_ROW(reg, hh) - r + 31];
-        }
-        const bf16_t* Kb = a.K + (int64_t)z.k0 * a.ldk + hk * D;
-        const bf16_t* Vb = a.V + (int64_t)z.k0 * a.ldv + hk * D;
-        const bf16_t* Qb = a.Q + (int64_t)z.q0 * a.ldq + h * D;
-        const bf16_t* Db = a.dO + (int64_t)z.q0 * a.lddo + h * D;
-        const float* lseb = a.lse + (int64_t)h * a.Tq + z.q0;
-        const float* delb = a.delta + (int64_t)h * a.Tq + z.q0;
-        const int half = tid >> 7, ti = tid & 127;                      // first or second tensor of a pair
-        auto fetch = [&](u32x4_t (&v)[PER], const bf16_t* t0p, int64_t ld0, const bf16_t* t1p, int64_t ld1, int row0, int n) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int id = ti + 128 * i, rr = id / ROWP, c = id - rr * ROWP;
-                int row = row0 + rr;
-                row = row < 0 ? 0 : (row < n ? row : n - 1);
-                v[i] = *reinterpret_cast<const u32x4_t*>((half ? t1p + (int64_t)row * ld1 : t0p + (int64_t)row * ld0) + 8 * c);
-            }
-        };
-        auto commit = [&](bf16_t* s, const u32x4_t (&v)[PER], uint32_t valid) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int id = ti + 128 * i, rr = id / ROWP, c = id - rr * ROWP;
-                u32x4_t w = v[i];
-                if (valid != ~0u && !((valid >> rr) & 1)) w = (u32x4_t){0u, 0u, 0u, 0u};
-                *reinterpret_cast<u32x4_t*>(s + half * TILE + rr * DP + 8 * c) = w;
-            }
-        };
-        // without a mask the byte comes from K's rows and does not count: one flow of loads, which the wait counts can follow
-        const uint8_t* mask = a.kmask != nullptr ? a.kmask + z.k0 : reinterpret_cast<const uint8_t*>(Kb);
-        auto kload = [&](int kt) -> int {                               // the lane's mask byte of tile kt (stays in flight)
-            int key = 32 * kt + (lane & 31);
-            key = key < 0 ? 0 : (key < z.nk ? key : z.nk - 1);
-            return mask[key];
-        };
-        auto kbits = [&](int kt, int byte) -> uint32_t {                // keys of the tile that exist and are not masked
-            const int key = 32 * kt + (lane & 31);
-            return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)__builtin_amdgcn_ballot_w64((byte != 0 || a.kmask == nullptr) && key >= 0 && key < z.nk));
-        };
-        auto qbits = [&](int i) -> uint32_t {
-            const int left = z.nq - 32 * i;
-            return left >= 32 ? ~0u : (1u << left) - 1;
-        };
-        for (int first = ch * chunk; first < nqt; first += nch * chunk) {
-            const int last = first + chunk < nqt ? first + chunk : nqt;
-            // what a step stages is fetched two steps ahead (a step computes for ~600 cycles, an L2 or MALL load takes longer): two register sets
-            struct Next { u32x4_t kv[PER], qd[PER]; float l, d; int smk, mk; } n0, n1;
-            auto ahead = [&](int i, Next& n) {                          // query tile i, its new key tile, the wave's key bits
-                fetch(n.kv, Kb, a.ldk, Vb, a.ldv, 32 * (i + t0 + 3), z.nk);
-                fetch(n.qd, Qb, a.ldq, Db, a.lddo, 32 * i, z.nq);
-                const int q = 32 * i + r < z.nq ? 32 * i + r : z.nq - 1;
-                n.l = lseb[q];
-                n.d = delb[q];
-                n.smk = kload(i + t0 + 3);
-                n.mk = kload(i + t);
-            };
-            int slot = 0;                                               // ring slot of the block's first diagonal
-            float nl, nd;
-            uint32_t bits;
-            auto enter = [&](int i, const Next& n, int kslot) {         // the step's tiles into LDS, its statistics into registers
-                commit(smem + kslot * 2 * TILE, n.kv, kbits(i + t0 + 3, n.smk));
-                commit(sQ + ((i - first) & 1) * 2 * TILE, n.qd, qbits(i));
-            };
-            auto take = [&](int i, const Next& n) {
-                const bool ok = 32 * i + r < z.nq && n.l != -INFINITY;
-                nl = ok ? -n.l * LOG2E : -INFINITY;
-                nd = ok ? -n.d : 0.f;
-                bits = kbits(i + t, n.mk);
-            };
-            auto compute = [&](int i) {
-                const int kt = i + t, kb = (32 * kt) & ~63, plo = 32 * i + shift, phi = plo + 31;
-                if (mine && bits != 0 && kb + 63 - plo > -a.far && kb - phi < a.far) {
-                    const int w = slot + wave < 5 ? slot + wave : slot + wave - 5;
-                    const bf16_t* tK = smem + w * 2 * TILE;
-                    const bf16_t* tV = tK + TILE;
-                    const bf16_t* tQ = sQ + ((i - first) & 1) * 2 * TILE;
-                    const bf16_t* tD = tQ + TILE;
-                    f32x16_t sc = cb, dp = splat16(nd);
-#pragma unroll
-                    for (int s = 0; s < KS; ++s) {
-                        sc = MFMA32(nat_frag<DP>(tK, r, hh, s), nat_frag<DP>(tQ, r, hh, s), sc);
-                        dp = MFMA32(nat_frag<DP>(tV, r, hh, s), nat_frag<DP>(tD, r, hh, s), dp);
-                    }
-                    float ds[16];
-#pragma unroll
-                    for (int reg = 0; reg < 16; ++reg) ds[reg] = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nl)) * dp[reg];
-                    if (bits != ~0u || (a.causal && 32 * kt + 31 > plo)) {
-                        asm volatile("");
-                        uint32_t vis = bits;
-                        if (a.causal) {
-                            const int c = plo + r - 32 * kt;
-                            vis = c < 0 ? 0 : (c >= 31 ? vis : vis & ((2u << c) - 1));
-                        }
-                        vis >>= 4 * hh;
-#pragma unroll
-                        for (int reg = 0; reg < 16; ++reg) ds[reg] = (vis >> ACC_ROW(reg, 0)) & 1 ? ds[reg] : 0.f;
-                    }
-#pragma unroll
-                    for (int reg = 0; reg < 16; ++reg) acc[reg] += ds[reg];
-                }
-            };
-            {
-                u32x4_t w[3][PER];
-                int ok[3];
-                for (int j = 0; j < 3; ++j) fetch(w[j], Kb, a.ldk, Vb, a.ldv, 32 * (first + t0 + j), z.nk);
-                ahead(first, n0);
-                for (int j = 0; j < 3; ++j) ok[j] = kload(first + t0 + j);
-                __syncthreads();
-                for (int j = 0; j < 3; ++j) commit(smem + j * 2 * TILE, w[j], kbits(first + t0 + j, ok[j]));
-                enter(first, n0, 3);
-                take(first, n0);
-            }
-            ahead(first + 1 < last ? first + 1 : first, n1);
-            __syncthreads();
-            auto step = [&](int i, Next& next, Next& after) {           // next: fetched for step i + 1; after: free
-                ahead(i + 2 < last ? i + 2 : i, after);                 // (always: a branch here would make the wait for `next` a wait for these)
-                compute(i);
-                if (i + 1 < last) {
-                    enter(i + 1, next, slot + 4 < 5 ? slot + 4 : slot - 1);
-                    take(i + 1, next);
-                }
-                slot = slot + 1 < 5 ? slot + 1 : 0;
-                __syncthreads();
-            };
-            for (int i = first; i < last; i += 2) {
-                step(i, n1, n0);
-                if (i + 1 < last) step(i + 1, n0, n1);
-            }
-        }
-    }
-    // ---- distances: the wave's 32 x 32 sums through LDS (rows of 33: no bank conflicts), lane u adds up the diagonal key - query = u - 31 (16 LDS
-    // additions at shared addresses instead took 7 us per block)
-    __syncthreads();
-    {
-        float* m = reinterpret_cast<float*>(smem) + 32 * 33 * wave;
-        static_assert(4 * 32 * 33 * 4 <= 10 * TILE * 2, "the sums fit where the K / V ring was");
-#pragma unroll
-        for (int reg = 0; reg < 16; ++reg) m[ACC_ROW(reg, hh) * 33 + r] = acc[reg];
-        __syncthreads();
-        float t = 0.f;
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-            const int row = lane - 31 + c;
-            t += row >= 0 && row < 32 ? m[(row & 31) * 33 + c] : 0.f;
-        }
-        sums[tid] = t;
-    }
-    __syncthreads();
-    // slot u of the block's 160 holds distance 32 t0 - shift - 31 + u, from two neighbouring diagonals; a thread per bucket collects its slots in order
-    float v = 0.f;
-    int id = -1;
-    if (tid < 160) {
-        const int w = tid >> 5, j = tid & 31;                           // wave w holds it at j, wave w - 1 at 32 + j
-        if (w < 4) v += sums[64 * w + j];
-        if (w > 0) v += sums[64 * (w - 1) + 32 + j];
-        int d = 32 * t0 - shift - 31 + tid;
-        d = d < -a.far ? -a.far : (d > a.far ? a.far : d);
-        id = a.plan[d + a.far];
-    }
-    float* val = sums;                                                  // [160] values, then [160] buckets
-    int* ids = reinterpret_cast<int*>(sums + 160);
-    __syncthreads();
-    if (tid < 160) { val[tid] = v; ids[tid] = id; }
-    __syncthreads();
-    if (tid < a.NB) {
-        float t = 0.f;
-#pragma unroll 4
-        for (int u = 0; u < 160; u += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(val + u);
-            const int4 y = *reinterpret_cast<const int4*>(ids + u);
-            t += y.x == tid ? x.x : 0.f;
-            t += y.y == tid ? x.y : 0.f;
-            t += y.z == tid ? x.z : 0.f;
-            t += y.w == tid ? x.w : 0.f;
-        }
-        a.part[(((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * a.H + h) * a.NB + tid] = t;
-    }
-}
-
 // dtable[b][h] = sum of the band's rows, and of the rows behind the borders where b is a side's last bucket, in order
 __global__ void __launch_bounds__(256) relattn_dtable_kernel(const float* band, int nband, const float* behind, int nbehind, float* dtable, int H, int NB, int causal) {
     __shared__ float s[256];
@@ -929,7 +715,15 @@ __global__ void __launch_bounds__(256) relattn_dtable_kernel(const float* band, 
 // ------------------------------------------------------------------------------------------------ backward: dK, dV
 // A block = one (sequence, key / value head) and 32 NW keys, 32 per wave; it walks the queries of every head of the group in 64-row tiles
 // of Q and dO, so the gradients of a shared head are summed in registers, in one order.  S[q][key]: rows = queries, lane = key.
-template <int D, int NW>
+//
+// TAB: the table's gradient of the tiles that relattn_dq_kernel does not count as lying behind a border; delta is the exact one by now.  A tile of dS goes
+// through 32 LDS rows of 33 (no bank conflicts) and lane l adds up its diagonals: column c of row (c + 31 - l) mod 32 belongs to the distance
+// base - 31 + l for c <= l, to base + 1 + l behind it (base = key - query of the tile's corner).  The next 32 queries lie 32 below: their upper
+// diagonals complete this tile's lower ones, so every 32 queries a wave adds 32 finished sums to an LDS array by distance.  Two arrays, of the even
+// and the odd waves: waves two apart touch distances 64 apart, and a barrier lies between two steps, so no addition meets another and
+// the order is fixed.  After each head the arrays fold into the buckets, a row of `part` per block.  (A kernel of its own for the band that computed
+// scores and dS again took 60 us where this adds @@CLIPS@@ us, 32 clips of 131 .. 490; LDS additions per element 340 us.)
+template <int D, int NW, bool TAB>
 __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
     constexpr bool WIDE = D >= 96;
@@ -937,7 +731,10 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
     constexpr int BUF = 2 * SC::TILE + 512;                             // Q and dO tiles + 4 x 64 floats of statistics
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
     float* bv = reinterpret_cast<float*>(smem + 2 * BUF);
-    const int blen = 2 * (a.far + PAD) + 1;
+    const int blen = 2 * (a.far + PAD) + 1, alen = (blen + 3) & ~3;
+    float* by = bv + alen;                                              // TAB: [2][alen] sums by distance, [NW][32][33] tiles, [alen] bucket ids
+    float* skew = by + 2 * alen;
+    uint8_t* ids = reinterpret_cast<uint8_t*>(skew + NW * 32 * 33);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // (wave-uniform for the compiler too)
     const int r = lane & 31, hh = lane >> 5;
     const Who w = who(a, a.Hkv);
@@ -952,6 +749,15 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
     const Seq z = seq_of(a, w.s);
     const int shift = z.nk - z.nq;
     const bool lone = lone_key(a, z, lane);
+    float* rows = TAB ? a.part + (((int64_t)w.s * a.tiles + w.tile) * a.H + hk * rep) * a.NB + tid : nullptr;
+    if (TAB) {
+        for (int i = tid; i < alen; i += NTHR) {
+            int x = i - (a.far + PAD);
+            x = x < -a.far ? -a.far : (x > a.far ? a.far : x);
+            ids[i] = (uint8_t)a.plan[x + a.far];
+        }
+        for (int g = 0; g < rep && tid < a.NB; ++g) rows[(int64_t)g * a.NB] = 0.f;
+    }
     Stage<D, NTHR> sg;
     sg.plan(tid, a.ldq, a.lddo);
     for (int64_t tile = w.tile; tile * 32 * NW < z.nk; tile += a.tiles) {
@@ -1013,6 +819,16 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
             };
             fetch_all(64 * p0);
             fill_bias(a, h, bv, tid, NTHR);
+            if (TAB)
+                for (int i = tid; i < 2 * alen; i += NTHR) by[i] = 0.f;
+            float* mine = by + (wave & 1) * alen + a.far + PAD + r;         // the wave's array, by distance
+            float* m = skew + wave * 32 * 33;
+            float prev = 0.f;                                           // lane l: sum of distance prev_base - 31 + l, still open
+            int prev_base = 0;
+            bool open = false;
+            auto close = [&](int at, float v) {                         // 32 finished sums, of distances at .. at + 31
+                if (hh == 0) mine[at] += v;
+            };
             __syncthreads();
             cleft = bv[0];
             cright = bv[blen - 1];
@@ -1079,6 +895,12 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                                 ds[reg] = rel <= ACC_ROW(reg, 0) ? ds[reg] : 0.f;
                             }
                         }
+                        const int plo = pb + 32 * half, kb = kw & ~63;
+                        const bool near = TAB && !lone && kb + 63 - plo > -a.far && kb - plo - 31 < a.far && !(a.causal && kw > plo + 31);
+                        if (near) {
+#pragma unroll
+                            for (int reg = 0; reg < 16; ++reg) m[(ACC_ROW(reg, 0) + 4 * hh) * 33 + r] = kok ? ds[reg] : 0.f;
+                        }
                         const bf16x8_t a0 = pack8(pr), a1 = pack8(pr + 8), d0 = pack8(ds), d1 = pack8(ds + 8);
                         if (!WIDE) trans(0);
 #pragma unroll
@@ -1090,9 +912,54 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                             dv[dt] = MFMA32(to[dt & 1][1], a1, dv[dt]);
                             dk[dt] = MFMA32(to[dt & 1][3], d1, dk[dt]);
                         }
+                        if (near) {
+                            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                            float lo = 0.f, all = 0.f;
+                            const float* m0 = m + (31 - r) * 33 + 16 * 34 * hh;     // column 16 hh of the lane's lower diagonal; the upper one 32 rows back
+                            const int behind = r - 16 * hh;
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) {
+                                const bool up = c > behind;
+                                const float v = (up ? m0 - 32 * 33 : m0)[34 * c];
+                                lo += up ? 0.f : v;
+                                all += v;
+                            }
+                            const float hi = half_sum(all - lo);
+                            const int base = kw - plo;
+                            close(base + 1, open ? hi + prev : hi);
+                            prev = half_sum(lo);
+                            prev_base = base;
+                            open = true;
+                        } else if (TAB && open) {
+                            close(prev_base - 31, prev);
+                            open = false;
+                        }
                     }
                 }
                 if (qp + 1 < np) commit_all(smem + ((qp + 1) & 1) * BUF, 64 * (qp + 1));
+                __syncthreads();
+            }
+            if (TAB && !lone) {                                         // a thread per bucket and slice of the distances, then the slices in order
+                if (open) close(prev_base - 31, prev);
+                __syncthreads();
+                const int nb2 = 1 << (32 - __builtin_clz(a.NB - 1)), sl = NTHR / nb2, b = tid & (nb2 - 1);
+                const int n4 = alen / 4, per = (n4 + sl - 1) / sl, from = tid / nb2 * per, to = min(from + per, n4);
+                float t = 0.f;
+#pragma unroll 2
+                for (int i = from; i < to; ++i) {
+                    const float4 x = *reinterpret_cast<const float4*>(by + 4 * i), y = *reinterpret_cast<const float4*>(by + alen + 4 * i);
+                    const uint32_t id = *reinterpret_cast<const uint32_t*>(ids + 4 * i);
+                    t += (int)(id & 255) == b ? x.x + y.x : 0.f;
+                    t += (int)(id >> 8 & 255) == b ? x.y + y.y : 0.f;
+                    t += (int)(id >> 16 & 255) == b ? x.z + y.z : 0.f;
+                    t += (int)(id >> 24) == b ? x.w + y.w : 0.f;
+                }
+                skew[tid] = t;
+                __syncthreads();
+                if (tid < a.NB) {
+                    for (int i = 1; i < sl; ++i) t += skew[i * nb2 + tid];
+                    rows[(int64_t)g * a.NB] += t;
+                }
                 __syncthreads();
             }
         }
@@ -1362,8 +1229,10 @@ RP make_rp(const stg_relattn_args* a) {
 }
 
 int64_t lds_fwd(int D, int far) { return (int64_t)4 * 64 * (D + 8) * 2 + (2 * (far + PAD) + 1) * 4; }
-int64_t lds_band(int D) { return (int64_t)14 * 32 * (D + 8) * 2 + 320 * 4; }
-int64_t lds_dkv(int D, int far) { return (int64_t)2 * (2 * 64 * (D + 8) + 512) * 2 + (2 * (far + PAD) + 1) * 4; }
+int64_t lds_dkv(int D, int far, bool table) {
+    const int64_t alen = (2 * (far + PAD) + 4) & ~3;
+    return (int64_t)2 * (2 * 64 * (D + 8) + 512) * 2 + alen * 4 + (table ? 2 * alen * 4 + 4 * 32 * 33 * 4 + alen : 0);
+}
 int64_t lds_dec(int D, int NB) { return (int64_t)8 * 32 * (D + 8) * 2 + (int64_t)NB * 32 * 4; }
 
 int64_t cover(int max_n, int64_t T, int rows) {
@@ -1408,27 +1277,17 @@ int launch_dq(const RP& p0, int max_q, hipStream_t st) {
     STG_LAUNCH_CHECK();
     return 0;
 }
-template <int D>
-int launch_band(const RP& p, int blocks, int tgroups, int chunk, hipStream_t st) {
-    static std::atomic<uint64_t> done{0};
-    auto k = relattn_band_kernel<D>;
-    STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_bwd: cannot reserve LDS");
-    if (p.S == 0) return 0;
-    k<<<dim3(blocks, p.H, p.S), 256, lds_band(D), st>>>(p, tgroups, chunk);
-    STG_LAUNCH_CHECK();
-    return 0;
-}
-template <int D>
+template <int D, bool TAB>
 int launch_dkv(const RP& p0, int max_k, hipStream_t st) {
     static std::atomic<uint64_t> done{0};
-    auto k = relattn_dkv_kernel<D, 4>;
+    auto k = relattn_dkv_kernel<D, 4, TAB>;
     STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_bwd: cannot reserve LDS");
     RP p = p0;
     p.tiles = grid_tiles(max_k, p.Tk, (int64_t)p.S * p.Hkv);
     const int64_t blocks = (int64_t)p.tiles * p.Hkv * (p.S + (p.zero_tail ? 1 : 0));
     STG_CHECK(blocks <= MAX_BLOCKS, -2, "relattn: %d sequences of %d heads are more than 2^24 blocks", p.S, p.H);
     if (blocks == 0) return 0;
-    k<<<dim3((unsigned)blocks), 256, lds_dkv(D, p.far), st>>>(p);
+    k<<<dim3((unsigned)blocks), 256, lds_dkv(D, p.far, TAB), st>>>(p);
     STG_LAUNCH_CHECK();
     return 0;
 }
@@ -1462,8 +1321,10 @@ int run_dq(const RP& p, int D, int max_q, hipStream_t st) {
     if (p.part) BY_DIM(D, (launch_dq<DIM, true>(p, max_q, st)));
     BY_DIM(D, (launch_dq<DIM, false>(p, max_q, st)));
 }
-int run_dkv(const RP& p, int D, int max_k, hipStream_t st) { BY_DIM(D, (launch_dkv<DIM>(p, max_k, st))); }
-int run_band(const RP& p, int D, int blocks, int tgroups, int chunk, hipStream_t st) { BY_DIM(D, (launch_band<DIM>(p, blocks, tgroups, chunk, st))); }
+int run_dkv(const RP& p, int D, int max_k, hipStream_t st) {
+    if (p.part) BY_DIM(D, (launch_dkv<DIM, true>(p, max_k, st)));
+    BY_DIM(D, (launch_dkv<DIM, false>(p, max_k, st)));
+}
 int run_decode(const DP_& p, int D, hipStream_t st) { BY_DIM(D, (launch_decode<DIM>(p, st))); }
 
 // Keys per block of the single-token form: about 1024 blocks at full length (two rounds of two per compute unit; 64 sequences of 1 .. 4096 tokens:
@@ -1486,26 +1347,14 @@ extern "C" int stg_relattn_fwd(const stg_relattn_args* a, void* stream) {
     return run_fwd(make_rp(a), a->D, a->max_q, (hipStream_t)stream);
 }
 
-// The band's grid: groups of four diagonals, and enough chunks of query tiles that about 2048 blocks exist (a chunk of at least 16 tiles pays
-// for the four key tiles a block stages before its first step).
-static void band_grid(const stg_relattn_args* a, int& tgroups, int& chunk, int& blocks) {
-    const int nt = ((a->causal ? a->far + 62 + 31 : 2 * a->far + 124) >> 5) + 2;
-    tgroups = (nt + 3) / 4;
-    const int64_t tiles = cover(a->max_q, a->Tq, 32), want = 2048 / ((int64_t)tgroups * a->H * (a->S > 0 ? a->S : 1)) + 1;
-    int64_t c = (tiles + want - 1) / want;
-    c = c < 16 ? 16 : c;
-    chunk = (int)c;
-    blocks = (int)(tgroups * ((tiles + c - 1) / c));
-}
+// rows of the table's partial gradients: one per block of the dQ and of the dK / dV kernel (and head)
+static int64_t behind_rows(const stg_relattn_args* a) { return a->Tq > 0 ? (int64_t)grid_tiles(a->max_q, a->Tq, (int64_t)a->S * a->H) * a->S : 0; }
+static int64_t band_rows(const stg_relattn_args* a) { return a->Tq > 0 && a->Tk > 0 ? (int64_t)grid_tiles(a->max_k, a->Tk, (int64_t)a->S * a->Hkv) * a->S : 0; }
 
 extern "C" int64_t stg_relattn_bwd_ws_floats(const stg_relattn_args* a, int want_table) {
-    if (a == nullptr || a->S < 0 || a->H <= 0 || a->Tq < 0 || a->num_buckets <= 0 || a->far <= 0) return -1;
+    if (a == nullptr || a->S < 0 || a->H <= 0 || a->Hkv <= 0 || a->Tq < 0 || a->Tk < 0 || a->num_buckets <= 0 || a->far <= 0) return -1;
     int64_t n = (int64_t)a->H * a->Tq;
-    if (want_table) {
-        int tg, chunk, blocks;
-        band_grid(a, tg, chunk, blocks);
-        n += (int64_t)a->S * a->H * ((int64_t)grid_tiles(a->max_q, a->Tq, (int64_t)a->S * a->H) * 2 + (int64_t)blocks * a->num_buckets);
-    }
+    if (want_table) n += a->H * (behind_rows(a) * 2 + band_rows(a) * a->num_buckets);
     return n > 0 ? n : 1;
 }
 
@@ -1525,20 +1374,14 @@ extern "C" int stg_relattn_bwd(const stg_relattn_args* a, const void* dO, int64_
     p.dO = (const bf16_t*)dO; p.lddo = lddo; p.dQ = (bf16_t*)dQ; p.lddq = lddq;
     p.dK = (bf16_t*)dK; p.lddk = lddk; p.dV = (bf16_t*)dV; p.lddv = lddv;
     p.delta = ws;
-    // table gradient: the dQ kernel's rows (two sums each), then the band's rows
-    const int nbehind = grid_tiles(a->max_q, a->Tq, (int64_t)a->S * a->H) * a->S;
     float* behind = ws + (int64_t)a->H * a->Tq;
-    float* band = behind + (int64_t)nbehind * a->H * 2;
-    int tgroups = 0, chunk = 0, blocks = 0;
-    band_grid(a, tgroups, chunk, blocks);
+    float* band = behind + behind_rows(a) * a->H * 2;
     p.part = dtable ? behind : nullptr;
     if (a->Tq > 0) { const int e = run_dq(p, a->D, a->max_q, st); if (e) return e; }
+    if (dtable) p.part = band_rows(a) > 0 ? band : nullptr;
     if (a->Tk > 0) { const int e = run_dkv(p, a->D, a->max_k, st); if (e) return e; }
     if (dtable) {
-        p.part = band;
-        if (a->Tq > 0) { const int e = run_band(p, a->D, blocks, tgroups, chunk, st); if (e) return e; }
-        relattn_dtable_kernel<<<dim3(a->H, a->num_buckets), 256, 0, st>>>(band, a->Tq > 0 ? blocks * a->S : 0, behind, a->Tq > 0 ? nbehind : 0, dtable, a->H,
-                                                                          a->num_buckets, a->causal != 0);
+        relattn_dtable_kernel<<<dim3(a->H, a->num_buckets), 256, 0, st>>>(band, (int)band_rows(a), behind, (int)behind_rows(a), dtable, a->H, a->num_buckets, a->causal != 0);
         STG_LAUNCH_CHECK();
     }
     return 0;
