@@ -722,7 +722,7 @@ __global__ void __launch_bounds__(256) relattn_dtable_kernel(const float* band, 
 // diagonals complete this tile's lower ones, so every 32 queries a wave adds 32 finished sums to an LDS array by distance.  Two arrays, of the even
 // and the odd waves: waves two apart touch distances 64 apart, and a barrier lies between two steps, so no addition meets another and
 // the order is fixed.  After each head the arrays fold into the buckets, a row of `part` per block.  (A kernel of its own for the band that computed
-// scores and dS again took 60 us where this adds @@CLIPS@@ us, 32 clips of 131 .. 490; LDS additions per element 340 us.)
+// scores and dS again took 60 us where this adds 38 us, 32 clips of 131 .. 490 x 12 x 64; LDS additions per element 340 us.)
 template <int D, int NW, bool TAB>
 __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
@@ -900,23 +900,12 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                         if (near) {
 #pragma unroll
                             for (int reg = 0; reg < 16; ++reg) m[(ACC_ROW(reg, 0) + 4 * hh) * 33 + r] = kok ? ds[reg] : 0.f;
-                        }
-                        const bf16x8_t a0 = pack8(pr), a1 = pack8(pr + 8), d0 = pack8(ds), d1 = pack8(ds + 8);
-                        if (!WIDE) trans(0);
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt) {
-                            if (dt + 1 < DT) trans(dt + 1);
-                            if (WIDE) __builtin_amdgcn_sched_barrier(0);
-                            dv[dt] = MFMA32(to[dt & 1][0], a0, dv[dt]);
-                            dk[dt] = MFMA32(to[dt & 1][2], d0, dk[dt]);
-                            dv[dt] = MFMA32(to[dt & 1][1], a1, dv[dt]);
-                            dk[dt] = MFMA32(to[dt & 1][3], d1, dk[dt]);
-                        }
-                        if (near) {
                             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                             float lo = 0.f, all = 0.f;
-                            const float* m0 = m + (31 - r) * 33 + 16 * 34 * hh;     // column 16 hh of the lane's lower diagonal; the upper one 32 rows back
-                            const int behind = r - 16 * hh;
+                            int at = (31 - r) * 33 + 16 * 34 * hh;      // column 16 hh of the lane's lower diagonal; the upper one 32 rows back
+                            int behind = r - 16 * hh;
+                            asm volatile("" : "+v"(at), "+v"(behind));  // (else the sixteen addresses are kept, and spilled, across the walk)
+                            const float* m0 = m + at;
 #pragma unroll
                             for (int c = 0; c < 16; ++c) {
                                 const bool up = c > behind;
@@ -933,6 +922,17 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                         } else if (TAB && open) {
                             close(prev_base - 31, prev);
                             open = false;
+                        }
+                        const bf16x8_t a0 = pack8(pr), a1 = pack8(pr + 8), d0 = pack8(ds), d1 = pack8(ds + 8);
+                        if (!WIDE) trans(0);
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) {
+                            if (dt + 1 < DT) trans(dt + 1);
+                            if (WIDE) __builtin_amdgcn_sched_barrier(0);
+                            dv[dt] = MFMA32(to[dt & 1][0], a0, dv[dt]);
+                            dk[dt] = MFMA32(to[dt & 1][2], d0, dk[dt]);
+                            dv[dt] = MFMA32(to[dt & 1][1], a1, dv[dt]);
+                            dk[dt] = MFMA32(to[dt & 1][3], d1, dk[dt]);
                         }
                     }
                 }
