@@ -66,10 +66,9 @@ __device__ __forceinline__ void gelu_fast(float x, float& y, float& dy) {
 // P (9 terms) and Q (8 terms) are weighted minimax fits (Lawson iteration, tools/gelu_fit.py) of the odd parts on [0, 4.5]:
 // |x Phi(x) error| <= 5.2e-5 over all x -- the level of the form it replaces, 1/35 of a bf16 half-ulp at 1 -- and |gelu' error|
 // <= 8.8e-4 (a fifth of the 8-bit derivative code's step; bf16 resolves 3.9e-3 at 1).  Beyond the clamp Phi is 1 - 3.4e-6 / 3.4e-6.
-// All multiply-adds: on PAIRS of values v_pk_mul_f32 / v_pk_fma_f32 carry two fp32 lanes per issue slot, so value + derivative cost
-// 1 (clamp) + 9.5 packed = 10.5 slots per value against 15, the value alone 6.5 against 12.  The fc1 epilogues and the fused MLP
-// kernels are VALU-bound on this function (10^9 values per stage-0 block).  The scalar and the packed forms run the same operations
-// in the same order: bit-identical.
+// All multiply-adds, written for PAIRS of values (the library is built without packed fp32 arithmetic, so a pair is two scalar
+// chains that fill each other's latency).  The fc1 epilogues and the fused MLP kernels are VALU-bound on this function (10^9 values
+// per stage-0 block).  The scalar and the paired forms run the same operations in the same order: bit-identical.
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2_t pk_fma(f32x2_t a, f32x2_t b, f32x2_t c) { return __builtin_elementwise_fma(a, b, c); }
 __device__ __forceinline__ f32x2_t pk_splat(float v) { return (f32x2_t){v, v}; }

@@ -268,7 +268,7 @@ __device__ __forceinline__ void gemm_epilogue_rows(const GemmParams& p, const Ac
                 float d[8];
                 if (!G && !c_f32) {                    // bf16 destinations: the polynomial form (common.h)
 #pragma unroll
-                    for (int j = 0; j < 8; j += 2) {   // packed fp32 pairs
+                    for (int j = 0; j < 8; j += 2) {   // fp32 pairs
                         f32x2_t y2, d2;
                         gelu_pw_both((f32x2_t){t[j], t[j + 1]}, y2, d2);
                         t[j] = y2.x; t[j + 1] = y2.y; d[j] = d2.x; d[j + 1] = d2.y;

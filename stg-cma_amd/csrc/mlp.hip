@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(512, 2) mlp_fwd_kernel(MlpP p) {
                 for (int mt = 0; mt < 2; ++mt) {
                     float x[8];
 #pragma unroll
-                    for (int r = 0; r < 4; r += 2) {     // packed fp32 pairs (common.h)
+                    for (int r = 0; r < 4; r += 2) {     // fp32 pairs (common.h)
                         const f32x2_t a2 = {S[2 * q][mt][r] + bv[r], S[2 * q][mt][r + 1] + bv[r + 1]};
                         const f32x2_t b2 = {S[2 * q + 1][mt][r] + bv[4 + r], S[2 * q + 1][mt][r + 1] + bv[4 + r + 1]};
                         const f32x2_t ya = DIAG == 1 ? a2 : gelu_pw(a2), yb = DIAG == 1 ? b2 : gelu_pw(b2);
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(512, 2) mlp_bwd_kernel(MlpB p) {
                     for (int mt = 0; mt < MT; ++mt) {
                         float x[8];
 #pragma unroll
-                        for (int r = 0; r < 4; r += 2) {          // packed fp32 pairs: only the derivative is needed here
+                        for (int r = 0; r < 4; r += 2) {          // fp32 pairs: only the derivative is needed here
                             const f32x2_t d0 = gelu_pw_grad((f32x2_t){S[0][mt][r] + bv[r], S[0][mt][r + 1] + bv[r + 1]});
                             const f32x2_t d1 = gelu_pw_grad((f32x2_t){S[1][mt][r] + bv[4 + r], S[1][mt][r + 1] + bv[4 + r + 1]});
                             x[r] = G[0][mt][r] * d0.x; x[r + 1] = G[0][mt][r + 1] * d0.y;
