@@ -2253,7 +2253,8 @@ def relattn_fwd(g, q, k, v, table, cu_q, cu_k=None, *, max_q=None, max_k=None, k
     entry at or below -1e30 hides its bucket like -inf); cu_q / cu_k int32
     [S + 1] on the device: sequence s owns rows cu[s] .. cu[s + 1] - 1 (cu_k = None: cu_q); max_q / max_k: the longest sequences, known on the host
     (they size the launch; without them the whole tensor is assumed).  key_mask bool [Tk]: False hides a key.  The last query of a sequence stands
-    at its last key.  Returns (o bf16 [Tq, H * D], lse fp32 [H, Tq] or None).  Rows behind the last sequence are zero in a fresh output and left alone in `out`."""
+    at its last key.  Returns (o bf16 [Tq, H * D], lse fp32 [H, Tq] or None).  Rows behind the last sequence are zero in a fresh output and left alone in `out`,
+    which must not overlap the inputs."""
     return _relattn_fwd(g, q, k, v, table, cu_q, cu_k, max_q, max_k, key_mask, out, want_lse)[:2]
 
 
@@ -2296,7 +2297,8 @@ def _relattn_bwd(a, dev, do, want_table):
 def relattn_decode(g, q, k_cache, v_cache, table, lens, out=None):
     """One new token per sequence over a key / value cache (stg_relattn_decode): q bf16 [S, H * D]; k_cache / v_cache bf16 [S, cap, Hkv * D] (any
     row and sequence strides that are multiples of 8, so a larger cache's slice is fine), the new token's own key and value already in
-    place; lens int32 [S] on the device: tokens in the cache, the new one included.  Returns o bf16 [S, H * D] (zero where lens is 0)."""
+    place; lens int32 [S] on the device: tokens in the cache, the new one included.  Returns o bf16 [S, H * D] (zero where lens is 0); `out` must not
+    overlap the inputs."""
     S, dev = q.shape[0], q.device
     hd, kd = g.H * g.D, g.Hkv * g.D
     _rel_chk(q, "q", BF16, hd, dev)

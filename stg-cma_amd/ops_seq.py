@@ -1,6 +1,7 @@
 """Sequence operators with gradients: attention over ragged token sequences with a learned relative position bias by buckets, and the norm - gate -
 residual - norm join around a block.  Forward and backward are libstgcma_hip.so launches on torch's current stream (relattn.hip, normjoin.hip);
-torch supplies memory only.  No state is kept between calls, so the calls may be captured, replayed and issued from several streams.
+torch supplies memory only.  No state is kept between calls, so the calls may be captured, replayed and issued from several streams.  (As for any
+captured backward: drop eager autograd graphs of the same leaves first, their accumulation nodes belong to the eager stream.)
 """
 import torch
 from torch.autograd.function import once_differentiable
