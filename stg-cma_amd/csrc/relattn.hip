@@ -143,9 +143,11 @@ __device__ __forceinline__ float raw_bias(float t, float inv_scale) {
     if (t > 1e8f && t < INFINITY) t = 1e8f;
     return t * inv_scale;
 }
-// bv[i] = bias of distance i - (far + PAD); distances past the border hold its value
+// bv[i] = bias of distance i - (far + PAD); distances past the border hold its value.  Under the causal rule no tile reaches more than 94 keys behind a
+// query (heads of 128, distances up to 2000: two blocks to a compute unit instead of one, @@C@@)
+__host__ __device__ __forceinline__ int bias_len(int far, bool causal) { return far + PAD + (causal ? PAD : far + PAD) + 1; }
 __device__ __forceinline__ void fill_bias(const RP& a, int h, float* bv, int tid, int nthr) {
-    const int len = 2 * (a.far + PAD) + 1;
+    const int len = bias_len(a.far, a.causal);
     for (int i = tid; i < len; i += nthr) {
         int d = i - (a.far + PAD);
         d = d < -a.far ? -a.far : (d > a.far ? a.far : d);
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
             stage_commit<D, NTHR>(smem, sv, tid, bits);
         }
         __syncthreads();
-        float cleft = bv[0], cright = bv[2 * (a.far + PAD)];
+        float cleft = bv[0], cright = bv[bias_len(a.far, a.causal) - 1];
         arrived(qf);
         asm volatile("" : "+v"(cleft), "+v"(cright));
         for (int kp = 0; kp < np; ++kp) {
@@ -457,7 +459,7 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
     constexpr bool SPLIT = D >= 96;
     using SC = StageC<D, NTHR>;
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
-    const int blen = 2 * (a.far + PAD) + 1;
+    const int blen = bias_len(a.far, a.causal);
     float* bv = reinterpret_cast<float*>(smem + 4 * SC::TILE);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // (wave-uniform for the compiler too)
     const int r = lane & 31, hh = lane >> 5;
@@ -738,7 +740,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
     constexpr int BUF = 2 * SC::TILE + 512;                             // Q and dO tiles + 4 x 64 floats of statistics
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
     float* bv = reinterpret_cast<float*>(smem + 2 * BUF);
-    const int blen = 2 * (a.far + PAD) + 1, alen = (blen + 3) & ~3;
+    const int blen = bias_len(a.far, a.causal), alen = (blen + 3) & ~3;
     float* by = bv + alen;                                              // TAB: [2][alen] sums by distance, [NW][32][33] tiles, [alen] bucket ids
     float* skew = by + 2 * alen;
     uint8_t* ids = reinterpret_cast<uint8_t*>(skew + NW * 32 * 33);
@@ -1236,9 +1238,9 @@ RP make_rp(const stg_relattn_args* a) {
     return p;
 }
 
-int64_t lds_fwd(int D, int far) { return (int64_t)4 * 64 * (D + 8) * 2 + (2 * (far + PAD) + 1) * 4; }
-int64_t lds_dkv(int D, int far, bool table) {
-    const int64_t alen = (2 * (far + PAD) + 4) & ~3;
+int64_t lds_fwd(int D, const RP& p) { return (int64_t)4 * 64 * (D + 8) * 2 + bias_len(p.far, p.causal) * 4; }
+int64_t lds_dkv(int D, const RP& p, bool table) {
+    const int64_t alen = (bias_len(p.far, p.causal) + 3) & ~3;
     return (int64_t)2 * (2 * 64 * (D + 8) + 512) * 2 + alen * 4 + (table ? 2 * alen * 4 + 4 * 32 * 33 * 4 + alen : 0);
 }
 int64_t lds_dec(int D, int NB) { return (int64_t)8 * 32 * (D + 8) * 2 + (int64_t)NB * 32 * 4; }
@@ -1267,7 +1269,7 @@ int launch_fwd(const RP& p0, int max_q, hipStream_t st) {
     const int64_t blocks = (int64_t)p.tiles * p.H * (p.S + (p.zero_tail ? 1 : 0));
     STG_CHECK(blocks <= MAX_BLOCKS, -2, "relattn: %d sequences of %d heads are more than 2^24 blocks", p.S, p.H);
     if (blocks == 0) return 0;
-    k<<<dim3((unsigned)blocks), 256, lds_fwd(D, p.far), st>>>(p);
+    k<<<dim3((unsigned)blocks), 256, lds_fwd(D, p), st>>>(p);
     STG_LAUNCH_CHECK();
     return 0;
 }
@@ -1281,7 +1283,7 @@ int launch_dq(const RP& p0, int max_q, hipStream_t st) {
     const int64_t blocks = (int64_t)p.tiles * p.H * (p.S + (p.zero_tail ? 1 : 0));
     STG_CHECK(blocks <= MAX_BLOCKS, -2, "relattn: %d sequences of %d heads are more than 2^24 blocks", p.S, p.H);
     if (blocks == 0) return 0;
-    k<<<dim3((unsigned)blocks), 256, lds_fwd(D, p.far), st>>>(p);
+    k<<<dim3((unsigned)blocks), 256, lds_fwd(D, p), st>>>(p);
     STG_LAUNCH_CHECK();
     return 0;
 }
@@ -1295,7 +1297,7 @@ int launch_dkv(const RP& p0, int max_k, hipStream_t st) {
     const int64_t blocks = (int64_t)p.tiles * p.Hkv * (p.S + (p.zero_tail ? 1 : 0));
     STG_CHECK(blocks <= MAX_BLOCKS, -2, "relattn: %d sequences of %d heads are more than 2^24 blocks", p.S, p.H);
     if (blocks == 0) return 0;
-    k<<<dim3((unsigned)blocks), 256, lds_dkv(D, p.far, TAB), st>>>(p);
+    k<<<dim3((unsigned)blocks), 256, lds_dkv(D, p, TAB), st>>>(p);
     STG_LAUNCH_CHECK();
     return 0;
 }
