@@ -44,6 +44,8 @@ struct RP {
     float* delta;                     // [H, Tq]
     float* part;                      // partial table gradients: [S * tiles, H, 2] behind the borders / [S * tiles, H, NB] of the band; or NULL
     int tiles;                        // blocks per (sequence, head)
+    int hsplit;                       // dK / dV: blocks that share the heads of one key / value head
+    float* pk;                        // their parts [hsplit][dK, dV][Tk, Hkv D], when there are several
 };
 
 // Which (tile, head, sequence) a block of the one-dimensional grid serves; the blocks that clear the rows behind the last sequence (s == S) come
@@ -144,7 +146,7 @@ __device__ __forceinline__ float raw_bias(float t, float inv_scale) {
     return t * inv_scale;
 }
 // bv[i] = bias of distance i - (far + PAD); distances past the border hold its value.  Under the causal rule no tile reaches more than 94 keys behind a
-// query (heads of 128, distances up to 2000: two blocks to a compute unit instead of one, @@C@@)
+// query (heads of 128, distances up to 2000: two blocks to a compute unit instead of one: 4 x 4096 x 16 heads 598 -> 400 us)
 __host__ __device__ __forceinline__ int bias_len(int far, bool causal) { return far + PAD + (causal ? PAD : far + PAD) + 1; }
 __device__ __forceinline__ void fill_bias(const RP& a, int h, float* bv, int tid, int nthr) {
     const int len = bias_len(a.far, a.causal);
@@ -746,8 +748,8 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
     uint8_t* ids = reinterpret_cast<uint8_t*>(skew + NW * 32 * 33);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // (wave-uniform for the compiler too)
     const int r = lane & 31, hh = lane >> 5;
-    const Who w = who(a, a.Hkv);
-    const int hk = w.h, rep = a.H / a.Hkv;
+    const Who w = who(a, a.Hkv * a.hsplit);
+    const int hk = w.h / a.hsplit, rep = a.H / a.Hkv / a.hsplit, head0 = w.h * rep;       // the block's heads: head0 .. head0 + rep - 1
     if (w.s == a.S) {
         const int64_t from = tail_start(a.cu_k, a.S, a.Tk);
         const int step = a.tiles * NTHR, off = w.tile * NTHR + tid;
@@ -758,7 +760,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
     const Seq z = seq_of(a, w.s);
     const int shift = z.nk - z.nq;
     const bool lone = lone_key(a, z, lane);
-    float* rows = TAB ? a.part + (((int64_t)w.s * a.tiles + w.tile) * a.H + hk * rep) * a.NB + tid : nullptr;
+    float* rows = TAB ? a.part + (((int64_t)w.s * a.tiles + w.tile) * a.H + head0) * a.NB + tid : nullptr;
     if (TAB) {
         for (int i = tid; i < alen; i += NTHR) {
             int x = i - (a.far + PAD);
@@ -798,7 +800,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
         arrived(kf);
         arrived(vf);
         for (int g = 0; g < rep && p0 < np; ++g) {
-            const int h = hk * rep + g;
+            const int h = head0 + g;
             const bf16_t* Qb = a.Q + (int64_t)z.q0 * a.ldq + h * D;
             const bf16_t* Db = a.dO + (int64_t)z.q0 * a.lddo + h * D;
             const float* lseb = a.lse + (int64_t)h * a.Tq + z.q0;
@@ -972,6 +974,29 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                 __syncthreads();
             }
         }
+        if (a.hsplit > 1) {
+            const int64_t n = a.Tk * a.Hkv * D;
+            float* kp = a.pk + 2 * (w.h - hk * a.hsplit) * n + (((int64_t)z.k0 + key) * a.Hkv + hk) * D + 4 * hh;
+            if (stored) {
+                const float sk = kok && !lone ? a.scale : 0.f;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4) {
+                        const int c = 32 * dt + 8 * g4;
+                        float x[4], y[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {                   // (a masked key's sums may be anything)
+                            x[j] = kok ? dk[dt][4 * g4 + j] * sk : 0.f;
+                            y[j] = kok ? dv[dt][4 * g4 + j] : 0.f;
+                        }
+                        *reinterpret_cast<float4*>(kp + c) = make_float4(x[0], x[1], x[2], x[3]);
+                        *reinterpret_cast<float4*>(kp + n + c) = make_float4(y[0], y[1], y[2], y[3]);
+                    }
+            }
+            __syncthreads();
+            continue;
+        }
         bf16_t* kp = a.dK + ((int64_t)z.k0 + key) * a.lddk + hk * D;
         bf16_t* vp = a.dV + ((int64_t)z.k0 + key) * a.lddv + hk * D;
 #pragma unroll
@@ -981,6 +1006,27 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
             store_tile32(vp + 32 * dt, dv[dt], 1.0f, hh, stored);
         }
         __syncthreads();
+    }
+}
+
+// dK and dV from the parts of the blocks that shared a key / value head's query heads, summed in order; rows behind the last sequence as in zero_tail
+__global__ void __launch_bounds__(256) relattn_kvsum_kernel(RP a, int kd) {
+    const int per = kd / 4;
+    const int64_t n = a.Tk * kd, from = tail_start(a.cu_k, a.S, a.Tk);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.Tk * per; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / per;
+        const int col = 4 * (int)(i - row * per);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+        if (row < from) {
+            const float* p = a.pk + row * kd + col;
+            for (int k = 0; k < a.hsplit; ++k, p += 2 * n) {
+                const float4 u = *reinterpret_cast<const float4*>(p), v = *reinterpret_cast<const float4*>(p + n);
+                x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
+                y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
+            }
+        } else if (!a.zero_tail) continue;
+        *reinterpret_cast<uint2*>(a.dK + row * a.lddk + col) = make_uint2(pack_bf2(x.x, x.y), pack_bf2(x.z, x.w));
+        *reinterpret_cast<uint2*>(a.dV + row * a.lddv + col) = make_uint2(pack_bf2(y.x, y.y), pack_bf2(y.z, y.w));
     }
 }
 
@@ -1234,6 +1280,7 @@ RP make_rp(const stg_relattn_args* a) {
     p.cu_q = a->cu_q; p.cu_k = a->cu_k; p.kmask = (const uint8_t*)a->key_mask;
     p.Tq = a->Tq; p.Tk = a->Tk; p.S = a->S; p.H = a->H; p.Hkv = a->Hkv; p.causal = a->causal != 0; p.zero_tail = a->zero_tail != 0;
     p.table = a->table; p.plan = a->plan; p.NB = a->num_buckets; p.far = a->far;
+    p.hsplit = 1;
     p.scale = a->scale; p.scale2 = a->scale * LOG2E; p.inv_scale = 1.0f / a->scale;
     return p;
 }
@@ -1294,11 +1341,17 @@ int launch_dkv(const RP& p0, int max_k, hipStream_t st) {
     STG_CHECK(stg_reserve_lds(k, 160 * 1024, done), -5, "stg_relattn_bwd: cannot reserve LDS");
     RP p = p0;
     p.tiles = grid_tiles(max_k, p.Tk, (int64_t)p.S * p.Hkv);
-    const int64_t blocks = (int64_t)p.tiles * p.Hkv * (p.S + (p.zero_tail ? 1 : 0));
+    const int64_t blocks = (int64_t)p.tiles * p.Hkv * p.hsplit * (p.S + (p.zero_tail && p.hsplit == 1 ? 1 : 0));
     STG_CHECK(blocks <= MAX_BLOCKS, -2, "relattn: %d sequences of %d heads are more than 2^24 blocks", p.S, p.H);
-    if (blocks == 0) return 0;
-    k<<<dim3((unsigned)blocks), 256, lds_dkv(D, p, TAB), st>>>(p);
-    STG_LAUNCH_CHECK();
+    if (blocks > 0) {
+        k<<<dim3((unsigned)blocks), 256, lds_dkv(D, p, TAB), st>>>(p);
+        STG_LAUNCH_CHECK();
+    }
+    if (p.hsplit > 1) {
+        const int64_t n = (p.Tk * (p.Hkv * D / 4) + 255) / 256;
+        relattn_kvsum_kernel<<<dim3((unsigned)(n < 2048 ? n : 2048)), 256, 0, st>>>(p, p.Hkv * D);
+        STG_LAUNCH_CHECK();
+    }
     return 0;
 }
 template <int D>
@@ -1357,13 +1410,26 @@ extern "C" int stg_relattn_fwd(const stg_relattn_args* a, void* stream) {
     return run_fwd(make_rp(a), a->D, a->max_q, (hipStream_t)stream);
 }
 
+// Blocks that share the query heads of a key / value head in the dK / dV kernel: as many as bring the launch to 1024 (four per compute unit at D >= 96, where one is
+// resident), by the rows alone, so that a length hint changes no bit.  @@H@@
+static int head_split(const stg_relattn_args* a) {
+    const int rep = a->H / a->Hkv;
+    const int64_t blocks = (a->Tk / 128 + a->S) * a->Hkv;
+    int n = 1;
+    while (n < rep && (rep % n != 0 || blocks * n < 1024)) ++n;
+    return n;
+}
+static int64_t split_floats(const stg_relattn_args* a) {
+    const int n = head_split(a);
+    return n > 1 ? (int64_t)n * 2 * a->Tk * a->Hkv * a->D : 0;
+}
 // rows of the table's partial gradients: one per block of the dQ and of the dK / dV kernel (and head)
 static int64_t behind_rows(const stg_relattn_args* a) { return a->Tq > 0 ? (int64_t)grid_tiles(a->max_q, a->Tq, (int64_t)a->S * a->H) * a->S : 0; }
 static int64_t band_rows(const stg_relattn_args* a) { return a->Tq > 0 && a->Tk > 0 ? (int64_t)grid_tiles(a->max_k, a->Tk, (int64_t)a->S * a->Hkv) * a->S : 0; }
 
 extern "C" int64_t stg_relattn_bwd_ws_floats(const stg_relattn_args* a, int want_table) {
-    if (a == nullptr || a->S < 0 || a->H <= 0 || a->Hkv <= 0 || a->Tq < 0 || a->Tk < 0 || a->num_buckets <= 0 || a->far <= 0) return -1;
-    int64_t n = (int64_t)a->H * a->Tq;
+    if (a == nullptr || a->S < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv != 0 || a->D <= 0 || a->Tq < 0 || a->Tk < 0 || a->num_buckets <= 0 || a->far <= 0) return -1;
+    int64_t n = (int64_t)a->H * a->Tq + split_floats(a);
     if (want_table) n += a->H * (behind_rows(a) * 2 + band_rows(a) * a->num_buckets);
     return n > 0 ? n : 1;
 }
@@ -1377,14 +1443,16 @@ extern "C" int stg_relattn_bwd(const stg_relattn_args* a, const void* dO, int64_
     STG_CHECK(lddo <= MAX_LD, -3, "stg_relattn_bwd: leading dimensions up to 2^24");
     STG_CHECK(lddo >= hd && lddq >= hd && lddk >= kd && lddv >= kd && lddo % 8 == 0 && lddq % 8 == 0 && lddk % 8 == 0 && lddv % 8 == 0, -3,
               "stg_relattn_bwd: leading dimensions must be multiples of 8 and hold every head");
-    STG_CHECK(!misaligned(dO) && !misaligned(dQ) && !misaligned(dK) && !misaligned(dV), -3, "stg_relattn_bwd: tensors must be 16-byte aligned");
+    STG_CHECK(!misaligned(dO) && !misaligned(dQ) && !misaligned(dK) && !misaligned(dV) && !misaligned(ws), -3, "stg_relattn_bwd: tensors must be 16-byte aligned");
     STG_CHECK(ws_floats >= stg_relattn_bwd_ws_floats(a, dtable != nullptr), -4, "stg_relattn_bwd: workspace of %lld floats is too small", (long long)ws_floats);
     hipStream_t st = (hipStream_t)stream;
     RP p = make_rp(a);
     p.dO = (const bf16_t*)dO; p.lddo = lddo; p.dQ = (bf16_t*)dQ; p.lddq = lddq;
     p.dK = (bf16_t*)dK; p.lddk = lddk; p.dV = (bf16_t*)dV; p.lddv = lddv;
-    p.delta = ws;
-    float* behind = ws + (int64_t)a->H * a->Tq;
+    p.hsplit = head_split(a);
+    p.pk = ws;
+    p.delta = ws + split_floats(a);
+    float* behind = p.delta + (int64_t)a->H * a->Tq;
     float* band = behind + behind_rows(a) * a->H * 2;
     p.part = dtable ? behind : nullptr;
     if (a->Tq > 0) { const int e = run_dq(p, a->D, a->max_q, st); if (e) return e; }

@@ -408,16 +408,18 @@ def test_wide_tables_and_lengths(stg, gpu, case):
         R.within(t, ref[name], name, 1e-6)
 
 
+@pytest.mark.parametrize("Hkv", [2, 1])
 @pytest.mark.parametrize("causal", [False, True])
-def test_many_sequences_without_a_hint(stg, gpu, causal):
-    """20 000 sequences, nearly all empty, one of 1500 rows: fewer blocks than the longest sequence has tiles, each striding over several."""
+def test_many_sequences_without_a_hint(stg, gpu, causal, Hkv):
+    """20 000 sequences, nearly all empty, one of 1500 rows: fewer blocks than the longest sequence has tiles, each striding over several; a shared head's
+    query heads stay in one block (elsewhere in this file they are split over several)."""
     from stgcma import kernels as K
     S, H, D = 20000, 2, 32
     lens = [0] * S
     lens[17], lens[4000], lens[4001], lens[19998] = 33, 1500, 700, 129
-    q, k, v, table, do = _make(gpu, lens, lens, H, H, D, 32, 71, tail=3)
-    geom = K.RelGeom(H, D, causal=causal, device=gpu)
-    ref = R.attention(q, k, v, table, lens, lens, H, H, D, 32, 128, causal, D ** -0.5, None, do)
+    q, k, v, table, do = _make(gpu, lens, lens, H, Hkv, D, 32, 71, tail=3)
+    geom = K.RelGeom(H, D, kv_heads=Hkv, causal=causal, device=gpu)
+    ref = R.attention(q, k, v, table, lens, lens, H, Hkv, D, 32, 128, causal, D ** -0.5, None, do)
     got = _all(K, geom, q, k, v, table, _cu(lens, gpu), None, do)
     for name, t in zip(("o", "lse", "dq", "dk", "dv", "dtable"), got):
         R.within(t, ref[name], name, 1e-6)
