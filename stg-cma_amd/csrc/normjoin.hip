@@ -242,7 +242,8 @@ __global__ void __launch_bounds__(Blk<TPR>::NT) norm_join_bwd_kernel(JP a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) aw1[c][i] = ab1[c][i] = aw2[c][i] = ab2[c][i] = ag[c][i] = 0.f;
     }
-    const float gate0 = a.gate_kind == 1 ? a.gate[0] : 1.f;
+    const bool one = a.gate_kind == 1;                                  // ag[0]: its gradient's sum and compensation
+    const float gate0 = one ? a.gate[0] : 1.f;
     auto set = [&](int c, int k, int64_t gr, bool fresh) {              // weights and gate of chunk c into slot k; fresh: the group's gate alone
         const int col = col0 + 8 * TPR * c;
         if (!fresh) {
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(Blk<TPR>::NT) norm_join_bwd_kernel(JP a) {
             row_sum2<TPR>(c1, c2, red);
             c1 = a.rms ? 0.f : c1 * invC;
             c2 *= invC;
-            float e1 = 0.f, e2 = 0.f;
+            float e1 = 0.f, e2 = 0.f, gsum = 0.f;
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
                 const bool ok = on[c] && row >= 0;
@@ -332,7 +333,9 @@ __global__ void __launch_bounds__(Blk<TPR>::NT) norm_join_bwd_kernel(JP a) {
                     t[c][k] = fmaf(st[3], dy[c][k] - fmaf(z[c][k], c2, c1), t[c][k]);     // gradient of x'
                     h[c][k] = ok ? (h[c][k] - st[0]) * st[1] : 0.f;
                     t[c][k] = ok ? t[c][k] : 0.f;
-                    ag[c][k] = fmaf(t[c][k], fmaf(h[c][k], w1[u][k], b1[u][k]), ag[c][k]);
+                    const float n = fmaf(h[c][k], w1[u][k], b1[u][k]);
+                    if (one) gsum = fmaf(t[c][k], n, gsum);
+                    else ag[c][k] = fmaf(t[c][k], n, ag[c][k]);
                     const float dn = t[c][k] * g[u][k];
                     aw1[c][k] = fmaf(dn, h[c][k], aw1[c][k]);
                     ab1[c][k] += dn;
@@ -342,6 +345,11 @@ __global__ void __launch_bounds__(Blk<TPR>::NT) norm_join_bwd_kernel(JP a) {
                     t[c][k] *= a.alpha;
                 }
                 if (ok) store8((XT*)a.dx + row * a.lddx + col0 + 8 * TPR * c, t[c]);
+            }
+            if (one) {                                                  // one sum of every element: compensated, or it loses what cancels in it
+                const float v = gsum - ag[0][1], q = ag[0][0] + v;
+                ag[0][1] = (q - ag[0][0]) - v;
+                ag[0][0] = q;
             }
             row_sum2<TPR>(e1, e2, red);
             e1 = a.rms ? 0.f : e1 * invC;
@@ -374,20 +382,17 @@ __global__ void __launch_bounds__(Blk<TPR>::NT) norm_join_bwd_kernel(JP a) {
         flush8<TPR, NCH>(aw2, sum, out, a.C, on); out += a.C;
         if (a.b2) { flush8<TPR, NCH>(ab2, sum, out, a.C, on); out += a.C; }
         if (a.gate_kind == 2) flush8<TPR, NCH>(ag, sum, out, a.C, on);
-        if (a.gate_kind == 1) {
-            float v = 0.f;
+        if (one) {
+            __shared__ double wsum[NW];
+            double v = (double)ag[0][0] - (double)ag[0][1];
 #pragma unroll
-            for (int c = 0; c < NCH; ++c)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v += ag[c][k];
-            v = wave_sum<64>(v);
-            __syncthreads();
-            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+            for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+            if ((threadIdx.x & 63) == 0) wsum[threadIdx.x >> 6] = v;
             __syncthreads();
             if (threadIdx.x == 0) {
-                float s = 0.f;
-                for (int w = 0; w < NW; ++w) s += red[w];
-                out[0] = s;
+                double t = 0.0;
+                for (int w = 0; w < NW; ++w) t += wsum[w];
+                out[0] = (float)t;
             }
         }
     }
@@ -395,11 +400,11 @@ __global__ void __launch_bounds__(Blk<TPR>::NT) norm_join_bwd_kernel(JP a) {
 
 // out[b][c] = sum_i in[b][i][c]: 16 columns x 64 row strides to a block (many blocks with few serial loads each), in a fixed order
 __global__ void __launch_bounds__(1024) norm_join_sum_kernel(const float* in, float* out, int n, int64_t cols) {
-    __shared__ float s[64][17];
+    __shared__ double s[64][17];
     const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
     const int64_t col = (int64_t)blockIdx.x * 16 + c;
     const float* p = in + (int64_t)blockIdx.y * n * cols;
-    float t = 0.f;
+    double t = 0.0;
     if (col < cols) {
 #pragma unroll 4
         for (int i = k; i < n; i += 64) t += p[(int64_t)i * cols + col];
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(1024) norm_join_sum_kernel(const float* in, fl
         if (k < w) s[k][c] += s[k + w][c];
         __syncthreads();
     }
-    if (k == 0 && col < cols) out[(int64_t)blockIdx.y * cols + col] = s[0][c];
+    if (k == 0 && col < cols) out[(int64_t)blockIdx.y * cols + col] = (float)s[0][c];
 }
 
 // the same for a handful of rows: a thread per column
