@@ -388,11 +388,20 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
                 for (int reg = 2; reg < 15; ++reg) mr = fmax3(mr, sA[reg], sB[reg + 1]);
                 mr = fmax2(mr, sA[15]);
                 mr = half_max(mr) + far;
-                const float mx = fmax2(m, mr * a.scale2);
-                const float nm = mx == -INFINITY ? 0.f : -mx;           // nothing seen so far: every exponent is -inf
-                const float alpha = __builtin_amdgcn_exp2f(m + nm);
+                // The reference follows the maximum only once some query's maximum is 2^8 above it (a probability is then below 2^8 and keeps its bits):
+                // following at once, half of the tiles of a few thousand keys rescale.
+                if (__builtin_amdgcn_ballot_w64(mr * a.scale2 > m + 8.f) != 0) {
+                    const float mx = fmax2(m, mr * a.scale2);
+                    const float alpha = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mx);
+                    m = mx;
+                    l *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int reg = 0; reg < 16; ++reg) o[dt][reg] *= alpha;
+                }
+                const float nm = m == -INFINITY ? 0.f : -m;             // nothing seen so far: every exponent is -inf
                 const float nf = far == 0.f ? nm : fmaf(far, a.scale2, nm);
-                m = mx;
                 float xA[16], xB[16];
                 float ls = 0.f;
 #pragma unroll
@@ -401,14 +410,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
                     xB[reg] = __builtin_amdgcn_exp2f(fmaf(sB[reg], a.scale2, nf));
                     ls += xA[reg] + xB[reg];
                 }
-                ls = half_sum(ls);
-                l = l * alpha + ls;
-                if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {  // rescale only when some query's maximum moved
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                        for (int reg = 0; reg < 16; ++reg) o[dt][reg] *= alpha;
-                }
+                l += half_sum(ls);
                 const bf16x8_t pf[4] = {pack8(xA), pack8(xA + 8), pack8(xB), pack8(xB + 8)};
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
