@@ -353,6 +353,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
                 // St[key][q] of keys kb .. + 31 / + 32 .. + 63.  Behind a border the bias is one number: it joins the exponent's constant and
                 // the MFMA starts at zero; nearer, the accumulator starts at the bias.
                 f32x16_t sA, sB;
+                __builtin_amdgcn_s_setprio(1);                          // products before the other waves' exponentials: 1 .. 4 % (in dQ: nothing)
                 float far = 0.f;
                 const bool left = kb + 63 - plo <= -a.far;
                 if (left || kb - phi >= a.far) {
@@ -369,6 +370,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
                     sA = MFMA32(nat_frag<DP>(sK, r, hh, s), qf[s], sA);
                     sB = MFMA32(nat_frag<DP>(sK + 32 * DP, r, hh, s), qf[s], sB);
                 }
+                __builtin_amdgcn_s_setprio(0);
                 if (bits != ~0ull || (a.causal && kb + 63 > plo)) {
                     uint64_t vis = bits;                                // keys this lane's query may see
                     if (a.causal) {
@@ -412,10 +414,12 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
                 }
                 l += half_sum(ls);
                 const bf16x8_t pf[4] = {pack8(xA), pack8(xA + 8), pack8(xB), pack8(xB + 8)};
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[dt] = MFMA32(tr_frag<DP>(sV, dt, i, hh, r), pf[i], o[dt]);
+                __builtin_amdgcn_s_setprio(0);
             }
             if (kp + 1 < np) {
                 bits = key_bits(a, z, mk, kb + 64, lane);
