@@ -272,8 +272,8 @@ __device__ __forceinline__ int64_t tail_start(const int32_t* cu, int S, int64_t 
 // Scores are computed transposed (rows = keys, lane = query): the softmax statistics are lane-local and P feeds the second MFMA from
 // registers.
 // Bound by issue: exponentials and their packing (a dozen VALU slots per score and four lanes) beside the products, 38 % of the cycles in
-// the matrix units at D = 64, 32 % at D = 128.  1.44 ms = 0.76 PFLOP/s (one sequence of 16384, 16 heads of 64), 0.35 ms = 0.60 PFLOP/s
-// (causal, 1311 .. 4097 x 32 / 8 heads of 128), 0.11 ms = 0.50 (985 .. 1970, 8 heads of 96).  Tiles of 64 queries and two waves: 1.8 times slower at every
+// the matrix units at D = 64, 33 % at D = 128.  1.35 ms = 0.81 PFLOP/s (one sequence of 16384, 16 heads of 64), 0.30 ms = 0.70 PFLOP/s
+// (causal, 1311 .. 4097 x 32 / 8 heads of 128), 0.105 ms = 0.54 (985 .. 1970, 8 heads of 96).  Tiles of 64 queries and two waves: 1.8 times slower at every
 // length (K and V staged twice as often by half the threads).
 template <int D, int NW>
 __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(RP a) {
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
 // the exact delta.  Each block leaves its sums in its own row of `part`, added up in a fixed order by relattn_dtable_kernel.
 // dQ and dK lose little by the rounded delta where many keys share a row; where a wave's queries see no more than one tile of keys, a first
 // pass over the tile (already in LDS) takes the exact one.
-// Bound like the forward (35 % of the cycles in the matrix units): 2.25 ms = 0.73 PFLOP/s (16384 x 16 x 64), 0.50 ms = 0.64 PFLOP/s (the documents).
+// Bound like the forward (35 % of the cycles in the matrix units): 2.25 ms = 0.73 PFLOP/s (16384 x 16 x 64), 0.45 ms = 0.70 PFLOP/s (the documents).
 struct Comp {                                                           // compensated running sum
     float s = 0.f, c = 0.f;
     __device__ __forceinline__ void add(float v) {
@@ -738,8 +738,9 @@ __global__ void __launch_bounds__(256) relattn_dtable_kernel(const float* band, 
 // and the odd waves: waves two apart touch distances 64 apart, and a barrier lies between two steps, so no addition meets another and
 // the order is fixed.  After each head the arrays fold into the buckets, a row of `part` per block.  (A kernel of its own for the band that computed
 // scores and dS again took 60 us where this adds 38 us, 32 clips of 131 .. 490 x 12 x 64; LDS additions per element 340 us.)
-// 2.40 ms = 0.92 PFLOP/s without the table's gradient (16384 x 16 x 64), 2.73 ms with it (distances up to 800); 0.80 / 0.93 ms (the documents, whose 490
-// registers leave one wave per SIMD: the walk waits for its own LDS reads; with 256 registers and two waves it spilled, 2.58 ms).
+// 2.40 ms = 0.92 PFLOP/s without the table's gradient (16384 x 16 x 64), 2.73 ms with it (distances up to 800); 0.62 / 0.75 ms (the documents, whose 490
+// registers leave one wave per SIMD: the walk waits for its own LDS reads.  Two waves per SIMD spilled, 2.58 ms, or, as eight waves with the keys in LDS
+// and half a tile's queries each, read a quarter more from LDS: 0.75 / 0.78 ms).
 template <int D, int NW, bool TAB>
 __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
