@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
 // the exact delta.  Each block leaves its sums in its own row of `part`, added up in a fixed order by relattn_dtable_kernel.
 // dQ and dK lose little by the rounded delta where many keys share a row; where a wave's queries see no more than one tile of keys, a first
 // pass over the tile (already in LDS) takes the exact one.
-// Bound like the forward (35 % of the cycles in the matrix units): 2.25 ms = 0.73 PFLOP/s (16384 x 16 x 64), 0.45 ms = 0.70 PFLOP/s (the documents).
+// Bound like the forward (35 % of the cycles in the matrix units): 1.79 ms = 0.92 PFLOP/s without the table's gradient (16384 x 16 x 64), 2.06 ms with it; 0.40 / 0.44 ms (the documents).
 struct Comp {                                                           // compensated running sum
     float s = 0.f, c = 0.f;
     __device__ __forceinline__ void add(float v) {
@@ -737,10 +737,10 @@ __global__ void __launch_bounds__(256) relattn_dtable_kernel(const float* band, 
 // diagonals complete this tile's lower ones, so every 32 queries a wave adds 32 finished sums to an LDS array by distance.  Two arrays, of the even
 // and the odd waves: waves two apart touch distances 64 apart, and a barrier lies between two steps, so no addition meets another and
 // the order is fixed.  After each head the arrays fold into the buckets, a row of `part` per block.  (A kernel of its own for the band that computed
-// scores and dS again took 60 us where this adds 38 us, 32 clips of 131 .. 490 x 12 x 64; LDS additions per element 340 us.)
-// 2.40 ms = 0.92 PFLOP/s without the table's gradient (16384 x 16 x 64), 2.73 ms with it (distances up to 800); 0.62 / 0.75 ms (the documents, whose 490
-// registers leave one wave per SIMD: the walk waits for its own LDS reads.  Two waves per SIMD spilled, 2.58 ms, or, as eight waves with the keys in LDS
-// and half a tile's queries each, read a quarter more from LDS: 0.75 / 0.78 ms).
+// scores and dS again took 60 us where this adds 35 us, 32 clips of 131 .. 490 x 12 x 64; LDS additions per element 340 us.)
+// 2.23 ms = 0.98 PFLOP/s without the table's gradient (16384 x 16 x 64), 2.51 ms with it (distances up to 800); 0.64 / 0.73 ms (the documents, whose 490
+// registers leave one wave per SIMD: the walk waits for its own LDS reads.  Two waves per SIMD spilled, 2.6 ms, or, as eight waves with the keys in LDS
+// and half a tile's queries each, read a quarter more from LDS: the whole backward 1.19 ms against 1.07 without the table).
 template <int D, int NW, bool TAB>
 __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
