@@ -649,7 +649,8 @@ int stg_bn_bwd(const void* x, const void* dy, const float* mean, const float* rs
  *   cu_q / cu_k int32 [S + 1] on the device: sequence s owns rows cu[s] .. cu[s + 1] - 1 (cu[0] is taken as 0; offsets outside the tensors are
  *   clamped, so no content of theirs makes a kernel leave its operands).  max_q / max_k: the longest sequences, on the host; they size the grid
  *   only -- every row of a longer sequence is still computed.
- *   table fp32 [num_buckets, H]; an entry at or below -1e30 (the type's lowest value too) hides its bucket's keys as -inf does.  plan int32 [2 far + 1] on the device: the bucket of every distance
+ *   table fp32 [num_buckets, H]; an entry at or below -1e30 (the type's lowest value too) hides its bucket's keys as -inf does; other
+ *   finite entries act as if held within +-1e8.  plan int32 [2 far + 1] on the device: the bucket of every distance
  *   -far .. far (key position - query position; larger distances share the ends); without `causal` the last buckets of the two sides are
  *   num_buckets / 2 - 1 (keys before the query) and num_buckets - 1, with it num_buckets - 1; far <= 2048.
  *   lse fp32 [H, Tq] (natural logarithm; may be NULL in a forward without backward).

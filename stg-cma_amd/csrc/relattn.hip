@@ -42,6 +42,8 @@ struct RP {
     bf16_t* dK; int64_t lddk;
     bf16_t* dV; int64_t lddv;
     float* delta;                     // [H, Tq]
+    float* fix;                       // [H, Tq]: what the score of a row far out (BIG_LSE) needs beside lse, in raw units; other rows' entries are not set
+    uint32_t* big; int qtiles;        // [S, H, qtiles, 4]: whether a wave of the dQ kernel met such a row; that kernel's `tiles`
     float* part;                      // partial table gradients: [S * tiles, H, 2] behind the borders / [S * tiles, H, NB] of the band; or NULL
     int tiles;                        // blocks per (sequence, head)
     int hsplit;                       // dK / dV: blocks that share the heads of one key / value head
@@ -137,8 +139,9 @@ __device__ __forceinline__ Seq seq_of(const RP& a, int s) {
 }
 
 // A table entry in units of the raw score.  Entries at or below -1e30 (the type's lowest value, a common mask) hide their bucket like -inf: as
-// scores they would swallow q.k in fp32 and leave rows that the log-sum-exp cannot describe.  Other finite entries are held within +-1e8,
-// where the row maximum's own rounding (2^-24 of it, common to the row) still cancels in the normalisation.
+// scores they would swallow q.k in fp32.  Other finite entries are held within +-1e8, where a row maximum's own rounding (at most 8 in the
+// exponent, common to the row) leaves every power of two in range and cancels in the normalisation: by the row's sum in the forward, by the sum of the
+// recomputed probabilities in the backward (BIG_LSE).
 __device__ __forceinline__ float raw_bias(float t, float inv_scale) {
     if (t <= -1e30f) return -INFINITY;
     if (t < -1e8f) t = -1e8f;
@@ -453,6 +456,14 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
 // dQ and dK lose little by the rounded delta where many keys share a row; where a wave's queries see no more than one tile of keys, a first
 // pass over the tile (already in LDS) takes the exact one.
 // Bound like the forward (35 % of the cycles in the matrix units): 1.79 ms = 0.92 PFLOP/s without the table's gradient (16384 x 16 x 64), 2.06 ms with it; 0.40 / 0.44 ms (the documents).
+// lse is one fp32 number: beyond 2^8 (in powers of two) its spacing leaves more than 2^-16 of a probability, at 1e6 five percent, at 1e8 nothing of log2(sum).
+// Rows that far out sum their recomputed probabilities and divide by the sum: dQ (linear in P) at its end, dK / dV through RP::fix, a second term of the
+// row's score.  Two sums, because the kernels round a score differently: here q.k joins the bias (as in the forward), there bias - lse.  Without
+// such a row none of it is done: dQ asks per wave, dK / dV learns of it by a word per wave of dQ.  Costs of asking: backward with the table's gradient
+// 152 -> 155 us (clips), 4.51 -> 4.54 ms (16384 x 16 x 64).
+constexpr float BIG_LSE = 256.f;
+// dK / dV start a row's scores here, in units of the raw score
+__device__ __forceinline__ float lse_start(float lse, float inv_scale) { return -lse * inv_scale; }
 struct Comp {                                                           // compensated running sum
     float s = 0.f, c = 0.f;
     __device__ __forceinline__ void add(float v) {
@@ -485,8 +496,11 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
     Stage<D, NTHR> sg;
     sg.plan(tid, a.ldk, a.ldv);
     float tab_l = 0.f, tab_r = 0.f;                                     // the lane's sums behind the borders, corrected
+    uint32_t far_out = 0;                                               // the wave met a row far out
+    uint32_t* word = a.big + (((int64_t)w.s * a.H + h) * a.tiles + w.tile) * NW + wave;
+    if ((int64_t)w.tile * 32 * NW >= z.nq && lane == 0) word[0] = 0;
     __syncthreads();
-    const float cleft = bv[0] * a.scale2, cright = bv[blen - 1] * a.scale2;
+    const float cleft = bv[0], cright = bv[blen - 1];
     for (int64_t tile = w.tile; tile * 32 * NW < z.nq; tile += a.tiles) {
         const int nt = (z.nq + 32 * NW - 1) / (32 * NW);
         const int qt = a.causal ? nt - 1 - (int)tile : (int)tile;
@@ -516,6 +530,11 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
         const bool seen = qok && lse != -INFINITY;                      // a row that saw no key has no gradient
         const float nl = seen ? -lse * LOG2E : -INFINITY;
         if (!seen) delta = 0.f;
+        const bool big = seen && fabsf(nl) > BIG_LSE;
+        const bool sums = __builtin_amdgcn_ballot_w64(big) != 0;        // some row of the wave needs its sum
+        far_out |= sums;
+        if (lane == 0) word[0] = far_out;
+        float psum = 0.f, ksum = 0.f;                                   // the lane's share of it, as here and as dK / dV add bias, lse and q.k
         f32x16_t dq[DT];
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) dq[dt] = splat16(0.f);
@@ -562,13 +581,13 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
         if (live && bits != 0 && span > 0 && span <= 64) {              // few keys: delta = rowsum(P dP) first (see above)
             float t = 0.f, l = 0.f;
             const uint64_t vis = visible(0, bits);
+            const bool left = 63 - plo <= -a.far, right = -phi >= a.far;
+            const float nf = left || right ? fmaf(left ? cleft : cright, a.scale2, nl) : nl;
 #pragma unroll 1
             for (int half = 0; half < 2; ++half) {
                 const bf16_t* tK = smem + half * 32 * DP;
-                f32x16_t sc, dp = splat16(0.f);
-                if (63 - plo <= -a.far) sc = splat16(bv[0]);
-                else if (-phi >= a.far) sc = splat16(bv[blen - 1]);
-                else sc = bias16(bv, 4 * hh - pos + a.far + PAD + 32 * half);
+                f32x16_t sc = splat16(0.f), dp = splat16(0.f);
+                if (!left && !right) sc = bias16(bv, 4 * hh - pos + a.far + PAD + 32 * half);
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
                     sc = MFMA32(nat_frag<DP>(tK, r, hh, s), qf[s], sc);
@@ -576,7 +595,7 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
                 }
 #pragma unroll
                 for (int reg = 0; reg < 16; ++reg) {
-                    const float e = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nl));
+                    const float e = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nf));
                     const bool on = (vis >> (32 * half + ACC_ROW(reg, 0))) & 1;
                     l += on ? e : 0.f;
                     t += on ? e * dp[reg] : 0.f;
@@ -605,7 +624,32 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
                 const int idx0 = kb + 4 * hh - pos + a.far + PAD;
                 const uint64_t vis = visible(kb, bits);
                 const bool edge = bits != ~0ull || (a.causal && kb + 63 > plo);
-                const float nf = left ? nl + cleft : (right ? nl + cright : nl);
+                const float nf = left || right ? fmaf(left ? cleft : cright, a.scale2, nl) : nl;
+                if (sums && act) {                                  // (apart from the products below, whose registers it would lengthen)
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        const float first = lse_start(a.lse[(int64_t)h * a.Tq + qrow], a.inv_scale);
+                        f32x16_t sc = splat16(0.f), sk = splat16(first + (left ? cleft : cright));
+                        if (!left && !right) {
+                            sc = bias16(bv, idx0 + 32 * half);
+#pragma unroll
+                            for (int reg = 0; reg < 16; ++reg) sk[reg] = first + sc[reg];
+                        }
+#pragma unroll
+                        for (int s = 0; s < KS; ++s) {
+                            const bf16x8_t kf = nat_frag<DP>(sK + half * 32 * DP, r, hh, s);
+                            sc = MFMA32(kf, qf[s], sc);
+                            sk = MFMA32(kf, qf[s], sk);
+                        }
+#pragma unroll
+                        for (int reg = 0; reg < 16; ++reg) {
+                            const bool on = (vis >> (32 * half + ACC_ROW(reg, 0))) & 1;
+                            const float e = __builtin_amdgcn_exp2f(fmaf(sc[reg], a.scale2, nf)), f = __builtin_amdgcn_exp2f(sk[reg] * a.scale2);
+                            psum += on ? e : 0.f;
+                            ksum += on ? f : 0.f;
+                        }
+                    }
+                }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {              // the two 32-key tiles, one after the other (register budget)
                     if (act) {
@@ -676,21 +720,28 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
             }
             __syncthreads();
         }
+        float norm = 1.f;                                               // of a row far out: 1 / sum P; dK / dV's second term goes to a.fix
+        if (sums) {
+            psum = half_sum(psum);
+            ksum = half_sum(ksum);
+            if (big && psum > 0.f) norm = 1.f / psum;
+            if (big && hh == 0) a.fix[(int64_t)h * a.Tq + qrow] = ksum > 0.f ? -__log2f(ksum) / a.scale2 : 0.f;
+        }
         bf16_t* dqp = a.dQ + ((int64_t)z.q0 + q) * a.lddq + h * D;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) store_tile32(dqp + 32 * dt, dq[dt], lone ? 0.f : a.scale, hh, qok);
+        for (int dt = 0; dt < DT; ++dt) store_tile32(dqp + 32 * dt, dq[dt], lone ? 0.f : a.scale * norm, hh, qok);
         if (TAB && !lone) {
-            const float rs = half_sum(all.s - all.c);
-            br = half_sum(br);
-            bn = half_sum(bn);
+            const float rs = half_sum(all.s - all.c) * norm;
+            br = half_sum(br) * norm;
+            bn = half_sum(bn) * norm;
             const float bl = fmaxf(1.f - br - bn, 0.f);
             if (hh == 0 && seen) {                                      // once per row: the halves' sums of dS enter below, one per lane
                 tab_l -= rs * bl;
                 tab_r -= rs * br;
             }
             delta += rs;                                                // rowsum(P dP) to fp32
-            tab_l += sl.s - sl.c;
-            tab_r += sr.s - sr.c;
+            tab_l += (sl.s - sl.c) * norm;
+            tab_r += (sr.s - sr.c) * norm;
         }
         if (qok && hh == 0) a.delta[(int64_t)h * a.Tq + qrow] = delta;
     }
@@ -741,12 +792,13 @@ __global__ void __launch_bounds__(256) relattn_dtable_kernel(const float* band, 
 // 2.23 ms = 0.98 PFLOP/s without the table's gradient (16384 x 16 x 64), 2.51 ms with it (distances up to 800); 0.64 / 0.73 ms (the documents, whose 490
 // registers leave one wave per SIMD: the walk waits for its own LDS reads.  Two waves per SIMD spilled, 2.6 ms, or, as eight waves with the keys in LDS
 // and half a tile's queries each, read a quarter more from LDS: the whole backward 1.19 ms against 1.07 without the table).
+constexpr int STATS = 2 * (5 * 64 + 4);           // 5 x 64 floats and the waves' votes, in bf16 elements
 template <int D, int NW, bool TAB>
 __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
     constexpr bool WIDE = D >= 96;
     using SC = StageC<D, NTHR>;
-    constexpr int BUF = 2 * SC::TILE + 512;                             // Q and dO tiles + 4 x 64 floats of statistics
+    constexpr int BUF = 2 * SC::TILE + STATS;                           // Q and dO tiles and their rows' statistics
     extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
     float* bv = reinterpret_cast<float*>(smem + 2 * BUF);
     const int blen = bias_len(a.far, a.causal), alen = (blen + 3) & ~3;
@@ -775,6 +827,14 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
             ids[i] = (uint8_t)a.plan[x + a.far];
         }
         for (int g = 0; g < rep && tid < a.NB; ++g) rows[(int64_t)g * a.NB] = 0.f;
+    }
+    uint32_t* vote = reinterpret_cast<uint32_t*>(smem + 2 * SC::TILE) + 320;      // (in the first buffer's statistics)
+    uint32_t any = 0;                                                   // did dQ meet a row far out among this block's heads?
+    {
+        const int n = rep * a.qtiles * 4;
+        const uint32_t* big = a.big + ((int64_t)w.s * a.H + head0) * a.qtiles * 4;
+        if (tid < n) any = big[tid];
+        for (int i = tid + NTHR; i < n; i += NTHR) any |= big[i];
     }
     Stage<D, NTHR> sg;
     sg.plan(tid, a.ldq, a.lddo);
@@ -806,12 +866,18 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
         const int p0 = qfirst >> 6, np = (z.nq + 63) >> 6;
         arrived(kf);
         arrived(vf);
+        if (tile == w.tile) {
+            const uint64_t b = __builtin_amdgcn_ballot_w64(any != 0);
+            if (lane == 0) vote[wave] = b != 0;
+            any = 0;
+        }
         for (int g = 0; g < rep && p0 < np; ++g) {
             const int h = head0 + g;
             const bf16_t* Qb = a.Q + (int64_t)z.q0 * a.ldq + h * D;
             const bf16_t* Db = a.dO + (int64_t)z.q0 * a.lddo + h * D;
             const float* lseb = a.lse + (int64_t)h * a.Tq + z.q0;
             const float* delb = a.delta + (int64_t)h * a.Tq + z.q0;
+            const float* fixb = a.fix + (int64_t)h * a.Tq + z.q0;
             u32x4_t sv[SC::PER];
             float nl = 0.f, nd = 0.f, cleft, cright;
             auto fetch_all = [&](int q0) {
@@ -822,17 +888,23 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                     nd = delb[qi];
                 }
             };
-            auto commit_all = [&](bf16_t* buf, int q0) {
+            auto commit_all = [&](bf16_t* buf, int q0, int apart) {
                 const int left = z.nq - q0;
                 stage_commit<D, NTHR>(buf, sv, tid, left >= 64 ? ~0ull : (1ull << left) - 1);
                 float* st = reinterpret_cast<float*>(buf + 2 * SC::TILE);
                 if (tid < 64) {                                         // lse in units of the raw score; a row that saw nothing, or none at all: P = 0
                     const bool ok = tid < left && nl != -INFINITY;
-                    const float l = ok ? -nl * a.inv_scale : -INFINITY;
+                    const float l = ok ? lse_start(nl, a.inv_scale) : -INFINITY;
                     st[tid] = l;
                     st[64 + tid] = l + cleft;
                     st[128 + tid] = l + cright;
                     st[192 + tid] = ok ? -nd : 0.f;
+                    if (apart != 0) {                                   // the second term: behind a border it joins the sum
+                        const float f = ok && fabsf(nl * LOG2E) > BIG_LSE ? fixb[q0 + tid] : 0.f;
+                        st[64 + tid] = (l + cleft) + f;
+                        st[128 + tid] = (l + cright) + f;
+                        st[256 + tid] = f;
+                    }
                 }
             };
             fetch_all(64 * p0);
@@ -850,7 +922,8 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
             __syncthreads();
             cleft = bv[0];
             cright = bv[blen - 1];
-            commit_all(smem + (p0 & 1) * BUF, 64 * p0);
+            int apart = __builtin_amdgcn_readfirstlane(vote[0] | vote[1] | vote[2] | vote[3]);
+            commit_all(smem + (p0 & 1) * BUF, 64 * p0, apart);
             __syncthreads();
             for (int qp = p0; qp < np; ++qp) {
                 const bf16_t* sQ = smem + (qp & 1) * BUF;
@@ -858,6 +931,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                 const float* sL = reinterpret_cast<const float*>(sQ + 2 * SC::TILE);
                 if (qp + 1 < np) fetch_all(64 * (qp + 1));
                 const int pb = 64 * qp + shift;                         // position of the tile's first query
+                asm volatile("" : "+s"(apart));                         // (else the walk is compiled twice, and spills)
                 if (live && !(a.causal && pb + 63 < kw)) {
                     const bool left = kw + 31 - pb <= -a.far, right = kw - (pb + 63) >= a.far;
                     const bool edge = a.causal && kw + 31 > pb;
@@ -881,6 +955,12 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                             const float* bp = bv + rel + a.far + PAD;
 #pragma unroll
                             for (int reg = 0; reg < 16; ++reg) sc[reg] += bp[-ACC_ROW(reg, 0)];
+                            if (apart != 0) {
+                                asm volatile("");
+                                const float* fx = sL + 256 + 32 * half + 4 * hh;
+#pragma unroll
+                                for (int reg = 0; reg < 16; ++reg) sc[reg] += fx[ACC_ROW(reg, 0)];
+                            }
                         }
                         // one wave per SIMD (D >= 96): nothing else hides the LDS latency, so the operands of a whole phase are asked for at once
                         bf16x8_t qa[KS], da[KS];
@@ -954,7 +1034,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                         }
                     }
                 }
-                if (qp + 1 < np) commit_all(smem + ((qp + 1) & 1) * BUF, 64 * (qp + 1));
+                if (qp + 1 < np) commit_all(smem + ((qp + 1) & 1) * BUF, 64 * (qp + 1), apart);
                 __syncthreads();
             }
             if (TAB && !lone) {                                         // a thread per bucket and slice of the distances, then the slices in order
@@ -1295,7 +1375,7 @@ RP make_rp(const stg_relattn_args* a) {
 int64_t lds_fwd(int D, const RP& p) { return (int64_t)4 * 64 * (D + 8) * 2 + bias_len(p.far, p.causal) * 4; }
 int64_t lds_dkv(int D, const RP& p, bool table) {
     const int64_t alen = (bias_len(p.far, p.causal) + 3) & ~3;
-    return (int64_t)2 * (2 * 64 * (D + 8) + 512) * 2 + alen * 4 + (table ? 2 * alen * 4 + 4 * 32 * 33 * 4 + alen : 0);
+    return (int64_t)2 * (2 * 64 * (D + 8) + STATS) * 2 + alen * 4 + (table ? 2 * alen * 4 + 4 * 32 * 33 * 4 + alen : 0);
 }
 int64_t lds_dec(int D, int NB) { return (int64_t)8 * 32 * (D + 8) * 2 + (int64_t)NB * 32 * 4; }
 
@@ -1434,11 +1514,12 @@ static int64_t split_floats(const stg_relattn_args* a) {
 }
 // rows of the table's partial gradients: one per block of the dQ and of the dK / dV kernel (and head)
 static int64_t behind_rows(const stg_relattn_args* a) { return a->Tq > 0 ? (int64_t)grid_tiles(a->max_q, a->Tq, (int64_t)a->S * a->H) * a->S : 0; }
+static int64_t big_words(const stg_relattn_args* a) { return behind_rows(a) * a->H * 4; }
 static int64_t band_rows(const stg_relattn_args* a) { return a->Tq > 0 && a->Tk > 0 ? (int64_t)grid_tiles(a->max_k, a->Tk, (int64_t)a->S * a->Hkv) * a->S : 0; }
 
 extern "C" int64_t stg_relattn_bwd_ws_floats(const stg_relattn_args* a, int want_table) {
     if (a == nullptr || a->S < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv != 0 || a->D <= 0 || a->Tq < 0 || a->Tk < 0 || a->num_buckets <= 0 || a->far <= 0) return -1;
-    int64_t n = (int64_t)a->H * a->Tq + split_floats(a);
+    int64_t n = (int64_t)2 * a->H * a->Tq + big_words(a) + split_floats(a);
     if (want_table) n += a->H * (behind_rows(a) * 2 + band_rows(a) * a->num_buckets);
     return n > 0 ? n : 1;
 }
@@ -1461,7 +1542,10 @@ extern "C" int stg_relattn_bwd(const stg_relattn_args* a, const void* dO, int64_
     p.hsplit = head_split(a);
     p.pk = ws;
     p.delta = ws + split_floats(a);
-    float* behind = p.delta + (int64_t)a->H * a->Tq;
+    p.fix = p.delta + (int64_t)a->H * a->Tq;
+    p.big = reinterpret_cast<uint32_t*>(p.fix + (int64_t)a->H * a->Tq);
+    p.qtiles = a->Tq > 0 ? grid_tiles(a->max_q, a->Tq, (int64_t)a->S * a->H) : 0;
+    float* behind = p.fix + (int64_t)a->H * a->Tq + big_words(a);
     float* band = behind + behind_rows(a) * a->H * 2;
     p.part = dtable ? behind : nullptr;
     if (a->Tq > 0) { const int e = run_dq(p, a->D, a->max_q, st); if (e) return e; }

@@ -2250,7 +2250,7 @@ def relattn_fwd(g, q, k, v, table, cu_q, cu_k=None, *, max_q=None, max_k=None, k
     """Attention over ragged sequences with a learned relative position bias by buckets (stg_relattn_fwd).
 
     q bf16 [Tq, H * D], k / v bf16 [Tk, Hkv * D] (column slices of a fused projection are fine); table fp32 [num_buckets, H] (an
-    entry at or below -1e30 hides its bucket like -inf); cu_q / cu_k int32
+    entry at or below -1e30 hides its bucket like -inf, other finite entries are held within +-1e8); cu_q / cu_k int32
     [S + 1] on the device: sequence s owns rows cu[s] .. cu[s + 1] - 1 (cu_k = None: cu_q); max_q / max_k: the longest sequences, known on the host
     (they size the launch; without them the whole tensor is assumed).  key_mask bool [Tk]: False hides a key.  The last query of a sequence stands
     at its last key.  Returns (o bf16 [Tq, H * D], lse fp32 [H, Tq] or None).  Rows behind the last sequence are zero in a fresh output and left alone in `out`,
