@@ -43,7 +43,7 @@ struct RP {
     bf16_t* dV; int64_t lddv;
     float* delta;                     // [H, Tq]
     float* fix;                       // [H, Tq]: what the score of a row far out (BIG_LSE) needs beside lse, in raw units; other rows' entries are not set
-    uint32_t* big; int qtiles;        // [S, H, qtiles, 4]: whether a wave of the dQ kernel met such a row; that kernel's `tiles`
+    uint32_t* seen; int qtiles;       // [S, H, qtiles, 4]: what a wave of the dQ kernel saw (FAR_OUT, LONE); that kernel's `tiles`
     float* part;                      // partial table gradients: [S * tiles, H, 2] behind the borders / [S * tiles, H, NB] of the band; or NULL
     int tiles;                        // blocks per (sequence, head)
     int hsplit;                       // dK / dV: blocks that share the heads of one key / value head
@@ -242,12 +242,20 @@ __device__ __forceinline__ uint64_t key_bits(const RP& a, const Seq& z, int byte
     const uint64_t b = __builtin_amdgcn_ballot_w64((byte != 0 || a.kmask == nullptr) && kb + lane < z.nk);
     return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
 }
-// A sequence in which at most one key is visible: a row's only probability is one and dS is zero, not what its terms' roundings leave of them.
+// A sequence in which at most one key is visible: a row's only probability is one and dS is zero, not what its terms' roundings leave of them.  Asked where the
+// first 64 keys show at most one (`few`), and ends at the second visible key.
+__device__ __forceinline__ bool few(uint64_t bits) { return (bits & (bits - 1)) == 0; }
 __device__ __forceinline__ bool lone_key(const RP& a, const Seq& z, int lane) {
     if (z.nk <= 1) return true;
-    if (a.kmask == nullptr || z.nk > 64) return false;
-    const uint64_t b = key_bits(a, z, key_load(a, z, 0, lane), 0, lane);
-    return (b & (b - 1)) == 0;
+    if (a.kmask == nullptr) return false;
+    bool one = false;
+#pragma unroll 1
+    for (int kb = 0; kb < z.nk; kb += 64) {
+        const uint64_t b = key_bits(a, z, key_load(a, z, kb, lane), kb, lane);
+        if (!few(b) || (b != 0 && one)) return false;
+        one = one || b != 0;
+    }
+    return true;
 }
 // start of a score accumulator: bias of rows kb + ACC_ROW(., hh) against the lane's query position (idx = bv index of row 0, hh included)
 __device__ __forceinline__ f32x16_t bias16(const float* bv, int idx) {
@@ -462,6 +470,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
 // such a row none of it is done: dQ asks per wave, dK / dV learns of it by a word per wave of dQ.  Costs of asking: backward with the table's gradient
 // 152 -> 155 us (clips), 4.51 -> 4.54 ms (16384 x 16 x 64).
 constexpr float BIG_LSE = 256.f;
+constexpr int FAR_OUT = 1, LONE = 2;              // what a wave of dQ leaves for dK / dV: such a row, a sequence with at most one visible key
 // dK / dV start a row's scores here, in units of the raw score
 __device__ __forceinline__ float lse_start(float lse, float inv_scale) { return -lse * inv_scale; }
 struct Comp {                                                           // compensated running sum
@@ -473,7 +482,7 @@ struct Comp {                                                           // compe
     }
 };
 template <int D, int NW, bool TAB>
-__global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
+__global__ void __launch_bounds__(NW * 64, D <= 32 ? 3 : 2) relattn_dq_kernel(RP a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, NTHR = NW * 64;
     constexpr bool SPLIT = D >= 96;
     using SC = StageC<D, NTHR>;
@@ -491,13 +500,12 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
     }
     const Seq z = seq_of(a, w.s);
     const int shift = z.nk - z.nq;
-    const bool lone = lone_key(a, z, lane);
     fill_bias(a, h, bv, tid, NTHR);
     Stage<D, NTHR> sg;
     sg.plan(tid, a.ldk, a.ldv);
     float tab_l = 0.f, tab_r = 0.f;                                     // the lane's sums behind the borders, corrected
-    uint32_t far_out = 0;                                               // the wave met a row far out
-    uint32_t* word = a.big + (((int64_t)w.s * a.H + h) * a.tiles + w.tile) * NW + wave;
+    int saw = 0;
+    uint32_t* word = a.seen + (((int64_t)w.s * a.H + h) * a.tiles + w.tile) * NW + wave;
     if ((int64_t)w.tile * 32 * NW >= z.nq && lane == 0) word[0] = 0;
     __syncthreads();
     const float cleft = bv[0], cright = bv[blen - 1];
@@ -532,8 +540,6 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
         if (!seen) delta = 0.f;
         const bool big = seen && fabsf(nl) > BIG_LSE;
         const bool sums = __builtin_amdgcn_ballot_w64(big) != 0;        // some row of the wave needs its sum
-        far_out |= sums;
-        if (lane == 0) word[0] = far_out;
         float psum = 0.f, ksum = 0.f;                                   // the lane's share of it, as here and as dK / dV add bias, lse and q.k
         f32x16_t dq[DT];
 #pragma unroll
@@ -570,6 +576,8 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
         __syncthreads();
         arrived(qf);
         arrived(df);
+        saw |= (sums ? FAR_OUT : 0) | (few(bits) && lone_key(a, z, lane) ? LONE : 0);
+        if (lane == 0) word[0] = saw;
         auto visible = [&](int kb, uint64_t in) -> uint64_t {           // the keys of a tile that the lane's query sees, from its half-wave's first on
             if (a.causal) {
                 const int c = pos - kb;
@@ -727,6 +735,7 @@ __global__ void __launch_bounds__(NW * 64, 2) relattn_dq_kernel(RP a) {
             if (big && psum > 0.f) norm = 1.f / psum;
             if (big && hh == 0) a.fix[(int64_t)h * a.Tq + qrow] = ksum > 0.f ? -__log2f(ksum) / a.scale2 : 0.f;
         }
+        const bool lone = (saw & LONE) != 0;
         bf16_t* dqp = a.dQ + ((int64_t)z.q0 + q) * a.lddq + h * D;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) store_tile32(dqp + 32 * dt, dq[dt], lone ? 0.f : a.scale * norm, hh, qok);
@@ -818,7 +827,6 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
     }
     const Seq z = seq_of(a, w.s);
     const int shift = z.nk - z.nq;
-    const bool lone = lone_key(a, z, lane);
     float* rows = TAB ? a.part + (((int64_t)w.s * a.tiles + w.tile) * a.H + head0) * a.NB + tid : nullptr;
     if (TAB) {
         for (int i = tid; i < alen; i += NTHR) {
@@ -829,13 +837,14 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
         for (int g = 0; g < rep && tid < a.NB; ++g) rows[(int64_t)g * a.NB] = 0.f;
     }
     uint32_t* vote = reinterpret_cast<uint32_t*>(smem + 2 * SC::TILE) + 320;      // (in the first buffer's statistics)
-    uint32_t any = 0;                                                   // did dQ meet a row far out among this block's heads?
+    uint32_t any = 0;                                                   // what dQ saw among this block's heads
     {
         const int n = rep * a.qtiles * 4;
-        const uint32_t* big = a.big + ((int64_t)w.s * a.H + head0) * a.qtiles * 4;
-        if (tid < n) any = big[tid];
-        for (int i = tid + NTHR; i < n; i += NTHR) any |= big[i];
+        const uint32_t* seen = a.seen + ((int64_t)w.s * a.H + head0) * a.qtiles * 4;
+        if (tid < n) any = seen[tid];
+        for (int i = tid + NTHR; i < n; i += NTHR) any |= seen[i];
     }
+    auto votes = [&]() -> int { return __builtin_amdgcn_readfirstlane(vote[0] | vote[1] | vote[2] | vote[3]); };
     Stage<D, NTHR> sg;
     sg.plan(tid, a.ldq, a.lddo);
     for (int64_t tile = w.tile; tile * 32 * NW < z.nk; tile += a.tiles) {
@@ -867,8 +876,8 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
         arrived(kf);
         arrived(vf);
         if (tile == w.tile) {
-            const uint64_t b = __builtin_amdgcn_ballot_w64(any != 0);
-            if (lane == 0) vote[wave] = b != 0;
+            const uint64_t far_out = __builtin_amdgcn_ballot_w64((any & FAR_OUT) != 0), lone = __builtin_amdgcn_ballot_w64((any & LONE) != 0);
+            if (lane == 0) vote[wave] = (far_out != 0 ? FAR_OUT : 0) | (lone != 0 ? LONE : 0);
             any = 0;
         }
         for (int g = 0; g < rep && p0 < np; ++g) {
@@ -922,7 +931,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
             __syncthreads();
             cleft = bv[0];
             cright = bv[blen - 1];
-            int apart = __builtin_amdgcn_readfirstlane(vote[0] | vote[1] | vote[2] | vote[3]);
+            int apart = votes() & FAR_OUT;
             commit_all(smem + (p0 & 1) * BUF, 64 * p0, apart);
             __syncthreads();
             for (int qp = p0; qp < np; ++qp) {
@@ -994,7 +1003,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                             }
                         }
                         const int plo = pb + 32 * half, kb = kw & ~63;
-                        const bool near = TAB && !lone && kb + 63 - plo > -a.far && kb - plo - 31 < a.far && !(a.causal && kw > plo + 31);
+                        const bool near = TAB && kb + 63 - plo > -a.far && kb - plo - 31 < a.far && !(a.causal && kw > plo + 31);
                         if (near) {
 #pragma unroll
                             for (int reg = 0; reg < 16; ++reg) m[(ACC_ROW(reg, 0) + 4 * hh) * 33 + r] = kok ? ds[reg] : 0.f;
@@ -1037,7 +1046,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                 if (qp + 1 < np) commit_all(smem + ((qp + 1) & 1) * BUF, 64 * (qp + 1), apart);
                 __syncthreads();
             }
-            if (TAB && !lone) {                                         // a thread per bucket and slice of the distances, then the slices in order
+            if (TAB && !(votes() & LONE)) {                             // a thread per bucket and slice of the distances, then the slices in order
                 if (open) close(prev_base - 31, prev);
                 __syncthreads();
                 const int nb2 = 1 << (32 - __builtin_clz(a.NB - 1)), sl = NTHR / nb2, b = tid & (nb2 - 1);
@@ -1061,6 +1070,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 2 : 1) relattn_dkv_kernel(R
                 __syncthreads();
             }
         }
+        const bool lone = p0 < np && (votes() & LONE);
         if (a.hsplit > 1) {
             const int64_t n = a.Tk * a.Hkv * D;
             float* kp = a.pk + 2 * (w.h - hk * a.hsplit) * n + (((int64_t)z.k0 + key) * a.Hkv + hk) * D + 4 * hh;
@@ -1514,12 +1524,12 @@ static int64_t split_floats(const stg_relattn_args* a) {
 }
 // rows of the table's partial gradients: one per block of the dQ and of the dK / dV kernel (and head)
 static int64_t behind_rows(const stg_relattn_args* a) { return a->Tq > 0 ? (int64_t)grid_tiles(a->max_q, a->Tq, (int64_t)a->S * a->H) * a->S : 0; }
-static int64_t big_words(const stg_relattn_args* a) { return behind_rows(a) * a->H * 4; }
+static int64_t seen_words(const stg_relattn_args* a) { return behind_rows(a) * a->H * 4; }
 static int64_t band_rows(const stg_relattn_args* a) { return a->Tq > 0 && a->Tk > 0 ? (int64_t)grid_tiles(a->max_k, a->Tk, (int64_t)a->S * a->Hkv) * a->S : 0; }
 
 extern "C" int64_t stg_relattn_bwd_ws_floats(const stg_relattn_args* a, int want_table) {
     if (a == nullptr || a->S < 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv != 0 || a->D <= 0 || a->Tq < 0 || a->Tk < 0 || a->num_buckets <= 0 || a->far <= 0) return -1;
-    int64_t n = (int64_t)2 * a->H * a->Tq + big_words(a) + split_floats(a);
+    int64_t n = (int64_t)2 * a->H * a->Tq + seen_words(a) + split_floats(a);
     if (want_table) n += a->H * (behind_rows(a) * 2 + band_rows(a) * a->num_buckets);
     return n > 0 ? n : 1;
 }
@@ -1543,9 +1553,9 @@ extern "C" int stg_relattn_bwd(const stg_relattn_args* a, const void* dO, int64_
     p.pk = ws;
     p.delta = ws + split_floats(a);
     p.fix = p.delta + (int64_t)a->H * a->Tq;
-    p.big = reinterpret_cast<uint32_t*>(p.fix + (int64_t)a->H * a->Tq);
+    p.seen = reinterpret_cast<uint32_t*>(p.fix + (int64_t)a->H * a->Tq);
     p.qtiles = a->Tq > 0 ? grid_tiles(a->max_q, a->Tq, (int64_t)a->S * a->H) : 0;
-    float* behind = p.fix + (int64_t)a->H * a->Tq + big_words(a);
+    float* behind = p.fix + (int64_t)a->H * a->Tq + seen_words(a);
     float* band = behind + behind_rows(a) * a->H * 2;
     p.part = dtable ? behind : nullptr;
     if (a->Tq > 0) { const int e = run_dq(p, a->D, a->max_q, st); if (e) return e; }

@@ -1,0 +1,53 @@
+"""Rows at the edges of the ragged attention: sequences with one visible key."""
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import seq_ref as R
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _cu(lens, dev):
+    c = [0]
+    for n in lens:
+        c.append(c[-1] + n)
+    return torch.tensor(c, dtype=torch.int32, device=dev)
+
+
+def _rn(gpu, seed):
+    g = torch.Generator(device=gpu)
+    g.manual_seed(seed)
+    return lambda *s, dtype=BF16: torch.randn(*s, generator=g, device=gpu, dtype=F32).to(dtype)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_one_visible_key_of_many(stg, gpu, causal, D):
+    """A mask that leaves one key of a long sequence, in its first tile of 64 or a later one, or none: the softmax is constant and dq, dk and dtable are zero."""
+    from stgcma import kernels as K
+    lens, shown, H, Hkv = [200, 90, 65, 130, 300], (130, 200 + 3, 290 + 64, 485 + 299), 4, 2
+    n, rn = sum(lens), _rn(gpu, 810)
+    q, k, v, do, table = rn(n, H * D), rn(n, Hkv * D), rn(n, Hkv * D), rn(n, H * D), rn(32, H, dtype=F32)
+    mask = torch.zeros(n, dtype=torch.bool, device=gpu)
+    mask[list(shown)] = True                                  # (the fourth sequence shows nothing)
+    geom = K.RelGeom(H, D, kv_heads=Hkv, causal=causal, device=gpu)
+    cu = _cu(lens, gpu)
+    ref = R.attention(q, k, v, table, lens, lens, H, Hkv, D, 32, 128, causal, D ** -0.5, mask, do)
+    o, lse = K.relattn_fwd(geom, q, k, v, table, cu, key_mask=mask)
+    R.within(o, ref["o"], "o")
+    for want_table in (True, False):
+        dq, dk, dv, dt = K.relattn_bwd(geom, q, k, v, table, cu, None, o, lse, do, key_mask=mask, want_table=want_table)
+        assert not dq.any() and not dk.any() and (dt is None or not dt.any())
+        R.within(dv, ref["dv"], "dv", 1e-6)
+    mask[131] = True                                          # two visible keys: gradients again
+    ref = R.attention(q, k, v, table, lens, lens, H, Hkv, D, 32, 128, causal, D ** -0.5, mask, do)
+    o, lse = K.relattn_fwd(geom, q, k, v, table, cu, key_mask=mask)
+    got = K.relattn_bwd(geom, q, k, v, table, cu, None, o, lse, do, key_mask=mask)
+    for name, t in zip(("dq", "dk", "dv", "dtable"), got):
+        R.within(t, ref[name], name, 1e-6)
+    assert bool(got[0][131:200].any()) and bool(got[1][130:132].any()) and not got[0][200:].any()
