@@ -654,7 +654,8 @@ int stg_bn_bwd(const void* x, const void* dy, const float* mean, const float* rs
  *   -far .. far (key position - query position; larger distances share the ends); without `causal` the last buckets of the two sides are
  *   num_buckets / 2 - 1 (keys before the query) and num_buckets - 1, with it num_buckets - 1; far <= 2048.
  *   lse fp32 [H, Tq] (natural logarithm; may be NULL in a forward without backward).
- *   Rows behind the last sequence are left as they were, or zeroed when zero_tail != 0 (by the backward too, in dQ, dK and dV).
+ *   Rows behind the last sequence are left as they were (zero_tail 0), or zero in O and -inf in lse (1; by the backward zero in dQ, dK and dV), or -inf in lse
+ *   alone (2; the backward leaves them).
  */
 typedef struct {
     const void* Q; int64_t ldq;

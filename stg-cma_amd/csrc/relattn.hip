@@ -24,6 +24,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int PAD = 96;               // a 64 x 32 tile that touches distance +-(far - 1) reaches at most 94 beyond it
 
+constexpr int TAIL_LSE = 2;           // zero_tail: the forward clears the rows of lse alone, the backward nothing
 struct RP {
     const bf16_t* Q; int64_t ldq;
     const bf16_t* K; int64_t ldk;
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
     if (w.s == a.S) {                                       // the slice that clears the rows behind the last sequence
         const int64_t from = tail_start(a.cu_q, a.S, a.Tq);
         const int step = a.tiles * NTHR, off = w.tile * NTHR + tid;
-        zero_rows(a.O, a.ldo, from, a.Tq, h * D, D, step, off);
+        if (a.zero_tail != TAIL_LSE) zero_rows(a.O, a.ldo, from, a.Tq, h * D, D, step, off);
         if (a.lse) for (int64_t i = from + off; i < a.Tq; i += step) a.lse[(int64_t)h * a.Tq + i] = -INFINITY;
         return;
     }
@@ -1375,7 +1376,7 @@ RP make_rp(const stg_relattn_args* a) {
     p.O = (bf16_t*)a->O; p.ldo = a->ldo;
     p.lse = a->lse;
     p.cu_q = a->cu_q; p.cu_k = a->cu_k; p.kmask = (const uint8_t*)a->key_mask;
-    p.Tq = a->Tq; p.Tk = a->Tk; p.S = a->S; p.H = a->H; p.Hkv = a->Hkv; p.causal = a->causal != 0; p.zero_tail = a->zero_tail != 0;
+    p.Tq = a->Tq; p.Tk = a->Tk; p.S = a->S; p.H = a->H; p.Hkv = a->Hkv; p.causal = a->causal != 0; p.zero_tail = a->zero_tail == TAIL_LSE ? TAIL_LSE : a->zero_tail != 0;
     p.table = a->table; p.plan = a->plan; p.NB = a->num_buckets; p.far = a->far;
     p.hsplit = 1;
     p.scale = a->scale; p.scale2 = a->scale * LOG2E; p.inv_scale = 1.0f / a->scale;
@@ -1549,6 +1550,7 @@ extern "C" int stg_relattn_bwd(const stg_relattn_args* a, const void* dO, int64_
     RP p = make_rp(a);
     p.dO = (const bf16_t*)dO; p.lddo = lddo; p.dQ = (bf16_t*)dQ; p.lddq = lddq;
     p.dK = (bf16_t*)dK; p.lddk = lddk; p.dV = (bf16_t*)dV; p.lddv = lddv;
+    p.zero_tail = p.zero_tail == 1;
     p.hsplit = head_split(a);
     p.pk = ws;
     p.delta = ws + split_floats(a);

@@ -2254,7 +2254,7 @@ def relattn_fwd(g, q, k, v, table, cu_q, cu_k=None, *, max_q=None, max_k=None, k
     [S + 1] on the device: sequence s owns rows cu[s] .. cu[s + 1] - 1 (cu_k = None: cu_q); max_q / max_k: the longest sequences, known on the host
     (they size the launch; without them the whole tensor is assumed).  key_mask bool [Tk]: False hides a key.  The last query of a sequence stands
     at its last key.  Returns (o bf16 [Tq, H * D], lse fp32 [H, Tq] or None).  Rows behind the last sequence are zero in a fresh output and left alone in `out`,
-    which must not overlap the inputs."""
+    which must not overlap the inputs; lse is -inf there."""
     return _relattn_fwd(g, q, k, v, table, cu_q, cu_k, max_q, max_k, key_mask, out, want_lse)[:2]
 
 
@@ -2262,7 +2262,7 @@ def _relattn_fwd(g, q, k, v, table, cu_q, cu_k, max_q, max_k, key_mask, out, wan
     o = torch.empty((q.shape[0], g.H * g.D), dtype=BF16, device=q.device) if out is None else out
     lse = torch.empty((g.H, q.shape[0]), dtype=F32, device=q.device) if want_lse else None
     a = _rel_fill(g, q, k, v, o, lse, table, cu_q, cu_k, max_q, max_k, key_mask)
-    a.zero_tail = int(out is None)
+    a.zero_tail = 1 if out is None else 2 * int(want_lse)     # (2: the rows of lse alone)
     _lib.check(_lib.lib().stg_relattn_fwd(C.byref(a), _stream()), "stg_relattn_fwd")
     return o, lse, a
 

@@ -1,4 +1,5 @@
-"""Rows at the edges of the ragged attention: sequences with one visible key."""
+"""Rows at the edges of the ragged attention: sequences with one visible key, rows behind the last sequence in a given
+output."""
 import os
 import sys
 
@@ -51,3 +52,22 @@ def test_one_visible_key_of_many(stg, gpu, causal, D):
     for name, t in zip(("dq", "dk", "dv", "dtable"), got):
         R.within(t, ref[name], name, 1e-6)
     assert bool(got[0][131:200].any()) and bool(got[1][130:132].any()) and not got[0][200:].any()
+
+
+def test_log_sums_behind_the_last_sequence(stg, gpu):
+    """lse is -inf behind the last sequence whether the output is fresh or given (whose own rows there stay as they were)."""
+    from stgcma import kernels as K
+    lens, tail, H, Hkv, D = [70, 33], 29, 4, 2, 64
+    n, rn = sum(lens) + tail, _rn(gpu, 820)
+    q, k, v, table = rn(n, H * D), rn(n, Hkv * D), rn(n, Hkv * D), rn(32, H, dtype=F32)
+    geom = K.RelGeom(H, D, kv_heads=Hkv, device=gpu)
+    cu = _cu(lens, gpu)
+    want, want_lse = K.relattn_fwd(geom, q, k, v, table, cu, max_q=70)
+    for hint in (70, None):
+        for _ in range(4):
+            junk = [torch.full((H, n), float("nan"), device=gpu) for _ in range(4)]
+            del junk                                          # a fresh lse finds these
+            mine = torch.full((n, H * D), 7.0, dtype=BF16, device=gpu)
+            o, lse = K.relattn_fwd(geom, q, k, v, table, cu, max_q=hint, out=mine)
+            assert torch.equal(lse, want_lse) and bool((lse[:, 103:] == -float("inf")).all())
+            assert torch.equal(o[:103], want[:103]) and bool((o[103:] == 7.0).all())
