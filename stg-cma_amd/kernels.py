@@ -2188,12 +2188,17 @@ class RelGeom:
         return p
 
 
+def _rel_ld(t):
+    """Leading dimension of a row tensor; a single row has none, whatever stride its view carries."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def _rel_chk(t, name, dtype, cols, dev, rows=None):
     _chk2d(t, name, dtype, cols, rows)
     if t.device != dev:
         raise RuntimeError(f"{name}: on {t.device}, expected {dev}")
-    if _ld(t) % 8 or t.data_ptr() % 16:
-        raise RuntimeError(f"{name}: rows must start 16-byte aligned (leading dimension {_ld(t)}, a multiple of 8)")
+    if _rel_ld(t) % 8 or t.data_ptr() % 16:
+        raise RuntimeError(f"{name}: rows must start 16-byte aligned (leading dimension {_rel_ld(t)}, a multiple of 8)")
 
 
 def _rel_rows(t, name, dtype, cols, dev, rows=None):
@@ -2206,7 +2211,7 @@ def _rel_rows(t, name, dtype, cols, dev, rows=None):
         if one == 1 and ld >= cols and not ld % 8 and not t.data_ptr() % 16:
             return ld
     _rel_chk(t, name, dtype, cols, dev, rows)
-    return _ld(t)
+    return _rel_ld(t)
 
 
 def _rel_int32(t, name, n, dev):
@@ -2289,7 +2294,7 @@ def _relattn_bwd(a, dev, do, want_table):
     ref = C.byref(a)
     n = lib.stg_relattn_bwd_ws_floats(ref, int(want_table))
     ws = torch.empty((max(n, 1),), dtype=F32, device=dev)
-    _lib.check(lib.stg_relattn_bwd(ref, _p(do), _ld(do), dq.data_ptr(), hd, dk.data_ptr(), kd, dv.data_ptr(), kd, dtable.data_ptr() if want_table else None,
+    _lib.check(lib.stg_relattn_bwd(ref, _p(do), _rel_ld(do), dq.data_ptr(), hd, dk.data_ptr(), kd, dv.data_ptr(), kd, dtable.data_ptr() if want_table else None,
                                    ws.data_ptr(), n, _stream()), "stg_relattn_bwd")
     return dq, dk, dv, dtable
 
@@ -2318,8 +2323,8 @@ def relattn_decode(g, q, k_cache, v_cache, table, lens, out=None):
         return out
     _rel_int32(lens, "lens", S, dev)
     many = S > 1
-    a = _lib.RelAttnDecodeArgs(_p(q), _ld(q), k_cache.data_ptr(), k_cache.stride(1) if cap > 1 else kd, k_cache.stride(0) if many else 0,
-                               v_cache.data_ptr(), v_cache.stride(1) if cap > 1 else kd, v_cache.stride(0) if many else 0, out.data_ptr(), _ld(out),
+    a = _lib.RelAttnDecodeArgs(_p(q), _rel_ld(q), k_cache.data_ptr(), k_cache.stride(1) if cap > 1 else kd, k_cache.stride(0) if many else 0,
+                               v_cache.data_ptr(), v_cache.stride(1) if cap > 1 else kd, v_cache.stride(0) if many else 0, out.data_ptr(), _rel_ld(out),
                                lens.data_ptr(), S, cap, g.H, g.Hkv, g.D, g.scale, g.causal, table.data_ptr(), g.plan(dev).data_ptr(), g.num_buckets, g.far)
     lib = _lib.lib()
     n = lib.stg_relattn_decode_ws_floats(S, cap, g.H, g.Hkv, g.D)
@@ -2453,6 +2458,6 @@ def _norm_join_bwd(a, dev, dtype, dy, dx_new, weights, gate, want_params, want_g
         nws = lib.stg_norm_join_bwd_ws_floats(ref)
         ws = torch.empty((nws,), dtype=F32, device=dev)
     ptr = lambda t: None if t is None else t.data_ptr()
-    _lib.check(lib.stg_norm_join_bwd(ref, _p(dy), _ld(dy), ptr(dx_new), _ld(dx_new) if dx_new is not None else 0, dx.data_ptr(), Cw, dh.data_ptr(), Cw, ptr(dpar),
+    _lib.check(lib.stg_norm_join_bwd(ref, _p(dy), _rel_ld(dy), ptr(dx_new), _rel_ld(dx_new) if dx_new is not None else 0, dx.data_ptr(), Cw, dh.data_ptr(), Cw, ptr(dpar),
                                      ptr(dgate), ptr(ws), nws, _stream()), "stg_norm_join_bwd")
     return [dx, dh] + out

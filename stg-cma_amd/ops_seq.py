@@ -45,7 +45,7 @@ class RelAttentionFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         a = type(ctx.call).from_buffer_copy(ctx.call)
         a.Q, a.K, a.V, a.O = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr()
-        a.ldq, a.ldk, a.ldv, a.ldo = K._ld(q), K._ld(k), K._ld(v), K._ld(o)      # (hooks may have stored a dense copy)
+        a.ldq, a.ldk, a.ldv, a.ldo = K._rel_ld(q), K._rel_ld(k), K._rel_ld(v), K._rel_ld(o)      # (hooks may have stored a dense copy)
         a.lse, a.table, a.cu_q, a.plan = lse.data_ptr(), table.data_ptr(), cu_q.data_ptr(), plan.data_ptr()
         a.cu_k = a.cu_q if cu_k is None else cu_k.data_ptr()
         a.key_mask = None if key_mask is None else key_mask.data_ptr()
@@ -79,7 +79,7 @@ class NormJoinFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         a = type(ctx.call).from_buffer_copy(ctx.call)
         a.xo, a.h, a.stats, a.w1, a.w2 = x_new.data_ptr(), h.data_ptr(), stats.data_ptr(), post_w.data_ptr(), pre_w.data_ptr()
-        a.ldxo, a.ldh = K._ld(x_new), K._ld(h)
+        a.ldxo, a.ldh = K._rel_ld(x_new), K._rel_ld(h)
         if gate is not None:
             a.gate = gate.data_ptr()
         if post_b is not None:

@@ -1,5 +1,5 @@
 """Rows at the edges of the ragged attention: sequences with one visible key, rows behind the last sequence in a given
-output."""
+output, single rows of wide buffers."""
 import os
 import sys
 
@@ -71,3 +71,25 @@ def test_log_sums_behind_the_last_sequence(stg, gpu):
             o, lse = K.relattn_fwd(geom, q, k, v, table, cu, max_q=hint, out=mine)
             assert torch.equal(lse, want_lse) and bool((lse[:, 103:] == -float("inf")).all())
             assert torch.equal(o[:103], want[:103]) and bool((o[103:] == 7.0).all())
+
+
+def test_single_rows_of_wide_buffers(stg, gpu):
+    """One row has no leading dimension to be misaligned: a row cut out of a buffer of any width goes through forward, backward and the single-token form."""
+    from stgcma import kernels as K, ops_seq
+    H, D = 4, 64
+    rn = _rn(gpu, 830)
+    big = rn(1, 3 * H * D + 5)
+    q, k, v = (big[:, i * H * D:(i + 1) * H * D] for i in range(3))
+    do, table = rn(1, H * D + 3)[:, :H * D], rn(32, H, dtype=F32)
+    geom = K.RelGeom(H, D, device=gpu)
+    cu = _cu([1], gpu)
+    dense = [t.contiguous().clone() for t in (q, k, v)]
+    outs = []
+    for a in ([q, k, v], dense):
+        leaf = [t.detach().requires_grad_(True) for t in a + [table]]
+        o = ops_seq.rel_attention(*leaf, geom, cu)
+        outs.append((o.detach(),) + torch.autograd.grad(o, leaf, do))
+        o, lse = K.relattn_fwd(geom, *a, table, cu)
+        outs[-1] += (o, lse) + K.relattn_bwd(geom, *a, table, cu, None, o, lse, do)
+        outs[-1] += (K.relattn_decode(geom, a[0], a[1][None], a[2][None], table, torch.ones(1, dtype=torch.int32, device=gpu)),)
+    assert all(torch.equal(x, y) for x, y in zip(*outs))
