@@ -2361,9 +2361,10 @@ def _norm_join_args(x, x_new, h, y, gate, weights, kind, alpha, eps, rows_per_gr
         ptrs.append(p)
     gk = rpg = 0
     if gate is not None:
-        if gate.device != dev or gate.dtype is not F32 or not gate.is_contiguous() or gate.data_ptr() % 16:
-            raise RuntimeError(f"gate: expected a contiguous, 16-byte aligned fp32 tensor on {dev}")
         sh = gate.shape
+        one = len(sh) == 0 or tuple(sh) == (1,)               # (read as one value: any element of a buffer)
+        if gate.device != dev or gate.dtype is not F32 or not gate.is_contiguous() or (gate.data_ptr() % 16 and not one):
+            raise RuntimeError(f"gate: expected a contiguous, 16-byte aligned fp32 tensor on {dev}")
         if len(sh) == 2:
             if not rows_per_group or int(rows_per_group) < 1:
                 raise RuntimeError("norm_join: a gate by row groups needs rows_per_group")
@@ -2371,7 +2372,7 @@ def _norm_join_args(x, x_new, h, y, gate, weights, kind, alpha, eps, rows_per_gr
             if tuple(sh) != (-(-R // rpg), Cw):
                 raise RuntimeError(f"gate: expected [{-(-R // rpg)}, {Cw}], got {tuple(sh)}")
             rpg = min(rpg, max(R, 1))
-        elif len(sh) == 0 or tuple(sh) == (1,):
+        elif one:
             gk = 1
         elif tuple(sh) == (Cw,):
             gk = 2
