@@ -423,9 +423,9 @@ __global__ void __launch_bounds__(256) norm_join_few_kernel(const float* in, flo
     const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (col >= cols) return;
     const float* p = in + (int64_t)blockIdx.y * n * cols + col;
-    float t = 0.f;
+    double t = 0.0;
     for (int i = 0; i < n; ++i) t += p[(int64_t)i * cols];
-    out[(int64_t)blockIdx.y * cols + col] = t;
+    out[(int64_t)blockIdx.y * cols + col] = (float)t;
 }
 
 bool bad16(const void* p) { return ((uintptr_t)p & 15) != 0; }
