@@ -716,7 +716,7 @@ int stg_norm_join_fwd(const stg_norm_join_args* a, void* stream);
 /* dy bf16 (gradient of y), dxo (gradient of xo from its other readers, x_dtype, or NULL = 0) -> dx (x_dtype), dh (bf16), and, unless NULL,
  * dparams: fp32, dw1 [C], db1 [C] (if b1), dw2 [C], db2 [C] (if b2), dgate [C] (gate_kind 2) or one value (gate_kind 1), one after the other and
  * padded to a multiple of 4; dgate_groups: fp32, the gate's gradient of gate_kind 3.  `a`: the forward's arguments (x and y are not read).  ws: fp32
- * scratch of stg_norm_join_bwd_ws_floats(a) floats.  stg_norm_join_param_floats(a): floats of dparams before the padding. */
+ * scratch of stg_norm_join_bwd_ws_floats(a) floats.  stg_norm_join_param_floats(a): floats of dparams, padding included (all of them are written). */
 int64_t stg_norm_join_param_floats(const stg_norm_join_args* a);
 int64_t stg_norm_join_bwd_ws_floats(const stg_norm_join_args* a);
 int stg_norm_join_bwd(const stg_norm_join_args* a, const void* dy, int64_t lddy, const void* dxo, int64_t lddxo, void* dx, int64_t lddx,

@@ -543,7 +543,7 @@ extern "C" int stg_norm_join_fwd(const stg_norm_join_args* a, void* stream) {
     return a->x_dtype == STG_F32 ? launch_fwd<float>(p, (hipStream_t)stream) : launch_fwd<bf16_t>(p, (hipStream_t)stream);
 }
 
-extern "C" int64_t stg_norm_join_param_floats(const stg_norm_join_args* a) { return a == nullptr ? -1 : part_cols(make(a)); }
+extern "C" int64_t stg_norm_join_param_floats(const stg_norm_join_args* a) { return a == nullptr ? -1 : part_pitch(make(a)); }
 
 extern "C" int64_t stg_norm_join_bwd_ws_floats(const stg_norm_join_args* a) {
     if (a == nullptr || a->rows < 0 || a->C <= 0 || (a->gate_kind == 3 && a->rows_per_group <= 0)) return -1;

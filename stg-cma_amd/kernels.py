@@ -2444,10 +2444,9 @@ def _norm_join_bwd(a, dev, dtype, dy, dx_new, weights, gate, want_params, want_g
         if gk in (1, 2):
             which.append(4)
             sizes.append(1 if gk == 1 else Cw)
-        n = sum(sizes)
-        if n % 4:
-            sizes.append(4 - n % 4)
-            n += 4 - n % 4
+        n = lib.stg_norm_join_param_floats(ref)
+        if n > sum(sizes):
+            sizes.append(n - sum(sizes))                      # the padding
         dpar = torch.empty((n,), dtype=F32, device=dev)
         for i, t in zip(which, dpar.split(sizes)):
             out[i] = t
