@@ -1,5 +1,5 @@
-"""Rows at the edges of the ragged attention: sequences with one visible key, rows behind the last sequence in a given
-output, single rows of wide buffers."""
+"""Rows at the edges of the ragged attention: sequences with one visible key, rows behind the last sequence in a given output, single rows of wide
+buffers, and query heads of a shared key / value head in fewer parts than heads."""
 import os
 import sys
 
@@ -93,3 +93,27 @@ def test_single_rows_of_wide_buffers(stg, gpu):
         outs[-1] += (o, lse) + K.relattn_bwd(geom, *a, table, cu, None, o, lse, do)
         outs[-1] += (K.relattn_decode(geom, a[0], a[1][None], a[2][None], table, torch.ones(1, dtype=torch.int32, device=gpu)),)
     assert all(torch.equal(x, y) for x, y in zip(*outs))
+
+
+@pytest.mark.parametrize("H,Hkv,D,causal,S,rows", [(32, 8, 32, True, 52, 43), (48, 8, 32, False, 45, 20), (16, 4, 128, False, 50, 60), (32, 8, 64, True, 45, 64)])
+def test_heads_of_a_group_in_a_few_parts(stg, gpu, H, Hkv, D, causal, S, rows):
+    """dK / dV of a shared key / value head whose query heads go to more than one block and fewer than one block each."""
+    from stgcma import kernels as K
+    from stgcma import _lib
+    import ctypes as C
+    g = torch.Generator().manual_seed(5)
+    lens = (rows + torch.randint(-9, 10, (S,), generator=g)).tolist()
+    n, rn = sum(lens), _rn(gpu, 840 + H)
+    q, k, v, do, table = rn(n, H * D), rn(n, Hkv * D), rn(n, Hkv * D), rn(n, H * D), rn(4, H, dtype=F32)
+    geom = K.RelGeom(H, D, kv_heads=Hkv, num_buckets=4, max_distance=10, causal=causal, device=gpu)
+    cu = _cu(lens, gpu)
+    ref = R.attention(q, k, v, table, lens, lens, H, Hkv, D, 4, 10, causal, D ** -0.5, None, do)
+    o, lse = K.relattn_fwd(geom, q, k, v, table, cu, max_q=max(lens))
+    a = K._rel_fill(geom, q, k, v, o, lse, table, cu, None, max(lens), None, None)
+    parts = _lib.lib().stg_relattn_bwd_ws_floats(C.byref(a), 0) // (2 * n * Hkv * D)       # the parts' share of the workspace
+    assert 1 < parts < H // Hkv, parts
+    for name, t in zip(("dq", "dk", "dv", "dtable"), K.relattn_bwd(geom, q, k, v, table, cu, None, o, lse, do, max_q=max(lens))):
+        R.within(t, ref[name], name, 1e-6)
+    ref = R.attention(q, k, v, table, lens, lens, H, Hkv, D, 4, 10, causal, D ** -0.5, None, do, table_grad=False)
+    for name, t in zip(("dq", "dk", "dv"), K.relattn_bwd(geom, q, k, v, table, cu, None, o, lse, do, max_q=max(lens), want_table=False)):
+        R.within(t, ref[name], name + " (frozen table)", 1e-6)
