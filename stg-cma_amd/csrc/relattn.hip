@@ -1137,7 +1137,7 @@ struct DP_ {
     const int32_t* lens;
     int S, cap, H, Hkv;
     const float* table; const int32_t* plan;
-    int NB, far, causal;
+    int NB, far;
     float scale2, inv_scale;
     int chunk, nsplit;
     float* po;                        // [S, nsplit, H, D] partial outputs (normalised by their own sum)
@@ -1152,7 +1152,7 @@ struct DP_ {
 template <int D>
 __global__ void __launch_bounds__(256, 2) relattn_decode_kernel(DP_ a) {
     constexpr int KS = D / 16, DT = D / 32, DP = D + 8, ROWP = D / 8, PER = 2 * 32 * ROWP / 64, TILE = 32 * DP;
-    extern __shared__ __attribute__((aligned(16))) bf16_t smem[];       // per wave {K, V} x [32][DP]; then bias [far + 1][32]: see host
+    extern __shared__ __attribute__((aligned(16))) bf16_t smem[];       // per wave {K, V} x [32][DP]; then the table's columns [NB][32]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // (wave-uniform for the compiler too)
     const int r = lane & 31, hh = lane >> 5;
     const int rep = a.H / a.Hkv, ncg = (rep + 31) / 32;
@@ -1596,7 +1596,7 @@ extern "C" int stg_relattn_decode(const stg_relattn_decode_args* a, float* ws, i
     p.V = (const bf16_t*)a->V; p.ldv = a->ldv; p.bsv = a->bsv;
     p.O = (bf16_t*)a->O; p.ldo = a->ldo;
     p.lens = a->lens; p.S = a->S; p.cap = a->cap; p.H = a->H; p.Hkv = a->Hkv;
-    p.table = a->table; p.plan = a->plan; p.NB = a->num_buckets; p.far = a->far; p.causal = a->causal != 0;
+    p.table = a->table; p.plan = a->plan; p.NB = a->num_buckets; p.far = a->far;
     p.scale2 = a->scale * LOG2E; p.inv_scale = 1.0f / a->scale;
     const int cap1 = a->cap > 0 ? a->cap : 1;
     p.chunk = decode_chunk(a->S, a->Hkv, a->H / a->Hkv, cap1);
