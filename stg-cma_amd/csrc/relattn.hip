@@ -244,17 +244,24 @@ __device__ __forceinline__ uint64_t key_bits(const RP& a, const Seq& z, int byte
     return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
 }
 // A sequence in which at most one key is visible: a row's only probability is one and dS is zero, not what its terms' roundings leave of them.  Asked where the
-// first 64 keys show at most one (`few`), and ends at the second visible key.
+// first 64 keys show at most one (`few`); ends at the second visible key, four loads in flight (a mask may hide a long beginning).
 __device__ __forceinline__ bool few(uint64_t bits) { return (bits & (bits - 1)) == 0; }
 __device__ __forceinline__ bool lone_key(const RP& a, const Seq& z, int lane) {
     if (z.nk <= 1) return true;
     if (a.kmask == nullptr) return false;
     bool one = false;
 #pragma unroll 1
-    for (int kb = 0; kb < z.nk; kb += 64) {
-        const uint64_t b = key_bits(a, z, key_load(a, z, kb, lane), kb, lane);
-        if (!few(b) || (b != 0 && one)) return false;
-        one = one || b != 0;
+    for (int64_t k0 = 0; k0 < z.nk; k0 += 256) {
+        const int kb = (int)k0;
+        int byte[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) byte[i] = key_load(a, z, kb + 64 * i, lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint64_t b = key_bits(a, z, byte[i], kb + 64 * i, lane);
+            if (!few(b) || (b != 0 && one)) return false;
+            one = one || b != 0;
+        }
     }
     return true;
 }

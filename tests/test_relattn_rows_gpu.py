@@ -117,3 +117,22 @@ def test_heads_of_a_group_in_a_few_parts(stg, gpu, H, Hkv, D, causal, S, rows):
     ref = R.attention(q, k, v, table, lens, lens, H, Hkv, D, 4, 10, causal, D ** -0.5, None, do, table_grad=False)
     for name, t in zip(("dq", "dk", "dv"), K.relattn_bwd(geom, q, k, v, table, cu, None, o, lse, do, max_q=max(lens), want_table=False)):
         R.within(t, ref[name], name + " (frozen table)", 1e-6)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shown", [(10, 290), (0, 64), (63, 599), (255, 256), (511, 513), (598, 599)])
+def test_two_visible_keys_anywhere(stg, gpu, causal, shown):
+    """Two keys of 600, near each other or far apart: no constant softmax."""
+    from stgcma import kernels as K
+    n, H, Hkv, D, rn = 600, 2, 1, 64, _rn(gpu, 850)
+    q, k, v, do, table = rn(n, H * D), rn(n, Hkv * D), rn(n, Hkv * D), rn(n, H * D), rn(32, H, dtype=F32)
+    mask = torch.zeros(n, dtype=torch.bool, device=gpu)
+    mask[list(shown)] = True
+    geom = K.RelGeom(H, D, kv_heads=Hkv, causal=causal, device=gpu)
+    cu = _cu([n], gpu)
+    ref = R.attention(q, k, v, table, [n], [n], H, Hkv, D, 32, 128, causal, D ** -0.5, mask, do)
+    o, lse = K.relattn_fwd(geom, q, k, v, table, cu, key_mask=mask)
+    got = K.relattn_bwd(geom, q, k, v, table, cu, None, o, lse, do, key_mask=mask)
+    for name, t in zip(("dq", "dk", "dv", "dtable"), got):
+        R.within(t, ref[name], name, 1e-6)
+    assert bool(got[0][shown[1]:].any())
