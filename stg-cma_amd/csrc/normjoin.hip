@@ -5,7 +5,7 @@
 // stays under it.  The gradients of the weights and the gate are column sums over all rows: every block keeps its columns' sums in registers
 // over its share of the rows and leaves ONE partial row, added up in a fixed order by a second kernel -- no atomics, repeatable bit for bit.
 // x' is rounded to the stream's type before the second norm reads it, so that the backward, which reads the stored x', sees the same values.
-// 62720 x 512, fp32 stream: 75 us forward (5.1 TB/s), 121 us backward (4.8 TB/s), a plain copy on the same card 4.75; 16384 x 4096, bf16 stream: 100 us forward
+// 62720 x 512, fp32 stream: 75 us forward (5.1 TB/s), 122 us backward (4.7 TB/s), plain copies of 256 MiB .. 8 GiB on such a card 5.4 .. 4.7; 16384 x 4096, bf16 stream: 100 us forward
 // (5.4 TB/s).
 #include <math.h>
 #include "common.h"

@@ -173,7 +173,8 @@ template <int D, int NTHR> struct StageC {
     static constexpr int PER = 2 * HALF;
     static constexpr int STEP = NTHR % ROWP == 0 ? NTHR / ROWP : 0;     // rows between a thread's pieces, 0: not one number
     static constexpr int NOFF = STEP ? 1 : HALF;
-    static constexpr int DP = D + 8;                         // padded pitch: conflict-free for row-wise and transposed reads
+    static constexpr int DP = D + 8;                         // padded pitch: conflict-free for row-wise reads; transposed ones conflict two-way at 64, four-way at 128
+                                                             // (10 % and 25 % as many conflict cycles as busy ones in the forward)
     static constexpr int TILE = 64 * DP;
     static_assert(64 * ROWP % NTHR == 0, "every thread moves the same number of pieces");
 };
@@ -409,8 +410,8 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
                 for (int reg = 2; reg < 15; ++reg) mr = fmax3(mr, sA[reg], sB[reg + 1]);
                 mr = fmax2(mr, sA[15]);
                 mr = half_max(mr) + far;
-                // The reference follows the maximum only once some query's maximum is 2^8 above it (a probability is then below 2^8 and keeps its bits):
-                // following at once, half of the tiles of a few thousand keys rescale.
+                // The reference follows the maximum only once some query's maximum is 2^8 above it (a probability is then below 2^8 and keeps its bits; a
+                // published idea): following at once, half of the tiles of a few thousand keys rescale.
                 if (__builtin_amdgcn_ballot_w64(mr * a.scale2 > m + 8.f) != 0) {
                     const float mx = fmax2(m, mr * a.scale2);
                     const float alpha = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mx);
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : 2) relattn_fwd_kernel(R
 // the exact delta.  Each block leaves its sums in its own row of `part`, added up in a fixed order by relattn_dtable_kernel.
 // dQ and dK lose little by the rounded delta where many keys share a row; where a wave's queries see no more than one tile of keys, a first
 // pass over the tile (already in LDS) takes the exact one.
-// Bound like the forward (35 % of the cycles in the matrix units): 1.79 ms = 0.92 PFLOP/s without the table's gradient (16384 x 16 x 64), 2.06 ms with it; 0.40 / 0.44 ms (the documents).
+// Bound like the forward (35 % of the cycles in the matrix units): 1.76 ms = 0.93 PFLOP/s without the table's gradient (16384 x 16 x 64), 2.00 ms with it; 0.39 / 0.42 ms (the documents).
 // lse is one fp32 number: beyond 2^8 (in powers of two) its spacing leaves more than 2^-16 of a probability, at 1e6 five percent, at 1e8 nothing of log2(sum).
 // Rows that far out sum their recomputed probabilities and divide by the sum: dQ (linear in P) at its end, dK / dV through RP::fix, a second term of the
 // row's score.  Two sums, because the kernels round a score differently: here q.k joins the bias (as in the forward), there bias - lse.  Without
@@ -806,7 +807,7 @@ __global__ void __launch_bounds__(256) relattn_dtable_kernel(const float* band, 
 // and the odd waves: waves two apart touch distances 64 apart, and a barrier lies between two steps, so no addition meets another and
 // the order is fixed.  After each head the arrays fold into the buckets, a row of `part` per block.  (A kernel of its own for the band that computed
 // scores and dS again took 60 us where this adds 35 us, 32 clips of 131 .. 490 x 12 x 64; LDS additions per element 340 us.)
-// 2.23 ms = 0.98 PFLOP/s without the table's gradient (16384 x 16 x 64), 2.51 ms with it (distances up to 800); 0.64 / 0.73 ms (the documents, whose 490
+// 2.17 ms = 1.01 PFLOP/s without the table's gradient (16384 x 16 x 64), 2.41 ms with it (distances up to 800); 0.65 / 0.75 ms (the documents, whose 492
 // registers leave one wave per SIMD: the walk waits for its own LDS reads.  Two waves per SIMD spilled, 2.6 ms, or, as eight waves with the keys in LDS
 // and half a tile's queries each, read a quarter more from LDS: the whole backward 1.19 ms against 1.07 without the table).
 constexpr int STATS = 2 * (5 * 64 + 4);           // 5 x 64 floats and the waves' votes, in bf16 elements
